@@ -2,7 +2,10 @@
 reference gets from vLLM's paged attention behind siirl/engine/rollout/vllm_rollout/vllm_rollout_spmd.py:261-416).
 
 Cache layout (one tensor for all layers): ``[layers, num_blocks, 2, Hkv, 64, D]`` bf16; ``block_table`` is
-``int32 [B, max_blocks]`` (-1 = unused).  The CPU path keeps the same layout and uses plain indexing."""
+``int32 [B, max_blocks]`` (-1 = unused).  The CPU path keeps the same layout and uses plain indexing.
+
+In the place of a layer's cache every function here takes a :class:`~siirl_b200.ops.kv_cache8.Cache8`, too: codes of 8 bits
+with a scale for each block and head."""
 from __future__ import annotations
 
 import ctypes
@@ -12,7 +15,9 @@ from typing import Optional
 
 import torch
 
+from . import kv_cache8
 from . import lib as _lib
+from .kv_cache8 import Cache8
 
 BLOCK = 64
 
@@ -26,6 +31,9 @@ def kv_append(qkv: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
               cache_layer: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int) -> None:
     """Write the k and v parts of every row of ``qkv`` ([T, (Hq+2Hkv)*D]) to ``cache_layer`` at
     ``(sequence seq_ids[t], position positions[t])``."""
+    if isinstance(cache_layer, Cache8):
+        kv_cache8.append(qkv, None, seq_ids, positions, block_table, cache_layer, n_heads, n_kv_heads, head_dim)
+        return
     T = qkv.shape[0]
     if qkv.is_cuda:
         L = _lib.get_lib()
@@ -51,6 +59,9 @@ def rope_kv_append(qkv: torch.Tensor, rope_positions: torch.Tensor, cos_tab: tor
     """Inference-only fusion of RoPE and cache append: rotates the q and k heads of ``qkv`` IN PLACE and writes the
     rotated k and the v heads to the cache (one kernel on CUDA).  Returns ``qkv``.  On CUDA ``qkv`` may be the partial sums
     ``[S, T, width]`` of :func:`siirl_b200.ops.dense.linear_slabs`, which are added up with ``bias`` on the way."""
+    if isinstance(cache_layer, Cache8):
+        return kv_cache8.append(qkv, (rope_positions, cos_tab, sin_tab, mrope_section), seq_ids, cache_positions, block_table,
+                                cache_layer, n_heads, n_kv_heads, head_dim, bias)
     slabs = None
     if qkv.dim() == 3:
         slabs = qkv
@@ -79,6 +90,9 @@ def rope_kv_append(qkv: torch.Tensor, rope_positions: torch.Tensor, cos_tab: tor
 
 def kv_copy_blocks(cache_layer: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     if src.numel() == 0:
+        return
+    if isinstance(cache_layer, Cache8):
+        kv_cache8.copy_blocks(cache_layer, src, dst)
         return
     if cache_layer.is_cuda:
         L = _lib.get_lib()
@@ -121,6 +135,8 @@ def decode_attention(q_rows: torch.Tensor, cache_layer: torch.Tensor, seq_lens: 
     """One query token per sequence against its cached context.  ``q_rows`` is ``[B, >= Hq*D]`` with the q heads in
     the first ``Hq*D`` columns (a packed qkv row works); ``seq_lens[b]`` counts the current token.  Returns
     ``[B, Hq*D]``."""
+    if isinstance(cache_layer, Cache8):
+        return kv_cache8.decode_attention(q_rows, cache_layer, seq_lens, block_table, n_heads, n_kv_heads, head_dim, scale, out)
     B = q_rows.shape[0]
     scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
     if out is None:
@@ -169,6 +185,8 @@ def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, sl
     the paged cache into one packed buffer, the packed-attention kernel computes only the query tiles that contain
     chunk rows, and the chunk rows of the result are returned ``[sum(chunk_lens), Hq*D]``."""
     from .attention import SeqInfo, attention_packed
+    if isinstance(cache_layer, Cache8):
+        kv_cache8.check_chunks(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads, head_dim)
     dev = qkv.device
     qw, kw = n_heads * head_dim, n_kv_heads * head_dim
     totals = [int(p) + int(c) for p, c in zip(prefix_lens, chunk_lens)]
@@ -177,7 +195,10 @@ def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, sl
     for p_, c_, t_, slot in zip(prefix_lens, chunk_lens, totals, slots):
         nb = (t_ + BLOCK - 1) // BLOCK
         blks = block_table[int(slot), :nb].long()
-        kv = cache_layer.index_select(0, blks)                      # [nb, 2, Hkv, 64, D]
+        if isinstance(cache_layer, Cache8):
+            kv = cache_layer.dequantize(blks, qkv.dtype)
+        else:
+            kv = cache_layer.index_select(0, blks)                  # [nb, 2, Hkv, 64, D]
         k = kv[:, 0].permute(0, 2, 1, 3).reshape(nb * BLOCK, kw)[:t_]
         v = kv[:, 1].permute(0, 2, 1, 3).reshape(nb * BLOCK, kw)[:t_]
         full[row:row + t_, qw:qw + kw] = k

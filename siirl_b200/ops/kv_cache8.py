@@ -1,0 +1,231 @@
+"""Paged key / value cache in 8 bits with a scale for each block of tokens and head.
+
+:class:`Cache8` stands where the functions of :mod:`siirl_b200.ops.kv_cache` take the cache of a layer (``rope_kv_append``,
+``kv_append``, ``decode_attention``, ``prefill_attention_with_prefix``, ``kv_copy_blocks``); those call what is here.  It holds
+``codes [num_blocks, 2, Hkv, 64, D]`` (e4m3; keys, then values) and ``scales [num_blocks, 2, Hkv]`` (fp32): a cached value is
+code times scale, half the bytes of the bf16 cache.
+
+Appending keeps each scale at the smallest power of two (at least 2^-126) with which every finite value that its block and
+head have met fits e4m3's range, ``|x| <= 448 * scale``.  New values are rounded once, from the rotated 32-bit ones, to the
+nearest code; infinities become +-448 times the scale, NaN stays NaN.  Where new rows raise a scale, the block's other rows are
+rounded to it.  A row at offset 0 of a block starts it anew: rows that the call does not write become zeros.  Rows of one call
+that lie in the same block have to follow one another; where one place is named twice, its last row counts."""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import lib as _lib
+
+BLOCK = 64
+LARGEST = 448.0             # of e4m3
+HEAD_DIMS = (64, 128)       # of the kernels; the CPU statements take any
+
+
+class Cache8(NamedTuple):
+    """Cache of one layer: a cached value is ``codes`` times the block's and head's scale in ``scales``."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def zeros(cls, num_blocks: int, n_kv_heads: int, head_dim: int, device=None) -> "Cache8":
+        return cls(torch.zeros(num_blocks, 2, n_kv_heads, BLOCK, head_dim, dtype=torch.uint8,
+                               device=device).view(torch.float8_e4m3fn),
+                   torch.zeros(num_blocks, 2, n_kv_heads, dtype=torch.float32, device=device))
+
+    def dequantize(self, blocks: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Values ``[len(blocks), 2, Hkv, 64, D]`` of some blocks; exact in bf16, too."""
+        codes = self.codes.view(torch.uint8)[blocks].view(torch.float8_e4m3fn)
+        return (codes.float() * self.scales[blocks][..., None, None]).to(dtype)
+
+
+def block_bytes(n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of one block of one layer, scales included."""
+    return 2 * n_kv_heads * (BLOCK * head_dim + 4)
+
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(f"8-bit cache: {what}")
+
+
+def _check(cache: Cache8, n_heads: int, n_kv_heads: int, head_dim: int, rows: torch.Tensor, *ints: torch.Tensor) -> None:
+    codes, scales = cache
+    _require(codes.dtype == torch.float8_e4m3fn and scales.dtype == torch.float32, "codes are float8_e4m3fn, scales float32")
+    _require(codes.dim() == 5 and tuple(codes.shape[1:]) == (2, n_kv_heads, BLOCK, head_dim),
+             f"codes are [blocks, 2, {n_kv_heads}, {BLOCK}, {head_dim}], got {tuple(codes.shape)}")
+    _require(scales.shape == codes.shape[:3], f"scales are {tuple(codes.shape[:3])}, got {tuple(scales.shape)}")
+    _require(codes.is_contiguous() and scales.is_contiguous(), "codes and scales are contiguous")
+    _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} query heads on {n_kv_heads} kv heads")
+    dev = rows.device
+    _require(codes.device == dev and scales.device == dev, "cache and rows are on one device")
+    for t in ints:
+        _require(t.dtype == torch.int32 and t.device == dev and t.is_contiguous(),
+                 "lengths, ids, positions and block tables are contiguous int32 tensors on the rows' device")
+    if rows.is_cuda:
+        _require(head_dim in HEAD_DIMS, f"the kernels take head widths {HEAD_DIMS}, not {head_dim}")
+        _require(n_heads // n_kv_heads <= 32, f"at most 32 query heads share a kv head, not {n_heads // n_kv_heads}")
+        _require(codes.data_ptr() % 16 == 0, "codes start on a 16-byte boundary")
+
+
+def _device(t: torch.Tensor):
+    """Makes the tensor's device current where it is not."""
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+# ---- appending ----------------------------------------------------------------------------------
+def _scale_of(amax: torch.Tensor) -> torch.Tensor:
+    half, exp = torch.frexp(amax)       # amax = half * 2^exp, 448 = 0.875 * 2^9
+    exp = torch.where(half == 0, torch.full_like(exp, -126), (exp - 9 + (half > 0.875)).clamp(min=-126))
+    return torch.ldexp(torch.ones_like(amax), exp)
+
+
+def _append_cpu(kv: torch.Tensor, seq_ids, positions, block_table, cache: Cache8) -> None:
+    """``kv [T, 2, Hkv, D]`` in fp32, rotated."""
+    codes, scales = cache
+    sequences, width = block_table.shape
+    ok = (seq_ids >= 0) & (seq_ids < sequences) & (positions >= 0) & (positions < width * BLOCK)
+    kv, seq_ids, positions = kv[ok], seq_ids[ok].long(), positions[ok].long()
+    blk = block_table[seq_ids, positions // BLOCK].long()
+    ok = (blk >= 0) & (blk < codes.shape[0])
+    kv, blk, off = kv[ok], blk[ok], positions[ok] % BLOCK
+    top = kv.abs()
+    top = torch.where(torch.isfinite(top), top, torch.zeros_like(top)).amax(-1)
+    for b in blk.unique().tolist():
+        rows = (blk == b).nonzero()[:, 0]
+        at = off[rows]
+        anew = bool((at == 0).any())
+        kept = torch.zeros_like(scales[b]) if anew else scales[b]
+        scale = torch.maximum(kept, _scale_of(top[rows].amax(0)))
+        values = torch.zeros(codes.shape[1:]) if anew else codes[b].float() * (kept / scale)[..., None, None]
+        for r, o in zip(rows.tolist(), at.tolist()):
+            values[:, :, o] = kv[r] / scale[..., None]
+        codes[b] = values.clamp(-LARGEST, LARGEST).to(codes.dtype)
+        scales[b] = scale
+
+
+def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tensor, block_table: torch.Tensor,
+           cache: Cache8, n_heads: int, n_kv_heads: int, head_dim: int, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Appends the k and v heads of ``qkv [T, (Hq + 2 Hkv) * D]`` to the cache.  ``rope`` (``positions [T] or [3, T], cos, sin,
+    mrope_section``, or None): rotates the q and k heads in place first.  ``qkv [S, T, width]``: partial sums, whose sum with
+    ``bias`` is rotated and returned as bf16 rows."""
+    slabs = qkv if qkv.dim() == 3 else None
+    T, width = qkv.shape[-2:]
+    _require(width == (n_heads + 2 * n_kv_heads) * head_dim, f"rows are {(n_heads + 2 * n_kv_heads) * head_dim} wide, got {width}")
+    _require(seq_ids.shape == (T,) and positions.shape == (T,), f"one sequence and position for each of {T} rows")
+    _check(cache, n_heads, n_kv_heads, head_dim, qkv, seq_ids, positions, block_table)
+    if slabs is not None:
+        _require(slabs.dtype == torch.float32 and slabs.is_contiguous() and slabs.shape[0] > 0, "partial sums are contiguous float32")
+        _require(bias is None or bias.numel() == width and bias.is_contiguous() and bias.device == qkv.device and
+                 bias.dtype == torch.bfloat16, f"the bias is {width} bf16 numbers")
+    else:
+        _require(bias is None, "a bias is added to partial sums only")
+    pos = cos = sin = None
+    s0 = s1 = rows = 0
+    if rope is not None:
+        pos, cos, sin, section = rope
+        pos = pos.to(torch.int32).contiguous()
+        rows = 1 if pos.dim() == 1 else pos.shape[0]
+        _require(pos.shape[-1] == T and rows in (1, 3) and pos.device == qkv.device, f"rope positions are [{T}] or [3, {T}]")
+        for t in (cos, sin):
+            _require(t.dtype == torch.float32 and t.is_contiguous() and t.shape[-1] == head_dim // 2 and t.device == qkv.device,
+                     f"cos and sin are contiguous float32 tables of width {head_dim // 2}")
+        if rows == 3:
+            s0, s1 = section[0], section[0] + section[1]
+    if not qkv.is_cuda:
+        if slabs is not None:
+            qkv = slabs.sum(0) + (0 if bias is None else bias.float())
+        x = qkv.float()
+        if rope is not None:
+            from . import reference as ref
+            n = (n_heads + n_kv_heads) * head_dim
+            turned = ref.rope(x[:, :n].reshape(T, n_heads + n_kv_heads, head_dim), pos if rows == 3 else pos.reshape(-1), cos,
+                              sin, rope[3])
+            x = torch.cat([turned.reshape(T, n), x[:, n:]], 1)
+        _append_cpu(x[:, n_heads * head_dim:].reshape(T, 2, n_kv_heads, head_dim), seq_ids, positions, block_table, cache)
+        if slabs is not None:
+            return x.to(torch.bfloat16)
+        if rope is not None:
+            qkv.copy_(x)
+        return qkv
+    if slabs is not None:
+        qkv = torch.empty(T, width, dtype=torch.bfloat16, device=slabs.device)
+    _require(qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0,
+             "rows are bf16 numbers next to one another, from an even one on")
+    with _device(qkv):
+        _lib.check(_lib.get_lib().sb_kv8_append(
+            _lib.ptr(qkv), qkv.stride(0), _lib.ptr(slabs), ctypes.c_longlong(qkv.numel()), 0 if slabs is None else slabs.shape[0],
+            _lib.ptr(bias), _lib.ptr(pos), rows, s0, s1, 0 if cos is None else cos.shape[0], _lib.ptr(cos), _lib.ptr(sin),
+            _lib.ptr(seq_ids), _lib.ptr(positions), _lib.ptr(block_table), block_table.shape[0], block_table.shape[1],
+            _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0], T, n_heads, n_kv_heads, head_dim,
+            _lib.stream()), "sb_kv8_append")
+    return qkv
+
+
+def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Blocks ``src[i]`` with their scales to ``dst[i]``."""
+    codes, scales = cache
+    if not codes.is_cuda:
+        codes.view(torch.uint8)[dst.long()] = codes.view(torch.uint8)[src.long()]
+        scales[dst.long()] = scales[src.long()]
+        return
+    _check(cache, codes.shape[2], codes.shape[2], codes.shape[4], codes, src, dst)
+    _require(src.shape == dst.shape and src.dim() == 1, "as many sources as destinations")
+    with _device(codes):
+        _lib.check(_lib.get_lib().sb_kv8_copy_blocks(
+            _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(src), _lib.ptr(dst), src.numel(), codes.shape[0], 2 * codes.shape[2],
+            ctypes.c_longlong(codes[0].numel()), _lib.stream()), "sb_kv8_copy_blocks")
+
+
+# ---- single tokens ------------------------------------------------------------------------------
+def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor, block_table: torch.Tensor, n_heads: int,
+                     n_kv_heads: int, head_dim: int, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`siirl_b200.ops.kv_cache.decode_attention` on an 8-bit cache."""
+    B, width = q_rows.shape[0], n_heads * head_dim
+    scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
+    _check(cache, n_heads, n_kv_heads, head_dim, q_rows, seq_lens, block_table)
+    _require(q_rows.dim() == 2 and q_rows.shape[1] >= width and q_rows.stride(1) == 1, f"query rows are at least {width} wide")
+    _require(seq_lens.shape == (B,) and block_table.dim() == 2 and block_table.shape[0] >= B, f"a length and a row of the table for each of {B} rows")
+    if out is None:
+        out = torch.empty(B, width, dtype=q_rows.dtype, device=q_rows.device)
+    _require(out.shape == (B, width) and out.is_contiguous() and out.dtype == q_rows.dtype and out.device == q_rows.device,
+             f"the output is a contiguous [{B}, {width}] of the rows' type")
+    if not q_rows.is_cuda:
+        rep = n_heads // n_kv_heads
+        out.zero_()
+        for b in range(B):
+            n = int(seq_lens[b])
+            if n == 0:
+                continue
+            x = cache.dequantize(block_table[b, :(n + BLOCK - 1) // BLOCK].long())
+            k, v = (x[:, i].permute(1, 0, 2, 3).reshape(n_kv_heads, -1, head_dim)[:, :n].repeat_interleave(rep, 0) for i in (0, 1))
+            s = torch.einsum("hd,hnd->hn", q_rows[b, :width].reshape(n_heads, head_dim).float(), k) * scale
+            out[b] = torch.einsum("hn,hnd->hd", torch.softmax(s, -1), v).reshape(-1).to(out.dtype)
+        return out
+    _require(q_rows.dtype == torch.bfloat16, "query rows are bf16")
+    with _device(q_rows):
+        _lib.check(_lib.get_lib().sb_kv8_decode(
+            _lib.ptr(q_rows), q_rows.stride(0), _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0],
+            _lib.ptr(seq_lens), _lib.ptr(block_table), block_table.shape[1], _lib.ptr(out), B, n_heads, n_kv_heads, head_dim,
+            ctypes.c_float(scale), _lib.stream()), "sb_kv8_decode")
+    return out
+
+
+# ---- chunks of prompts --------------------------------------------------------------------------
+def check_chunks(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Cache8, block_table: torch.Tensor, n_heads: int,
+                 n_kv_heads: int, head_dim: int) -> None:
+    """Refuses chunks that the cache or the rows cannot hold."""
+    _check(cache, n_heads, n_kv_heads, head_dim, qkv, block_table)
+    _require(len(chunk_lens) == len(prefix_lens) == len(slots), "a chunk, a prefix and a slot for each sequence")
+    rows, width = sum(chunk_lens), (n_heads + 2 * n_kv_heads) * head_dim
+    _require(qkv.dim() == 2 and qkv.shape == (rows, width), f"{rows} rows of {width} numbers, got {tuple(qkv.shape)}")
+    for c, p, s in zip(chunk_lens, prefix_lens, slots):
+        _require(c >= 0 and p >= 0 and 0 <= s < block_table.shape[0] and c + p <= block_table.shape[1] * BLOCK,
+                 f"slot {s} of {block_table.shape[0]} with {p} + {c} tokens in {block_table.shape[1]} blocks")
+    if qkv.is_cuda:
+        _require(qkv.dtype == torch.bfloat16, "rows are bf16")

@@ -1,0 +1,317 @@
+"""Paged cache in 8 bits: the kernels against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import kv8_oracle as oracle
+from siirl_b200.ops import kv_cache as kvc
+from siirl_b200.ops import lib
+from siirl_b200.ops import reference as ref
+from siirl_b200.ops.kv_cache import Cache8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = 2.0 ** -8        # half a step of bf16, relative to the value
+
+
+def _random_cache(nb, hkv, d, spread=1.0):
+    """Codes over their whole range, scales of unlike blocks."""
+    codes = (torch.randn(nb, 2, hkv, 64, d) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = 2.0 ** torch.round(-7 + spread * torch.randn(nb, 2, hkv))
+    return Cache8(codes, scales)
+
+
+def _gpu(cache):
+    return Cache8(cache.codes.to(DEV), cache.scales.to(DEV))
+
+
+def _check_append(cache, rows, pos, section, seq, at, table, hq, hkv, d, slabs=0, bias=None, rope=True):
+    """One call on the GPU against the definition.  Bounds: a rotated value is a * c - b * s in 32 bits (three roundings of
+    2^-24 of |a| + |b|), sums of S partial sums add S + 1 more; bf16 rows half a step, codes half a step of e4m3."""
+    cos, sin = ref.rope_tables(d, 512, 1e4)
+    if rope is False:
+        cos = sin = None
+    g = _gpu(cache)
+    t = lambda x: None if x is None else x.to(DEV)  # noqa: E731
+    full = rows.double() if not slabs else rows.double().sum(0) + (0 if bias is None else bias.double())
+    dev_rows = t(rows)
+    if rope:
+        out = kvc.rope_kv_append(dev_rows, t(pos), t(cos), t(sin), section, t(seq), t(at), t(table), g, hq, hkv, d, t(bias))
+    else:
+        kvc.kv_append(dev_rows, t(seq), t(at), t(table), g, hq, hkv, d)
+        out = dev_rows
+    want, raw, codes, scales, tops = oracle.append(full, pos, cos, sin, section, seq, at, table, *cache, hq, hkv, d)
+    out = out.cpu().double()
+    width = (hq + hkv) * d
+    reach = (rows.double().abs().sum(0) + (0 if bias is None else bias.double().abs())) if slabs else full.abs()
+    r = reach.view(len(reach), hq + 2 * hkv, 2, d // 2)
+    reach = (r + r.flip(2)).view_as(reach)
+    fine = torch.isfinite(want)
+    err = (3 + slabs + 1) * 2.0 ** -23 * reach if rope else torch.zeros_like(reach)     # without rotation: exact
+    assert bool(((out - want).abs() <= BF16 * want.abs() + err)[fine].all())
+    if not slabs:
+        assert torch.equal(out[:, width:][fine[:, width:]], full[:, width:][fine[:, width:]])
+    got_s = g.scales.cpu().double()
+    # the kernel's largest value may be off by its rounding: where the border lies within that, either scale is right
+    edge = torch.zeros_like(scales, dtype=torch.bool)
+    for i in (tops > 0).nonzero().tolist():
+        top = float(tops[tuple(i)])
+        edge[tuple(i)] = abs(math.remainder(math.log2(top / 448.0), 1.0)) < 2.0 ** -18
+    assert torch.equal(got_s[~edge], scales[~edge])
+    kept = torch.isnan(raw) & torch.isfinite(codes)
+    kept &= (got_s == scales)[..., None, None]
+    got = g.codes.cpu().double()
+    assert torch.equal(got[kept], codes[kept])
+    new = torch.isfinite(raw)
+    s = got_s[..., None, None].expand_as(raw)
+    bound = torch.maximum(2.0 ** -4 * raw.abs(), 2.0 ** -10 * s) + 2.0 ** -19 * (raw.abs().nan_to_num().amax(-1, keepdim=True) + s * 2.0 ** -9)
+    assert bool(((got * s - raw).abs() <= bound)[new].all())
+    inf = torch.isinf(raw)
+    assert bool((got[inf] == 448 * torch.sign(raw[inf])).all())
+    lib.check_status()
+    return g, out
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (3, 3, 128), (2, 1, 64)])
+@pytest.mark.parametrize("rows", [1, 7, 61])
+def test_append_single_rows(hq, hkv, d, rows):
+    """A decoding step: every sequence at its own place, first, inner and last rows of blocks, idle slots."""
+    nb, most = 2 * rows + 3, 3
+    cache = _random_cache(nb, hkv, d)
+    order = torch.randperm(nb).to(torch.int32)
+    table = torch.full((rows, most), -1, dtype=torch.int32)
+    table[:, :2] = order[:2 * rows].view(rows, 2)
+    at = torch.tensor([[0, 63, 64, 127, 1, 100, 30][i % 7] for i in range(rows)], dtype=torch.int32)
+    seq = torch.arange(rows, dtype=torch.int32)
+    if rows > 7:
+        seq[9], at[12], at[20] = -1, -1, 128     # idle, idle, no block
+    x = torch.randn(rows, (hq + 2 * hkv) * d) * torch.exp(2 * torch.randn(rows, 1))
+    _check_append(cache, x.bfloat16(), at.clamp(min=0) + 5, None, seq, at, table, hq, hkv, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d,slabs,bias", [(28, 4, 128, 3, True), (14, 2, 64, 1, False), (2, 2, 64, 5, True)])
+def test_append_partial_sums(hq, hkv, d, slabs, bias):
+    rows, width = 13, (hq + 2 * hkv) * d
+    cache = _random_cache(rows, hkv, d)
+    table = torch.arange(rows, dtype=torch.int32)[:, None].contiguous()
+    at = torch.randint(0, 64, (rows,), dtype=torch.int32)
+    b = torch.randn(width).bfloat16() if bias else None
+    _check_append(cache, torch.randn(slabs, rows, width), at, None, torch.arange(rows, dtype=torch.int32), at, table, hq, hkv, d,
+                  slabs, b)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (1, 1, 128)])
+@pytest.mark.parametrize("lens,starts", [((1, 2, 63, 64, 65, 200), (0, 0, 0, 0, 0, 0)), ((5, 130, 64, 1), (61, 30, 64, 63)),
+                                         ((300,), (1,))])
+def test_append_chunks(hq, hkv, d, lens, starts):
+    """Whole prompts and later chunks: blocks that begin, go on and end in the call; rows with positions of three axes."""
+    need = [(s + n + 63) // 64 for n, s in zip(lens, starts)]
+    cache = _random_cache(sum(need) + 2, hkv, d, 3.0)
+    table = torch.full((len(lens), max(need) + 1), -1, dtype=torch.int32)
+    order, a = torch.randperm(sum(need)).to(torch.int32), 0
+    for i, k in enumerate(need):
+        table[i, :k] = order[a:a + k]
+        a += k
+    seq = torch.repeat_interleave(torch.arange(len(lens), dtype=torch.int32), torch.tensor(lens))
+    at = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for n, s in zip(lens, starts)])
+    x = torch.randn(len(seq), (hq + 2 * hkv) * d) * torch.exp(torch.randn(len(seq), 1))
+    _check_append(cache, x.bfloat16(), at, None, seq, at, table, hq, hkv, d)
+    pos = torch.stack([at, at // 2, at // 3 + 7])
+    _check_append(cache, x.bfloat16(), pos, (d // 8, d // 4, d // 8), seq, at, table, hq, hkv, d)
+    _check_append(cache, x.bfloat16(), pos, None, seq, at, table, hq, hkv, d, rope=False)
+
+
+def test_append_odd_values_and_places_named_twice():
+    hq, hkv, d = 4, 2, 128
+    cache = _random_cache(4, hkv, d)
+    table = torch.tensor([[2, 0], [3, 1]], dtype=torch.int32)
+    seq = torch.tensor([0, 0, 0, 0, 1, 1], dtype=torch.int32)
+    at = torch.tensor([5, 6, 5, 70, 0, 9], dtype=torch.int32)
+    x = torch.randn(6, (hq + 2 * hkv) * d)
+    x[1, hq * d + 3], x[1, hq * d + 9], x[4, -1] = math.inf, -math.inf, math.nan
+    x[3, (hq + hkv) * d:] = 0
+    x[5, hq * d:] *= 1e30
+    x = x.bfloat16()
+    _check_append(cache, x, at, None, seq, at, table, hq, hkv, d, rope=False)
+
+
+def test_append_takes_rows_of_a_wider_buffer():
+    hq, hkv, d = 4, 2, 64
+    cache, table = _gpu(_random_cache(3, hkv, d)), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    cos, sin = (x.to(DEV) for x in ref.rope_tables(d, 64, 1e4))
+    wide = torch.randn(9, (hq + 2 * hkv) * d + 22, device=DEV).bfloat16()
+    rows, at = wide[:, 8:8 + (hq + 2 * hkv) * d], torch.arange(20, 29, dtype=torch.int32, device=DEV)
+    seq = torch.zeros(9, dtype=torch.int32, device=DEV)
+    other = Cache8(cache.codes.clone(), cache.scales.clone())
+    want = kvc.rope_kv_append(rows.contiguous(), at, cos, sin, None, seq, at, table, other, hq, hkv, d)
+    edges = wide[:, :8].clone(), wide[:, 8 + rows.shape[1]:].clone()
+    got = kvc.rope_kv_append(rows, at, cos, sin, None, seq, at, table, cache, hq, hkv, d)
+    assert torch.equal(got, want) and torch.equal(cache.codes.view(torch.uint8), other.codes.view(torch.uint8))
+    assert torch.equal(wide[:, :8], edges[0]) and torch.equal(wide[:, 8 + rows.shape[1]:], edges[1])
+
+
+def _decode(lens, hq, hkv, d, max_blocks, spread=1.0, q_scale=1.0, stride=0):
+    need = [(n + 63) // 64 for n in lens]
+    cache = _random_cache(sum(need) + 3, hkv, d, spread)
+    table = torch.full((len(lens), max_blocks), -1, dtype=torch.int32)
+    order, a = torch.randperm(sum(need) + 3).to(torch.int32), 0
+    for i, k in enumerate(need):
+        table[i, :k] = order[a:a + k]
+        a += k
+    q = (q_scale * torch.randn(len(lens), (hq + 2 * hkv) * d + stride)).bfloat16()
+    return cache, table, q, torch.tensor(lens, dtype=torch.int32)
+
+
+def _check_decode(cache, table, q, lens, hq, hkv, d, scale=None):
+    """Bounds: the output is rounded to bf16; weights carry at most 2^-11 of their value or 2^-18 of the largest weight (three e4m3
+    terms), scores 2^-22 sum |q k| and 2^-20 of themselves; sums of 32 bits over n tokens stay below that."""
+    g = _gpu(cache)
+    out = kvc.decode_attention(q.to(DEV), g, lens.to(DEV), table.to(DEV), hq, hkv, d, scale)
+    lib.check_status()
+    again = kvc.decode_attention(q.to(DEV), g, lens.to(DEV), table.to(DEV), hq, hkv, d, scale)
+    assert torch.equal(out, again)
+    for b, n in enumerate(lens.tolist()):
+        want, size = oracle.attention(q[b:b + 1, :hq * d], *cache, table[b, :-(-n // 64)].long(), [n], hq, hkv, d,
+                                      d ** -0.5 if scale is None else scale)
+        err = (out[b].cpu().double() - want[0]).abs()
+        assert bool((err <= BF16 * want[0].abs() + 2.0 ** -10 * size[0]).all()), (b, n, float((err / (size[0] + 1e-300)).max()))
+
+
+HEADS = [(28, 4, 128), (14, 2, 64), (4, 4, 128), (32, 1, 128), (9, 1, 64), (24, 2, 128)]
+
+
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("lens,width", [((1,), 1), ((64, 0, 65, 127, 128, 129), 4), ((2, 1000, 0, 513), 20), ((0, 0), 2)])
+def test_decode_attention(hq, hkv, d, lens, width):
+    _check_decode(*_decode(lens, hq, hkv, d, width), hq, hkv, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (32, 2, 128)])
+def test_decode_attention_of_many_and_long_sequences(hq, hkv, d):
+    _check_decode(*_decode([3000 - 41 * i if i % 5 else 0 for i in range(70)], hq, hkv, d, 50), hq, hkv, d)
+    _check_decode(*_decode([9001], hq, hkv, d, 150), hq, hkv, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (32, 2, 128)])
+def test_decode_attention_of_sharp_scores_and_unlike_scales(hq, hkv, d):
+    """Scores whose maximum moves from block to block, scales 2^12 apart, a scale given by the caller; values of zero."""
+    _check_decode(*_decode([700, 64, 1], hq, hkv, d, 20, 4.0, 8.0), hq, hkv, d)
+    _check_decode(*_decode([333, 90], hq, hkv, d, 20, 1.0, 0.3), hq, hkv, d, 1.0)
+    cache, table, q, lens = _decode([400, 130], hq, hkv, d, 8)
+    cache.codes.view(torch.uint8)[table[0, 3].long(), 1] = 0
+    cache.scales[table[0, 3].long(), 1] = 2.0 ** -126
+    cache.scales[table[1, 0].long(), 0] = 2.0 ** -126
+    _check_decode(cache, table, q, lens, hq, hkv, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (32, 2, 128)])
+def test_decode_attention_ignores_what_it_does_not_see(hq, hkv, d):
+    """NaN codes behind the last token, blocks of no sequence, idle slots with tables of anything."""
+    lens = [70, 0, 129, 1, 63]
+    cache, table, q, n = _decode(lens, hq, hkv, d, 4)
+    clean = kvc.decode_attention(q.to(DEV), _gpu(cache), n.to(DEV), table.to(DEV), hq, hkv, d)
+    codes = cache.codes.view(torch.uint8)
+    for b, k in enumerate(lens):
+        if k % 64:
+            codes[table[b, k // 64].long(), :, :, k % 64:] = 0x7f
+    used = torch.zeros(len(codes), dtype=torch.bool)
+    used[table[table >= 0].long()] = True
+    codes[~used] = 0xff
+    cache.scales[~used] = math.nan
+    table[1] = torch.tensor([10 ** 6, -7, 2 ** 31 - 1, 0])
+    got = kvc.decode_attention(q.to(DEV), _gpu(cache), n.to(DEV), table.to(DEV), hq, hkv, d)
+    assert torch.equal(got, clean)
+
+
+def test_decode_attention_of_strided_rows_on_another_stream_and_in_a_graph():
+    hq, hkv, d = 28, 4, 128
+    cache, table, q, n = _decode([300, 65, 0, 1500], hq, hkv, d, 30, stride=24)
+    g, q, n, table = _gpu(cache), q.to(DEV), n.to(DEV), table.to(DEV)
+    want = kvc.decode_attention(q.contiguous(), g, n, table, hq, hkv, d)
+    out = torch.full((4, hq * d), 7.0, device=DEV, dtype=torch.bfloat16)
+    assert kvc.decode_attention(q, g, n, table, hq, hkv, d, out=out) is out and torch.equal(out, want)
+    odd = torch.cat([q[:, :2], q], 1)[:, 2:]        # rows that start 4 bytes behind a boundary
+    assert torch.equal(kvc.decode_attention(odd, g, n, table, hq, hkv, d), want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = kvc.decode_attention(q, g, n, table, hq, hkv, d)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = kvc.decode_attention(q, g, n, table, hq, hkv, d)
+    n.copy_(torch.tensor([1, 64, 500, 0]))
+    graph.replay()
+    assert torch.equal(held[[0, 1, 3]], kvc.decode_attention(q, g, n, table, hq, hkv, d)[[0, 1, 3]])
+    lib.check_status()
+
+
+def _check_prefix(new, old, hq, hkv, d, spread=1.0, q_scale=1.0):
+    """Bounds: weights and output are rounded to 16 bits; see _check_decode for the rest."""
+    total = [a + b for a, b in zip(new, old)]
+    need = [(n + 63) // 64 for n in total]
+    cache = _random_cache(sum(need) + 2, hkv, d, spread)
+    n = len(new)
+    table = torch.full((n + 2, max(need) + 1), -1, dtype=torch.int32)
+    slots = [int(x) for x in torch.randperm(n + 2)[:n]]
+    order, a = torch.randperm(sum(need)).to(torch.int32), 0
+    for i, k in zip(slots, need):
+        table[i, :k] = order[a:a + k]
+        a += k
+    rows = (q_scale * torch.randn(sum(new), (hq + 2 * hkv) * d)).bfloat16()
+    out = kvc.prefill_attention_with_prefix(rows.to(DEV), new, old, slots, _gpu(cache), table.to(DEV), hq, hkv, d).cpu().double()
+    lib.check_status()
+    assert out.shape == (sum(new), hq * d)
+    at = 0
+    for i, a, o, k in zip(slots, new, old, need):
+        seen = [o + j + 1 for j in range(a)]
+        pick = sorted(set(list(range(min(a, 3))) + list(range(0, a, 37)) + [a - 1])) if a else []
+        want, size = oracle.attention(rows[[at + j for j in pick], :hq * d], *cache, table[i, :k].long(), [seen[j] for j in pick],
+                                      hq, hkv, d, d ** -0.5)
+        err = (out[[at + j for j in pick]] - want).abs()
+        assert bool((err <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size).all()), (a, o)
+        at += a
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (2, 2, 128), (4, 1, 64)])
+@pytest.mark.parametrize("new,old", [((1,), (64,)), ((9,), (130,)), ((64, 1, 200), (1, 700, 64)), ((128, 129), (128, 63)),
+                                     ((300, 5), (0, 1000)), ((257,), (255,))])
+def test_prefix_attention(hq, hkv, d, new, old):
+    _check_prefix(new, old, hq, hkv, d)
+
+
+def test_prefix_attention_of_sharp_scores_and_unlike_scales():
+    _check_prefix((100, 30), (200, 90), 28, 4, 128, 4.0, 8.0)
+    _check_prefix((100, 30), (200, 90), 14, 2, 64, 4.0, 8.0)
+
+
+def test_copied_blocks_bring_their_scales():
+    cache = _gpu(_random_cache(6, 1, 64))
+    idx = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    want = cache.dequantize(idx(1, 3).long())
+    rest = cache.dequantize(idx(1, 2, 3, 5).long())
+    kvc.kv_copy_blocks(cache, idx(1, 3, 2), idx(0, 4, 99))
+    assert torch.equal(cache.dequantize(idx(0, 4).long()), want)
+    assert torch.equal(cache.dequantize(idx(1, 2, 3, 5).long()), rest)
+
+
+def test_refusals():
+    hq, hkv, d = 4, 2, 64
+    cache = _gpu(_random_cache(4, hkv, d))
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    q = torch.randn(2, (hq + 2 * hkv) * d, device=DEV).bfloat16()
+    wide = Cache8.zeros(4, hkv, 96, DEV)
+    for call in (lambda: kvc.decode_attention(q.float(), cache, lens, table, hq, hkv, d),
+                 lambda: kvc.decode_attention(q, cache, lens.cpu(), table, hq, hkv, d),
+                 lambda: kvc.decode_attention(q, Cache8(cache.codes.cpu(), cache.scales), lens, table, hq, hkv, d),
+                 lambda: kvc.decode_attention(q, wide, lens, table, 2, hkv, 96),
+                 lambda: kvc.decode_attention(torch.zeros(2, 66 * d, device=DEV).bfloat16(), Cache8.zeros(4, 1, d, DEV), lens, table, 66, 1, d),
+                 lambda: kvc.kv_append(q.float(), lens, lens, table, cache, hq, hkv, d),
+                 lambda: kvc.prefill_attention_with_prefix(q.float(), [2], [3], [0], cache, table, hq, hkv, d),
+                 lambda: kvc.prefill_attention_with_prefix(q, [2], [127], [0], cache, table, hq, hkv, d),
+                 lambda: kvc.prefill_attention_with_prefix(q, [2], [3], [2], cache, table, hq, hkv, d),
+                 lambda: kvc.prefill_attention_with_prefix(q, [3], [3], [0], cache, table, hq, hkv, d)):
+        with pytest.raises(ValueError, match="8-bit cache"):
+            call()

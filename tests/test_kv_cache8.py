@@ -1,0 +1,135 @@
+"""Paged cache in 8 bits: definitions on the CPU, refusals, the rollout engine on it."""
+import math
+
+import pytest
+import torch
+
+import kv8_oracle as oracle
+from siirl_b200.ops import kv_cache as kvc
+from siirl_b200.ops import reference as ref
+from siirl_b200.ops.kv_cache import Cache8
+
+
+def _tables(d, n=600):
+    return ref.rope_tables(d, n, 1e4)
+
+
+def _append_cpu(rows, pos, cos, sin, section, seq, at, table, cache, hq, hkv, d):
+    out = kvc.rope_kv_append(rows.clone(), pos, cos, sin, section, seq, at, table, cache, hq, hkv, d)
+    return out
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 32), (4, 2, 64)])
+def test_append_follows_its_definition(hq, hkv, d):
+    """Fresh blocks, a block whose scale grows, one whose scale stays, rows of no sequence, a place named twice."""
+    cache = Cache8.zeros(7, hkv, d)
+    cos, sin = _tables(d)
+    table = torch.tensor([[3, 0, 5], [6, 2, -1]], dtype=torch.int32)
+    steps = [([0] * 70, list(range(70)), 1.0), ([1, 1], [0, 1], 1e-3), ([1], [2], 900.0), ([1, 0, -1, 1], [3, 70, 4, -1], 0.5),
+             ([0, 0], [71, 71], 3.0), ([1], [130], 1.0)]
+    for n, (seq, at, size) in enumerate(steps):
+        seq, at = torch.tensor(seq, dtype=torch.int32), torch.tensor(at, dtype=torch.int32)
+        rows = size * torch.randn(len(seq), (hq + 2 * hkv) * d)
+        pos = at.clamp(min=0) + 3
+        old = cache.codes.clone(), cache.scales.clone()
+        got = _append_cpu(rows, pos, cos, sin, None, seq, at, table, cache, hq, hkv, d)
+        want, raw, codes, scales, _ = oracle.append(rows, pos, cos, sin, None, seq, at, table, *old, hq, hkv, d)
+        assert torch.allclose(got.double(), want, rtol=2 ** -20, atol=2 ** -20 * size)
+        assert torch.equal(cache.scales.double(), scales), n
+        # old rows exactly; new ones to half a step of their code (2^-4 of the value, 2^-10 scales below 2^-6 of them)
+        kept = torch.isnan(raw)
+        assert torch.equal(cache.codes.double()[kept], codes[kept])
+        off = (cache.codes.double() * scales[..., None, None] - raw).abs()
+        bound = torch.maximum(2 ** -4 * raw.abs(), 2 ** -10 * scales[..., None, None].expand_as(raw)) * (1 + 2 ** -18)
+        assert bool((off <= bound)[~kept].all())
+
+
+def test_scales_are_the_smallest_powers_of_two_and_survive_odd_values():
+    cache = Cache8.zeros(2, 1, 32)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    seq = torch.zeros(1, dtype=torch.int32)
+    row = torch.zeros(1, 96)
+    for at, (top, want) in enumerate([(0.0, 2.0 ** -126), (1e-41, 2.0 ** -126), (448.0, 1.0), (448.0001, 2.0), (3.0e38, 2.0 ** 120)]):
+        row[0, 32:64] = 0
+        row[0, 40] = -top
+        kvc.kv_append(row, seq, torch.tensor([at], dtype=torch.int32), table, cache, 1, 1, 32)
+        assert float(cache.scales[0, 0, 0]) == want
+    cache = Cache8.zeros(2, 1, 32)
+    row[0, 32:64] = 3.0
+    row[0, 33], row[0, 34], row[0, 35] = math.inf, -math.inf, math.nan
+    kvc.kv_append(row, seq, torch.zeros(1, dtype=torch.int32), table, cache, 1, 1, 32)
+    got = cache.codes[0, 0, 0, 0].float()
+    scale = 2.0 ** -7         # 3 <= 448 * 2^-7
+    assert float(cache.scales[0, 0, 0]) == scale and got[1] == 448 and got[2] == -448 and math.isnan(got[3]) and got[0] * scale == 3
+    # the block begun anew holds nothing of that any more
+    row.fill_(1.0)
+    kvc.kv_append(row, seq, torch.zeros(1, dtype=torch.int32), table, cache, 1, 1, 32)
+    assert bool(torch.isfinite(cache.codes.float()).all())
+
+
+def test_dequantized_values_are_exact_in_bf16():
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    codes = torch.where(torch.isnan(codes.float()), torch.zeros(()), codes.float()).to(torch.float8_e4m3fn)
+    cache = Cache8(codes.repeat(4).view(1, 2, 1, 64, 8).contiguous(), torch.full((1, 2, 1), 2.0 ** -9))
+    blocks = torch.zeros(1, dtype=torch.int64)
+    assert torch.equal(cache.dequantize(blocks, torch.bfloat16).float(), cache.dequantize(blocks))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 2, 32), (6, 2, 64)])
+def test_attention_follows_its_definition(hq, hkv, d):
+    cache = Cache8((torch.randn(9, 2, hkv, 64, d) * 50).clamp(-400, 400).to(torch.float8_e4m3fn),
+                   2.0 ** torch.randint(-9, -4, (9, 2, hkv)).float())
+    table = torch.tensor([[0, 3, 5], [1, -1, -1], [2, 4, 8], [7, 6, -1]], dtype=torch.int32)
+    lens = torch.tensor([130, 0, 192, 65], dtype=torch.int32)
+    q = torch.randn(4, (hq + 2 * hkv) * d)
+    got = kvc.decode_attention(q, cache, lens, table, hq, hkv, d)
+    for b in range(4):
+        n = int(lens[b])
+        want, size = oracle.attention(q[b:b + 1, :hq * d], *cache, table[b, :-(-n // 64)].long(), [n], hq, hkv, d, d ** -0.5)
+        assert bool(((got[b] - want).abs() <= 1e-5 * size + 1e-30).all())
+    new, old = [2, 1, 64, 7], [120, 0, 128, 58]
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d)
+    got = kvc.prefill_attention_with_prefix(rows, new, old, [0, 1, 2, 3], cache, table, hq, hkv, d)
+    at = 0
+    for i, (a, o) in enumerate(zip(new, old)):
+        want, size = oracle.attention(rows[at:at + a, :hq * d], *cache, table[i, :-(-(a + o) // 64)].long(),
+                                      [o + j + 1 for j in range(a)], hq, hkv, d, d ** -0.5)
+        assert bool(((got[at:at + a] - want).abs() <= 1e-5 * size).all())
+        at += a
+
+
+def test_copied_blocks_bring_their_scales():
+    cache = Cache8.zeros(5, 2, 32)
+    cache.codes.view(torch.uint8).copy_(torch.randint(0, 120, cache.codes.shape))
+    cache.scales.copy_(2.0 ** torch.randint(-9, 9, cache.scales.shape))
+    want = cache.dequantize(torch.tensor([1, 3]))
+    kvc.kv_copy_blocks(cache, torch.tensor([1, 3], dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32))
+    assert torch.equal(cache.dequantize(torch.tensor([0, 4])), want)
+
+
+def test_refusals():
+    hq, hkv, d = 4, 2, 64
+    cache = Cache8.zeros(4, hkv, d)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    q = torch.randn(2, (hq + 2 * hkv) * d)
+    cos, sin = _tables(d)
+
+    def decode(q=q, cache=cache, lens=lens, table=table, hq=hq, hkv=hkv, d=d, out=None):
+        return kvc.decode_attention(q, cache, lens, table, hq, hkv, d, out=out)
+
+    def append(q=q, seq=lens, at=lens, cache=cache, cos=cos, pos=lens, bias=None):
+        return kvc.rope_kv_append(q, pos, cos, sin, None, seq, at, table, cache, hq, hkv, d, bias)
+    decode(), append(q.clone())
+    half = Cache8(cache.codes.to(torch.bfloat16), cache.scales)
+    for call in (lambda: decode(cache=half), lambda: decode(cache=Cache8(cache.codes, cache.scales[:3])),
+                 lambda: decode(cache=Cache8(cache.codes, cache.scales.half())), lambda: decode(hkv=1), lambda: decode(hq=3),
+                 lambda: decode(d=32), lambda: decode(lens=lens.long()), lambda: decode(lens=lens[:1]),
+                 lambda: decode(table=table.long()), lambda: decode(table=table.repeat(1, 2)[:, :2]), lambda: decode(q=q[:, :hq * d - 1]),
+                 lambda: decode(table=table[:1]), lambda: decode(q=q.t().contiguous().t()),
+                 lambda: decode(out=torch.empty(2, hq * d, dtype=torch.float16)), lambda: decode(out=torch.empty(3, hq * d)),
+                 lambda: append(q[:, :-1]), lambda: append(seq=lens[:1]), lambda: append(at=lens.long()),
+                 lambda: append(cos=cos[:, :-1]), lambda: append(cos=cos.double()), lambda: append(pos=lens[:1]),
+                 lambda: append(bias=torch.zeros(q.shape[1])), lambda: append(q.half()[None]),
+                 lambda: append(cache=Cache8(cache.codes.transpose(2, 3), cache.scales))):
+        with pytest.raises(ValueError, match="8-bit cache"):
+            call()
