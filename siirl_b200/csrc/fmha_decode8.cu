@@ -1,0 +1,814 @@
+// Single-token attention against a paged cache of e4m3 codes (kv_cache8.cu), on the 8-bit tensor cores.
+//
+// o = sum_t softmax(scale q . k_t)_t v_t with k_t = ks * code, v_t = vs * code, one ks and vs per cache block and head.  Both
+// products run on codes as they lie in the cache: nothing is converted on the way.  What meets the codes is split instead, into
+// e4m3 terms that are columns of one product and are added up afterwards:
+//   * a query row, divided by a power of two, into two terms, the second 16 times enlarged: 4 + 4 bits hold all that a bf16
+//     number has, down to 2^-22 of the row's largest;
+//   * a weight into three terms (each remainder 16 times enlarged): off by at most 2^-12 of itself or 2^-21 of the largest.
+// The block's scales go into the score and into the weight, in 32 bits.
+//
+// A tile is 128 rows of 128 bytes: two cache blocks at D = 128; at D = 64, where a row holds two tokens, four.
+//   S^T[row, (token of the row, term, head)] = K Q^T     A = the K tile, B = the terms of all query heads of a kv head
+//   O^T[byte of a row, (token of the row, term, head)] += V^T W^T    A = the V tile through an MN-major descriptor
+// The tile fills the 128 rows of the MMA whatever the number of heads, and shared memory is read once per product.  At D = 64
+// only the diagonal (token of the row) blocks of O^T mean something; the query terms of the other token's half are zeros.
+//
+// The tiles of all (sequence, kv head, group of at most 16 query heads) form one list, and every CTA of a persistent grid of
+// one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry; a piece that is not
+// the whole entry leaves a normalised partial result and its log-sum-exp in a workspace, two slots per CTA, and a small
+// kernel merges them.  The warps:
+//   0..3   soft-max, thread = row of the tile.  The weights' references are shared by the four: a vote per tile says whether
+//          one of them has to be raised (a weight above 2^8; a fresh one puts the largest weight at 2^3)
+//   4..7   output: O^T of a piece while the next piece's tiles are under way (O^T is double-buffered)
+//   8      producer: a ring of K and V tiles, ids and scales of the next 32 cache blocks of the list in registers
+//   9      MMA issuer: scores one tile ahead of the weighted sums
+//   10     query terms of the next piece
+//   11     zero rows of idle slots
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "launchers.h"
+
+namespace sb {
+
+constexpr int kQ8Rows = 1024;        // sequences of one launch
+constexpr int kQ8Smem = 227 * 1024;
+constexpr int kQ8MinTiles = 2;       // tiles of a range, where there are so few that not every SM gets as many
+constexpr float kQ8None = -3.0e38f;  // reference before anything has been seen
+
+__device__ __forceinline__ void umma_e4m3_ss_if(uint32_t leader, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// kind::f8f6f4 with e4m3 operands and fp32 accumulation
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int a_mn, int b_mn) {
+  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// largest of a warp
+__device__ __forceinline__ float redux_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// whether `any` is set in one of the 128 threads of the soft-max warps
+__device__ __forceinline__ bool vote_128(bool any) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)any)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+struct Decode8Params {
+  const __nv_bfloat16* q;   // [B, row_stride], q heads first
+  long long row_stride;
+  const float* scales;      // [num_blocks, 2, Hkv]
+  const int* seq_lens;      // [B]
+  const int* block_table;   // [B, max_blocks]
+  int num_blocks, max_blocks, B, Hq, Hkv, groups;
+  __nv_bfloat16* out;       // [B, Hq * D]
+  float* ws_o;              // [2 * grid][NR][D]
+  float* ws_lse;            // [2 * grid][NR]
+  int* ws_pre;              // [B + 1] tiles before each sequence, written by the first CTA
+  float scale_log2;
+  int* status;
+};
+
+// NR: query heads of a group (rows of a piece), 8 or 16
+template <int D, int NR>
+struct D8 {
+  static constexpr int PACK = 128 / D;             // tokens of a 128-byte row
+  static constexpr int RPB = 64 / PACK;            // rows of a cache block
+  static constexpr int BPT = 2 * PACK;             // cache blocks of a tile
+  static constexpr int TT = 64 * BPT;              // tokens of a tile
+  static constexpr int NS = PACK * 2 * NR;         // columns of S^T
+  static constexpr int NO = (PACK * 3 * NR + 15) / 16 * 16;   // columns of O^T: a legal N of the MMA
+  static constexpr int kQBytes = NS * 128, kPBytes = NO * 128, kStage = 32768;
+  static constexpr int kXBytes = PACK == 2 ? 64 * NR * 4 : 0; // the second tokens' share of a result
+  static constexpr int kFixed = 2 * kQBytes + 2 * kPBytes + kXBytes + (kQ8Rows + 1 + 32) * 4 + 4096;
+  static constexpr int kStages = (kQ8Smem - kFixed) / kStage < 6 ? (kQ8Smem - kFixed) / kStage : 6;
+  static constexpr int kQOff = kStages * kStage, kPOff = kQOff + 2 * kQBytes, kXOff = kPOff + 2 * kPBytes;
+  static constexpr int kScaleOff = kXOff + kXBytes;                    // [stages][BPT] {ks, log2 vs}
+  static constexpr int kRedOff = kScaleOff + kStages * BPT * 8;        // [4][NR] {max z, max z + log2 vs}
+  static constexpr int kStatOff = kRedOff + 4 * NR * 8;                // per O^T buffer: l [4][NR], m [NR], M [NR]
+  static constexpr int kFactorOff = kStatOff + 2 * 6 * NR * 4;         // per query buffer: factor of the scores [NR]
+  static constexpr int kBarOff = (kFactorOff + 2 * NR * 4 + 7) / 8 * 8;
+  static constexpr int kBars = 3 * kStages + 18;
+  static constexpr int kPreOff = kBarOff + kBars * 8 + 16;
+  static constexpr int kTotal = kPreOff + (kQ8Rows + 1 + 32) * 4;
+  static constexpr int kTmemS = 0, kTmemO = 2 * NS;                    // columns
+  static constexpr int kTmemCols = 2 * (NS + NO) <= 128 ? 128 : 2 * (NS + NO) <= 256 ? 256 : 512;
+};
+
+struct D8Piece {
+  int row, entry, t0, n, tiles;    // entry: kv head * groups + group
+  bool whole;
+};
+// the piece at list position `cur` of a range that ends at `end`; pre[b] = tiles of one entry of the sequences before b
+__device__ __forceinline__ D8Piece d8_piece(const int* pre, int B, int entries, int cur, int end) {
+  int lo = 0, hi = B;       // the last sequence that begins at or before cur (those without tiles have no width)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] * entries <= cur) lo = mid;
+    else hi = mid;
+  }
+  D8Piece q;
+  q.row = lo;
+  q.tiles = pre[lo + 1] - pre[lo];
+  const int at = cur - pre[lo] * entries;
+  q.entry = at / q.tiles;
+  q.t0 = at - q.entry * q.tiles;
+  q.n = min(q.tiles - q.t0, end - cur);
+  q.whole = q.n == q.tiles;
+  return q;
+}
+__device__ __forceinline__ int d8_tiles(const Decode8Params& p, int b, int tile_tokens) {
+  return (min(max(p.seq_lens[b], 0), p.max_blocks * 64) + tile_tokens - 1) / tile_tokens;
+}
+// ranges of the list, and the first position of one
+__device__ __forceinline__ int d8_ranges(int total, int grid) { return min(grid, max(1, total / kQ8MinTiles)); }
+__device__ __forceinline__ int d8_begin(int total, int cta, int ranges) { return (int)((long long)total * min(cta, ranges) / ranges); }
+
+template <int D, int NR>
+__global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_constant__ CUtensorMap map_c, Decode8Params p) {
+  using L = D8<D, NR>;
+  constexpr int PACK = L::PACK, NST = L::kStages, BPT = L::BPT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, (int)kStatusBadArgument);
+    return;
+  }
+  uint8_t *sQ = smem + L::kQOff, *sP = smem + L::kPOff;
+  float* s_x = reinterpret_cast<float*>(smem + L::kXOff);
+  float2* s_scale = reinterpret_cast<float2*>(smem + L::kScaleOff);
+  float2* s_red = reinterpret_cast<float2*>(smem + L::kRedOff);
+  float* s_stat = reinterpret_cast<float*>(smem + L::kStatOff);
+  float* s_factor = reinterpret_cast<float*>(smem + L::kFactorOff);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* v_full = k_full + NST;
+  uint64_t* kv_empty = v_full + NST;
+  uint64_t* q_full = kv_empty + NST;    // pairs
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_empty + 2;
+  uint64_t* p_empty = p_full + 2;
+  uint64_t* o_full = p_empty + 2;       // the piece's MMAs have completed
+  uint64_t* o_empty = o_full + 2;       // the output warps have read O^T and the statistics
+  uint64_t* x_full = o_empty + 2;       // second tokens' share
+  uint64_t* x_empty = x_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_empty + 1);
+  volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [2]: before the first, the second vote of a tile
+  int* s_pre = reinterpret_cast<int*>(smem + L::kPreOff);
+  int* s_tot = s_pre + kQ8Rows + 1;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int entries = p.Hkv * p.groups, rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups;
+  if (tid == 0) {
+    tma_prefetch_desc(&map_c);
+    for (int i = 0; i < 3 * NST; ++i) mbar_init(&k_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 5);     // the MMAs, the four soft-max warps
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&p_empty[i], 1);
+      mbar_init(&o_full[i], 5);      // the MMAs, the statistics of four warps
+      mbar_init(&o_empty[i], 4);
+    }
+    mbar_init(x_full, 2);
+    mbar_init(x_empty, 2);
+    s_fail[0] = s_fail[1] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
+  // rows of P that no head owns
+  for (int i = tid; i < 2 * L::kPBytes / 16; i += 384) reinterpret_cast<uint4*>(sP)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_sync();
+  // running sum of the sequences' tiles: chunks of 32 by warp, then their totals
+  const int chunks = (p.B + 31) / 32;
+  for (int c = warp; c < chunks; c += 12) {
+    const int b = c * 32 + lane;
+    int v = b < p.B ? d8_tiles(p, b, L::TT) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (b < p.B) s_pre[b + 1] = v;
+    if (lane == 31) s_tot[c] = v;
+  }
+  __syncthreads();
+  for (int c = warp; c < chunks; c += 12) {
+    int before = lane < c ? s_tot[lane] : 0;      // at most 32 chunks
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int b = c * 32 + lane;
+    if (b < p.B) s_pre[b + 1] += before;
+  }
+  if (tid == 0) s_pre[0] = 0;
+  __syncthreads();
+  const int total = s_pre[p.B] * entries, ranges = d8_ranges(total, gridDim.x);
+  const int begin = d8_begin(total, blockIdx.x, ranges), end = d8_begin(total, blockIdx.x + 1, ranges);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= p.B; i += 384) p.ws_pre[i] = s_pre[i];
+
+  if (warp == 8) {
+    // ------------------------------ producer ------------------------------
+    // lane i: cache block i % BPT of the tile i / BPT places on in the list
+    constexpr int kAhead = 32 / BPT;
+    auto find = [&](int at, int& entry) {      // block id, or -1
+      const int cur = at + lane / BPT;
+      entry = 0;
+      if (cur >= end) return -1;
+      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      entry = q.entry;
+      const int j = q.t0 * BPT + lane % BPT;
+      if (j * 64 >= min(p.seq_lens[q.row], p.max_blocks * 64)) return -1;
+      const int blk = p.block_table[(size_t)q.row * p.max_blocks + j];
+      return blk < p.num_blocks ? blk : -1;
+    };
+    auto scales = [&](int blk, int entry) {
+      if (blk < 0) return make_float2(0.f, 0.f);
+      const float* s = p.scales + (size_t)blk * 2 * p.Hkv + entry / p.groups;
+      return make_float2(s[0], s[p.Hkv]);
+    };
+    uint32_t tile_no = 0;
+    bool ok = true;
+    int entry, entry2 = 0, blk2 = -1;
+    int blk = find(begin, entry);
+    float2 sc = scales(blk, entry), sc2 = make_float2(0.f, 0.f);
+    for (int at = begin; at < end && ok; at += kAhead) {
+      const int n = min(kAhead, end - at);
+      blk2 = find(at + kAhead, entry2);
+      for (int k = 0; k < n; ++k, ++tile_no) {
+        if (k == n / 2) sc2 = scales(blk2, entry2);
+        const int stage = tile_no % NST;
+        if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((tile_no / NST) & 1) ^ 1, p.status, kStatusTimeoutProducer))) {
+          ok = false;
+          break;
+        }
+        const bool mine = lane / BPT == k, loads = mine && blk >= 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, loads)) * (uint32_t)(L::RPB * 128);
+        const int part = lane % BPT;
+        // a block that is not there: a scale that nothing else has
+        if (mine) s_scale[stage * BPT + part] = make_float2(sc.x, blk >= 0 ? log2f(sc.y) : INFINITY);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&k_full[stage], bytes);
+          mbar_arrive_expect_tx(&v_full[stage], bytes);
+        }
+        __syncwarp();
+        if (loads) {
+          uint8_t* dst = smem + stage * L::kStage + part * (L::RPB * 128);
+          const int row = (blk * 2 * p.Hkv + entry / p.groups) * L::RPB;
+          tma_load_2d(dst, &map_c, &k_full[stage], 0, row);
+          tma_load_2d(dst + 16384, &map_c, &v_full[stage], 0, row + p.Hkv * L::RPB);
+        }
+      }
+      blk = blk2; entry = entry2; sc = sc2;
+    }
+    if (!ok) {      // no copy may be in flight when shared memory is given back
+      const uint32_t first = tile_no > (uint32_t)NST ? tile_no - NST : 0;
+      for (uint32_t j = first; j < tile_no; ++j) {
+        mbar_wait(&k_full[j % NST], (j / NST) & 1, nullptr, 0);
+        mbar_wait(&v_full[j % NST], (j / NST) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------ MMA issuer (the whole warp, converged; one lane issues) ------------------------------
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    constexpr uint32_t idesc_s = umma_idesc_e4m3(128, L::NS, 0, 0), idesc_o = umma_idesc_e4m3(128, L::NO, 1, 0);
+    const uint64_t dk = umma_smem_desc(smem_u32(smem), 16, 1024), dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024);
+    const uint64_t dq = umma_smem_desc(smem_u32(sQ), 16, 1024), dp = umma_smem_desc(smem_u32(sP), 16, 1024);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool r = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma));
+      tc_fence_after();
+      return r;
+    };
+    auto tiles_at = [&](int cur) { return __shfl_sync(0xffffffffu, cur < end ? d8_piece(s_pre, p.B, entries, cur, end).n : 0, 0); };
+    // pieces and tiles left in them, of the scores and, one tile behind, of the weighted sums
+    uint32_t s_piece = 0, o_piece = 0;
+    int s_left = tiles_at(begin), o_left = s_left;
+    bool s_first = true, o_first = true;
+    for (int i = 0; i <= end - begin && ok; ++i) {
+      if (i < end - begin) {
+        const uint32_t b = i & 1, stage = i % NST, ib = s_piece & 1;
+        ok = (!s_first || wait(&q_full[ib], (s_piece >> 1) & 1)) && wait(&k_full[stage], (i / NST) & 1) &&
+             wait(&s_empty[b], ((i >> 1) & 1) ^ 1);
+        if (!ok) break;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_e4m3_ss_if(leader, tmem_base + L::kTmemS + b * L::NS, dk + stage * (L::kStage >> 4) + 2 * kk,
+                          dq + ib * (L::kQBytes >> 4) + 2 * kk, idesc_s, kk ? 1u : 0u);
+        umma_commit_if(leader, &s_full[b]);
+        s_first = --s_left == 0;
+        if (s_first) {
+          umma_commit_if(leader, &q_empty[ib]);
+          ++s_piece;
+          s_left = tiles_at(begin + i + 1);
+        }
+      }
+      if (i > 0) {
+        const int j = i - 1;
+        const uint32_t b = j & 1, stage = j % NST, ib = o_piece & 1;
+        ok = (!o_first || wait(&o_empty[ib], ((o_piece >> 1) & 1) ^ 1)) && wait(&v_full[stage], (j / NST) & 1) &&
+             wait(&p_full[b], (j >> 1) & 1);
+        if (!ok) break;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + ib * L::NO, dv + stage * (L::kStage >> 4) + 256 * kk,
+                          dp + b * (L::kPBytes >> 4) + 2 * kk, idesc_o, (!o_first || kk) ? 1u : 0u);
+        umma_commit_if(leader, &kv_empty[stage]);
+        umma_commit_if(leader, &p_empty[b]);
+        o_first = --o_left == 0;
+        if (o_first) {
+          umma_commit_if(leader, &o_full[ib]);
+          ++o_piece;
+          o_left = tiles_at(begin + i);
+        }
+      }
+    }
+  } else if (warp == 10) {
+    // ------------------------------ query terms ------------------------------
+    constexpr int E = D / 32;       // elements of a lane
+    uint32_t piece_no = 0;
+    for (int cur = begin; cur < end; ++piece_no) {
+      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      cur += q.n;
+      const int ib = piece_no & 1, group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
+      const __nv_bfloat16* src = p.q + (size_t)q.row * p.row_stride + (size_t)(q.entry / p.groups * rep + group * per_group) * D + lane * E;
+      float x[NR][E];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = r < left ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + (size_t)r * D + e)) : make_float2(0.f, 0.f);
+          x[r][e] = v.x;
+          x[r][e + 1] = v.y;
+        }
+      if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[ib], ((piece_no >> 1) & 1) ^ 1, p.status, kStatusTimeoutProducer))) break;
+      uint8_t* dst = sQ + ib * L::kQBytes;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[r][e]));
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) odd |= !(fabsf(x[r][e]) <= 3.402823466e38f);
+        odd = __any_sync(0xffffffffu, odd);
+        top = redux_max(top);
+        // a power of two s with top / s in (224, 448] (or s = 2^-126)
+        const uint32_t u = __float_as_uint(top);
+        const int ex = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+        const float s = __uint_as_float((uint32_t)max(ex, 1) << 23), inv = 1.f / s;
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float a = x[r][e] * inv, b = x[r][e + 1] * inv;
+          const uint32_t h = e4m3x2(a, b);
+          const float2 f = from_e4m3x2(h);
+          hi |= h << (8 * e);
+          lo |= e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (8 * e);
+        }
+        // row (token of the row, term, head); 16-byte pieces lie at their number xor the row's, modulo 8
+#pragma unroll
+        for (int c = 0; c < PACK; ++c)
+#pragma unroll
+          for (int term = 0; term < 2; ++term) {
+            const int row = (c * 2 + term) * NR + r;
+#pragma unroll
+            for (int half = 0; half < PACK; ++half) {
+              const int byte = half * D + lane * E;
+              uint8_t* at = dst + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
+              const uint32_t v = half == c ? (term ? lo : hi) : 0u;
+              if (E == 4) *reinterpret_cast<uint32_t*>(at) = v;
+              else *reinterpret_cast<uint16_t*>(at) = (uint16_t)v;
+            }
+          }
+        if (lane == 0) s_factor[ib * NR + r] = odd ? __int_as_float(0x7fc00000) : s * p.scale_log2;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[ib]);
+    }
+  } else if (warp == 11) {
+    // ------------------------------ idle slots ------------------------------
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+      if (s_pre[b + 1] > s_pre[b]) continue;
+      uint4* row = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Hq * D);
+      for (int i = lane; i < p.Hq * D / 8; i += 32) row[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else if (warp < 4) {
+    // ------------------------------ soft-max: thread = row of the tile ------------------------------
+    const int r = tid, part = r / L::RPB;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    uint32_t tile_no = 0, piece_no = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutEpilogue)) != 0;
+    };
+    for (int cur = begin; cur < end; ++piece_no) {
+      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      const int ctx = min(p.seq_lens[q.row], p.max_blocks * 64);
+      const uint32_t ib = piece_no & 1;
+      const uint32_t tmem_o = tmem_base + lane_off + L::kTmemO + ib * L::NO;
+      ok = ok && wait(&q_full[ib], (piece_no >> 1) & 1);
+      float factor[NR], m[NR], M[NR], l[NR];
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        factor[h] = s_factor[ib * NR + h];
+        m[h] = M[h] = kQ8None;
+        l[h] = 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[ib]);
+      bool gone = false;
+      for (int t = 0; t < q.n; ++t) {
+        const uint32_t tn = tile_no + t, b = tn & 1, stage = tn % NST;
+        ok = ok && wait(&s_full[b], (tn >> 1) & 1) && wait(&k_full[stage], (tn / NST) & 1);
+        if (!ok) s_fail[0] = 1;
+        tc_fence_after();
+        float z[PACK][NR];
+        const float2 sc = s_scale[stage * BPT + part];
+        const float lv = sc.y;
+        const int tok = ((q.t0 + t) * BPT + part) * 64 + (r % L::RPB) * PACK;   // first token of the row
+        const bool there = lv != INFINITY;
+#pragma unroll
+        for (int c = 0; c < PACK; ++c) {
+          uint32_t raw[2 * NR];
+#pragma unroll
+          for (int i = 0; i < 2 * NR; i += 16) tmem_ld_32x16(tmem_base + lane_off + L::kTmemS + b * L::NS + c * 2 * NR + i, *reinterpret_cast<uint32_t(*)[16]>(raw + i));
+          tmem_ld_wait();
+          const bool seen = there && tok + c < ctx;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float s = fmaf(__uint_as_float(raw[NR + h]), 0.0625f, __uint_as_float(raw[h]));
+            z[c][h] = seen ? s * (sc.x * factor[h]) : -INFINITY;
+          }
+        }
+        if constexpr (PACK == 2) {
+          // The last token shares its row with what lies behind it: where that is NaN, zero times it has spoilt the sums, and
+          // the scores are computed here
+          bool spoilt = false;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) spoilt |= z[0][h] != z[0][h];
+          if (spoilt && tok + 1 == ctx) {
+            const uint8_t* k = smem + stage * L::kStage + r * 128;
+            const int group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
+            const __nv_bfloat16* src = p.q + (size_t)q.row * p.row_stride + (size_t)(q.entry / p.groups * rep + group * per_group) * D;
+#pragma unroll
+            for (int h = 0; h < NR; ++h) {
+              float s = 0.f;
+#pragma unroll 1
+              for (int d = 0; d < D && h < left; ++d)
+                s = fmaf(__bfloat162float(src[(size_t)h * D + d]), from_e4m3x2(k[(((d >> 4) ^ (r & 7)) << 4) + (d & 15)]).x, s);
+              z[0][h] = s * sc.x * p.scale_log2;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[b]);
+        // a weight beyond 2^8, or a sum that grows out of its reference's reach
+        bool raise = t == 0 || !ok;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) {
+          const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
+          raise |= top + lv > M[h] + 8.f || top > m[h] + 64.f;
+        }
+        if (vote_128(raise)) {
+          // a wait that ran out: all four warps leave together, or the others would stay in a vote.  One flag per vote: a
+          // warp may be ahead of the others by what lies between two votes
+          if (s_fail[0]) {
+            gone = true;
+            break;
+          }
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
+            const float a = redux_max(top), v = redux_max(top == -INFINITY ? -INFINITY : top + lv);
+            if (lane == h) s_red[warp * NR + h] = make_float2(a, v);
+          }
+          // O^T is scaled below: the products of the tile before have to be in it
+          if (t > 0) ok = wait(&p_empty[b ^ 1], ((tn - 1) >> 1) & 1);
+          if (!ok) s_fail[1] = 1;
+          vote_128(false);
+          if (s_fail[1]) {
+            gone = true;
+            break;
+          }
+          float alpha[NR];
+          bool moved = false;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            float a = m[h], v = M[h];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const float2 x = s_red[w * NR + h];
+              a = fmaxf(a, x.x);
+              v = fmaxf(v, x.y - 3.f);
+            }
+            l[h] *= fast_exp2(m[h] - a);
+            alpha[h] = fast_exp2(M[h] - v);
+            moved |= v != M[h];
+            m[h] = a;
+            M[h] = v;
+          }
+          if (t > 0 && moved) {
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < PACK * 3; ++i) {
+              uint32_t o[NR];
+              if constexpr (NR == 8) tmem_ld_32x8(tmem_o + i * NR, o);
+              else tmem_ld_32x16(tmem_o + i * NR, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int h = 0; h < NR; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * alpha[h]);
+              if constexpr (NR == 8) tmem_st_32x8(tmem_o + i * NR, o);
+              else tmem_st_32x16(tmem_o + i * NR, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        // the weighted sum of the tile two before has read this buffer
+        ok = ok && wait(&p_empty[b], ((tn >> 1) & 1) ^ 1);
+        uint8_t* dst = sP + b * L::kPBytes + (r & 15);
+#pragma unroll
+        for (int c = 0; c < PACK; ++c)
+#pragma unroll
+          for (int h = 0; h < NR; h += 2) {
+            l[h] += fast_exp2(z[c][h] - m[h]);
+            l[h + 1] += fast_exp2(z[c][h + 1] - m[h + 1]);
+            const bool seen = z[c][h] != -INFINITY || z[c][h + 1] != -INFINITY;
+            float2 w = make_float2(fast_exp2(z[c][h] - M[h] + lv), fast_exp2(z[c][h + 1] - M[h + 1] + lv));
+            if (!seen) w = make_float2(0.f, 0.f);      // -inf plus the mark of a block that is not there
+#pragma unroll
+            for (int term = 0; term < 3; ++term) {
+              const uint32_t code = e4m3x2(w.x, w.y);
+              const int row = (c * 3 + term) * NR + h;
+              dst[row * 128 + (((r >> 4) ^ (row & 7)) << 4)] = (uint8_t)code;
+              dst[(row + 1) * 128 + (((r >> 4) ^ ((row + 1) & 7)) << 4)] = (uint8_t)(code >> 8);
+              const float2 f = from_e4m3x2(code);
+              w = make_float2((w.x - f.x) * 16.f, (w.y - f.y) * 16.f);
+            }
+          }
+        // rows behind the last token may hold anything, NaN too: zero weights alone would not do
+        if ((q.t0 + t + 1) * L::TT > ctx || !there) {
+          ok = ok && wait(&v_full[stage], (tn / NST) & 1);
+          uint8_t* v = smem + stage * L::kStage + 16384 + r * 128;
+#pragma unroll
+          for (int c = 0; c < PACK; ++c)
+            if (!there || tok + c >= ctx)
+#pragma unroll
+              for (int i = 0; i < 8 / PACK; ++i)
+                *reinterpret_cast<uint4*>(v + (((c * (8 / PACK) + i) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+      }
+      if (gone) break;
+      tile_no += q.n;
+      cur += q.n;
+      // sums over the warp: half of the heads go to the other half of the lanes at every step
+      float* stat = s_stat + ib * 6 * NR;
+      ok = ok && wait(&o_empty[ib], ((piece_no >> 1) & 1) ^ 1);
+#pragma unroll
+      for (int n = NR, o = 16; o > 0; o >>= 1) {
+        if (n > 1) {
+          n >>= 1;
+#pragma unroll
+          for (int i = 0; i < NR / 2; ++i)
+            if (i < n) {
+              const bool up = lane & o;
+              const float mine = up ? l[i + n] : l[i], other = up ? l[i] : l[i + n];
+              l[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+            }
+        } else {
+          l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        }
+      }
+      constexpr int kLow = NR == 8 ? 2 : 1;      // lane bits below are copies
+      if ((lane & ((1 << kLow) - 1)) == 0) stat[warp * NR + (lane >> kLow)] = l[0];
+      if (warp == 0) {
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+          if (lane == h) {
+            stat[4 * NR + h] = m[h];
+            stat[5 * NR + h] = M[h];
+          }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_full[ib]);
+    }
+  } else {
+    // ------------------------------ output: thread = byte of a row ------------------------------
+    const int quarter = warp - 4, byte = quarter * 32 + lane, d = byte % D, c = byte / D;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    uint32_t piece_no = 0;
+    for (int cur = begin; cur < end; ++piece_no) {
+      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      const uint32_t ib = piece_no & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&o_full[ib], (piece_no >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
+      tc_fence_after();
+      float o[NR];
+      {
+        uint32_t x[3][NR];
+        const uint32_t at = tmem_base + lane_off + L::kTmemO + ib * L::NO + c * 3 * NR;
+#pragma unroll
+        for (int term = 0; term < 3; ++term) {
+          if constexpr (NR == 8) tmem_ld_32x8(at + term * NR, x[term]);
+          else tmem_ld_32x16(at + term * NR, x[term]);
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+          o[h] = fmaf(fmaf(__uint_as_float(x[2][h]), 0.0625f, __uint_as_float(x[1][h])), 0.0625f, __uint_as_float(x[0][h]));
+      }
+      const float* stat = s_stat + ib * 6 * NR;
+      float lse = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        const float sum = (stat[h] + stat[NR + h]) + (stat[2 * NR + h] + stat[3 * NR + h]);
+        const float m = stat[4 * NR + h];
+        o[h] *= sum == 0.f ? 0.f : fast_exp2(stat[5 * NR + h] - m) / sum;
+        if (lane == h && sum > 0.f) lse = m + log2f(sum);
+        if (lane == h && sum != sum) lse = sum;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[ib]);
+      if constexpr (PACK == 2) {
+        // the odd tokens' warps hand their share to the even tokens'
+        if (c == 1) {
+          if (!__all_sync(0xffffffffu, mbar_wait(x_empty, (piece_no & 1) ^ 1, p.status, kStatusTimeoutEpilogue))) break;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) s_x[h * 64 + d] = o[h];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(x_full);
+        } else {
+          if (!__all_sync(0xffffffffu, mbar_wait(x_full, piece_no & 1, p.status, kStatusTimeoutEpilogue))) break;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) o[h] += s_x[h * 64 + d];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(x_empty);
+        }
+      }
+      if (c == 0) {
+        const int group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
+        const int head0 = q.entry / p.groups * rep + group * per_group;
+        const int slot = 2 * blockIdx.x + (cur == begin ? 0 : 1);
+        __nv_bfloat16* orow = p.out + ((size_t)q.row * p.Hq + head0) * D + d;
+        float* wrow = p.ws_o + (size_t)slot * NR * D + d;
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+          if (h < left) {
+            if (q.whole) orow[h * D] = __float2bfloat16(o[h]);
+            else wrow[h * D] = o[h];
+          }
+        if (!q.whole && quarter == 0 && lane < NR) p.ws_lse[(size_t)slot * NR + lane] = lse;
+      }
+      cur += q.n;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kTmemCols);
+  }
+}
+
+// entries whose tiles are spread over several ranges: mean of the partial results, weighted by 2^(log-sum-exp)
+template <int D, int NR>
+__global__ void __launch_bounds__(128) fmha_decode8_merge_kernel(Decode8Params p, int grid) {
+  chain_sync();
+  const int entries = p.Hkv * p.groups, b = blockIdx.x, entry = blockIdx.y;
+  const int total = p.ws_pre[p.B] * entries, before = p.ws_pre[b], tiles = p.ws_pre[b + 1] - before;
+  if (tiles == 0) return;
+  const int ranges = d8_ranges(total, grid);
+  const int first = before * entries + entry * tiles;
+  // the range that holds position x is the last one that begins at or before it
+  const int c0 = (int)(((long long)(first + 1) * ranges - 1) / total), c1 = (int)(((long long)(first + tiles) * ranges - 1) / total);
+  if (c0 == c1) return;
+  const int rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups, group = entry % p.groups;
+  const int left = min(per_group, rep - group * per_group), head0 = entry / p.groups * rep + group * per_group;
+  for (int i = threadIdx.x * 4; i < left * D; i += 128 * 4) {
+    const int h = i / D;
+    float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = c0; c <= c1; ++c) {
+      const int slot = 2 * c + (d8_begin(total, c, ranges) >= first ? 0 : 1);
+      const float lse = p.ws_lse[(size_t)slot * NR + h];
+      const float4 o = *reinterpret_cast<const float4*>(p.ws_o + (size_t)slot * NR * D + i);
+      const float now = fmaxf(top, lse);
+      const float f = now == -INFINITY ? 0.f : exp2f(top - now), w = lse == -INFINITY ? 0.f : exp2f(lse - now);
+      sum = sum * f + w;
+      acc[0] = acc[0] * f + w * o.x; acc[1] = acc[1] * f + w * o.y; acc[2] = acc[2] * f + w * o.z; acc[3] = acc[3] * f + w * o.w;
+      top = now;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.Hq + head0) * D + i) =
+        make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  }
+}
+
+template <int D, int NR>
+static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int grid, cudaStream_t stream) {
+  using L = D8<D, NR>;
+  static_assert(L::kStages >= 4 && L::kTotal <= kQ8Smem && 2 * (L::NS + L::NO) <= 512, "");
+  auto kernel = fmha_decode8_kernel<D, NR>;
+  static int configured = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured != dev) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e != cudaSuccess) return (int)e;
+    configured = dev;
+  }
+  const int rc = launch_chained(kernel, (unsigned)grid, 384, L::kTotal, stream, mc, p);
+  if (rc || p.max_blocks <= L::BPT) return rc;      // one tile per entry: nothing is split
+  return launch_chained(fmha_decode8_merge_kernel<D, NR>, dim3(p.B, p.Hkv * p.groups), 128, 0, stream, p, grid);
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+// Query heads of a group (rows of a partial result): ws_o = 2 * num_sms * rows * D floats, ws_lse = 2 * num_sms * rows,
+// ws_pre = B + 1 ints.
+extern "C" int sb_kv8_decode_rows(int Hq, int Hkv) { return Hq / Hkv <= 8 ? 8 : 16; }
+extern "C" int sb_kv8_decode_grid() { return num_sms(); }
+
+// One query row per sequence (at most 1024) against its cached context of seq_lens[b] tokens, the current one included; 0: idle
+// slot, its output row is zero.  Rows start on 4-byte boundaries.
+extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const float* scales, int num_blocks,
+                             const int* seq_lens, const int* block_table, int max_blocks, void* out, float* ws_o,
+                             float* ws_lse, int* ws_pre, int B, int Hq, int Hkv, int D, float scale, int* status,
+                             cudaStream_t stream) {
+  if (B == 0) return 0;
+  if (D != 64 && D != 128) return -2;
+  if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || max_blocks < 1 || num_blocks < 1) return -3;
+  const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (long long)(max_blocks + 1) / 2 * B * Hkv * 2;
+  if (rows > 0x7fffffffll || tiles > 0x7fffffffll) return -4;
+  static thread_local bool tl_context_bound = false;
+  if (!tl_context_bound) {
+    cudaFree(0);
+    tl_context_bound = true;
+  }
+  // rows of 128 bytes, as 64 16-bit numbers; a box is a cache block of one head
+  CUtensorMap mc;
+  const int r = make_tensor_map_bf16_2d(&mc, codes, 64, rows, 64, 64, D / 2);
+  if (r) return r;
+  Decode8Params p;
+  p.q = (const __nv_bfloat16*)q; p.row_stride = row_stride; p.scales = scales; p.seq_lens = seq_lens;
+  p.block_table = block_table; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
+  p.groups = Hq / Hkv > 16 ? 2 : 1;
+  p.out = (__nv_bfloat16*)out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.ws_pre = ws_pre;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  const int grid = num_sms();
+  if (Hq / Hkv <= 8) return D == 128 ? launch_decode8<128, 8>(mc, p, grid, stream) : launch_decode8<64, 8>(mc, p, grid, stream);
+  return D == 128 ? launch_decode8<128, 16>(mc, p, grid, stream) : launch_decode8<64, 16>(mc, p, grid, stream);
+}

@@ -189,53 +189,6 @@ __global__ void __launch_bounds__(256) copy8_blocks_kernel(uint8_t* codes, float
   }
 }
 
-// ---------------------------------------------------------------------------------------
-// single-token attention, one block per (sequence, query head): a warp takes every eighth token, a lane D / 32 columns
-// ---------------------------------------------------------------------------------------
-template <int D>
-__global__ void __launch_bounds__(256) decode8_simple_kernel(const __nv_bfloat16* q, int row_stride, const uint8_t* codes,
-                                                             const float* scales, int num_blocks, const int* seq_lens,
-                                                             const int* block_table, int max_blocks, __nv_bfloat16* out,
-                                                             int Hq, int Hkv, float scale_log2) {
-  chain_sync();
-  constexpr int N = D / 32;
-  __shared__ float s_m[8], s_l[8], s_o[8][D];
-  const int b = blockIdx.x, h = blockIdx.y, g = h / (Hq / Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = min(seq_lens[b], max_blocks * kB8);
-  float qv[N], o[N] = {}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < N; ++i) qv[i] = __bfloat162float(q[(size_t)b * row_stride + (size_t)h * D + lane * N + i]) * scale_log2;
-  for (int t = warp; t < n; t += 8) {
-    const int blk = block_table[(size_t)b * max_blocks + t / kB8];
-    if (blk < 0 || blk >= num_blocks) continue;
-    const size_t ks = ((size_t)blk * 2) * Hkv + g, vs = ks + Hkv;
-    float k[N], v[N], s = 0.f;
-    for (int i = 0; i < N; i += 2) {
-      const float2 a = values_of(*reinterpret_cast<const uint16_t*>(codes + (ks * kB8 + t % kB8) * D + lane * N + i));
-      const float2 c = values_of(*reinterpret_cast<const uint16_t*>(codes + (vs * kB8 + t % kB8) * D + lane * N + i));
-      k[i] = a.x; k[i + 1] = a.y; v[i] = c.x; v[i + 1] = c.y;
-    }
-    for (int i = 0; i < N; ++i) s += qv[i] * k[i];
-    s = warp_sum(s) * scales[ks];
-    const float m_new = fmaxf(m, s), f = exp2f(m - m_new), w = exp2f(s - m_new);
-    l = l * f + w;
-    for (int i = 0; i < N; ++i) o[i] = o[i] * f + w * scales[vs] * v[i];
-    m = m_new;
-  }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-  for (int i = 0; i < N; ++i) s_o[warp][lane * N + i] = o[i];
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  float top = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < 8; ++w) {
-    const float f = s_l[w] > 0.f ? exp2f(s_m[w] - top) : 0.f;
-    sum += s_l[w] * f;
-    acc += f > 0.f ? s_o[w][threadIdx.x] * f : 0.f;
-  }
-  out[((size_t)b * Hq + h) * D + threadIdx.x] = __float2bfloat16(n > 0 && sum != 0.f ? acc / sum : 0.f);
-}
-
 }  // namespace sb
 
 using namespace sb;
@@ -267,15 +220,4 @@ extern "C" int sb_kv8_copy_blocks(void* codes, float* scales, const int* src, co
   copy8_blocks_kernel<<<dim3(8, n_pairs < 4096 ? n_pairs : 4096), 256, 0, stream>>>((uint8_t*)codes, scales, src, dst, n_pairs,
                                                                                      num_blocks, per_block, bytes);
   return (int)cudaGetLastError();
-}
-
-extern "C" int sb_kv8_decode(const void* q, int row_stride, const void* codes, const float* scales, int num_blocks,
-                             const int* seq_lens, const int* block_table, int max_blocks, void* out, int B, int Hq, int Hkv,
-                             int D, float scale, cudaStream_t stream) {
-  if (B == 0) return 0;
-  if (D != 64 && D != 128) return -2;
-  if (Hq % Hkv) return -3;
-  return launch_chained(D == 128 ? decode8_simple_kernel<128> : decode8_simple_kernel<64>, dim3(B, Hq), 256, 0, stream,
-                        (const __nv_bfloat16*)q, row_stride, (const uint8_t*)codes, scales, num_blocks, seq_lens, block_table,
-                        max_blocks, (__nv_bfloat16*)out, Hq, Hkv, scale * 1.4426950408889634f);
 }

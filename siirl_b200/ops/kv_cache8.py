@@ -24,6 +24,7 @@ from . import lib as _lib
 BLOCK = 64
 LARGEST = 448.0             # of e4m3
 HEAD_DIMS = (64, 128)       # of the kernels; the CPU statements take any
+ROWS = 1024                 # sequences of one launch of the single-token kernel
 
 
 class Cache8(NamedTuple):
@@ -208,11 +209,26 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
             out[b] = torch.einsum("hn,hnd->hd", torch.softmax(s, -1), v).reshape(-1).to(out.dtype)
         return out
     _require(q_rows.dtype == torch.bfloat16, "query rows are bf16")
+    if q_rows.stride(0) % 2 or q_rows.data_ptr() % 4:
+        q_rows = q_rows[:, :width].contiguous()
+    L = _lib.get_lib()
     with _device(q_rows):
-        _lib.check(_lib.get_lib().sb_kv8_decode(
-            _lib.ptr(q_rows), q_rows.stride(0), _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0],
-            _lib.ptr(seq_lens), _lib.ptr(block_table), block_table.shape[1], _lib.ptr(out), B, n_heads, n_kv_heads, head_dim,
-            ctypes.c_float(scale), _lib.stream()), "sb_kv8_decode")
+        grid, rows = L.sb_kv8_decode_grid(), L.sb_kv8_decode_rows(n_heads, n_kv_heads)
+        for at in range(0, B, ROWS):
+            n = min(ROWS, B - at)
+            # two partial results per block of the grid, and the sequences' places in the list of tiles.  A buffer of the
+            # call's own: calls on other streams and graphs that hold one write to theirs
+            ws = torch.empty(2 * grid * rows * (head_dim + 1) + n + 1, dtype=torch.float32, device=q_rows.device)
+            o, e = ws.data_ptr(), 2 * grid * rows
+            _lib.check(L.sb_kv8_decode(
+                ctypes.c_void_p(q_rows.data_ptr() + 2 * at * q_rows.stride(0)), ctypes.c_longlong(q_rows.stride(0)),
+                _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0],
+                ctypes.c_void_p(seq_lens.data_ptr() + 4 * at),
+                ctypes.c_void_p(block_table.data_ptr() + 4 * at * block_table.shape[1]), block_table.shape[1],
+                ctypes.c_void_p(out.data_ptr() + 2 * at * width), ctypes.c_void_p(o), ctypes.c_void_p(o + 4 * e * head_dim),
+                ctypes.c_void_p(o + 4 * e * (head_dim + 1)), n, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale),
+                _lib.ptr(_lib.status_word(q_rows.device)), _lib.stream()), "sb_kv8_decode")
+            _lib.add_launches(int(block_table.shape[1] > 2 * 128 // head_dim))      # ranges' shares are merged
     return out
 
 
