@@ -18,13 +18,14 @@
 // one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry; a piece that is not
 // the whole entry leaves a normalised partial result and its log-sum-exp in a workspace, two slots per CTA, and a small
 // kernel merges them.  The warps:
-//   0..3   soft-max, thread = row of the tile.  The weights' references are shared by the four: a vote per tile says whether
-//          one of them has to be raised (a weight above 2^8; a fresh one puts the largest weight at 2^3)
-//   4..7   output: O^T of a piece while the next piece's tiles are under way (O^T is double-buffered)
-//   8      producer: a ring of K and V tiles, ids and scales of the next 32 cache blocks of the list in registers
-//   9      MMA issuer: scores one tile ahead of the weighted sums
-//   10     query terms of the next piece
-//   11     zero rows of idle slots
+//   0..7   soft-max, thread = row of the tile.  Four warps take the even tiles of the range, four the odd ones, each with an
+//          O^T and weights' references of its own, so that two tiles are under way and nobody waits for the other four.  A
+//          vote of the four per tile says whether a reference has to be raised (a weight above 2^8; a fresh one puts the
+//          largest weight at 2^3)
+//   8..11  output: joins the two O^T of a piece while the next piece's tiles are under way (double-buffered)
+//   12     producer: a ring of K and V tiles, ids and scales of the next 32 cache blocks of the list in registers
+//   13, 14 MMA issuers: scores; weighted sums
+//   15     query terms of the next pieces
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -68,16 +69,16 @@ __device__ __forceinline__ float redux_max(float x) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-// whether `any` is set in one of the 128 threads of the soft-max warps
-__device__ __forceinline__ bool vote_128(bool any) {
+// whether `any` is set in one of the 128 threads of four soft-max warps
+__device__ __forceinline__ bool vote_128(int group, bool any) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)any)
+      : "r"((uint32_t)any), "r"(1 + group)
       : "memory");
   return r != 0;
 }
@@ -113,26 +114,28 @@ struct D8 {
   static constexpr int TT = 64 * BPT;              // tokens of a tile
   static constexpr int NS = PACK * 2 * NR;         // columns of S^T
   static constexpr int NO = (PACK * 3 * NR + 15) / 16 * 16;   // columns of O^T: a legal N of the MMA
+  static constexpr int NQ = NS <= 32 ? 4 : 2;      // query buffers
   static constexpr int kQBytes = NS * 128, kPBytes = NO * 128, kStage = 32768;
   static constexpr int kXBytes = PACK == 2 ? 64 * NR * 4 : 0; // the second tokens' share of a result
-  static constexpr int kFixed = 2 * kQBytes + 2 * kPBytes + kXBytes + (kQ8Rows + 1 + 32) * 4 + 4096;
+  static constexpr int kFixed = NQ * kQBytes + 2 * kPBytes + kXBytes + (2 * kQ8Rows + 1 + 32) * 4 + 4096;
   static constexpr int kStages = (kQ8Smem - kFixed) / kStage < 6 ? (kQ8Smem - kFixed) / kStage : 6;
-  static constexpr int kQOff = kStages * kStage, kPOff = kQOff + 2 * kQBytes, kXOff = kPOff + 2 * kPBytes;
-  static constexpr int kScaleOff = kXOff + kXBytes;                    // [stages][BPT] {ks, log2 vs}
-  static constexpr int kRedOff = kScaleOff + kStages * BPT * 8;        // [4][NR] {max z, max z + log2 vs}
-  static constexpr int kStatOff = kRedOff + 4 * NR * 8;                // per O^T buffer: l [4][NR], m [NR], M [NR]
-  static constexpr int kFactorOff = kStatOff + 2 * 6 * NR * 4;         // per query buffer: factor of the scores [NR]
-  static constexpr int kBarOff = (kFactorOff + 2 * NR * 4 + 7) / 8 * 8;
-  static constexpr int kBars = 3 * kStages + 18;
-  static constexpr int kPreOff = kBarOff + kBars * 8 + 16;
-  static constexpr int kTotal = kPreOff + (kQ8Rows + 1 + 32) * 4;
-  static constexpr int kTmemS = 0, kTmemO = 2 * NS;                    // columns
-  static constexpr int kTmemCols = 2 * (NS + NO) <= 128 ? 128 : 2 * (NS + NO) <= 256 ? 256 : 512;
+  static constexpr int kQOff = kStages * kStage, kPOff = kQOff + NQ * kQBytes, kXOff = kPOff + 2 * kPBytes;
+  static constexpr int kBlockOff = kXOff + kXBytes;                    // [stages][BPT] {ks, log2 vs, visible tokens}
+  static constexpr int kPieceOff = kBlockOff + kStages * BPT * 16;     // [NQ] {sequence, entry, first tile, tiles}
+  static constexpr int kRedOff = kPieceOff + NQ * 16;                  // [2 groups][4][NR] {max z, max z + log2 vs}
+  static constexpr int kStatOff = kRedOff + 2 * 4 * NR * 8;            // [2 buffers][2 groups]: l [4][NR], m [NR], M [NR]
+  static constexpr int kFactorOff = kStatOff + 4 * 6 * NR * 4;         // [NQ][NR] factor of the scores
+  static constexpr int kBarOff = kFactorOff + NQ * NR * 4;
+  static constexpr int kBars = 3 * kStages + 2 * NQ + 14;
+  static constexpr int kPreOff = kBarOff + kBars * 8 + 24;
+  static constexpr int kTotal = kPreOff + (2 * kQ8Rows + 1 + 32) * 4;
+  // TMEM columns: S^T of the two groups, O^T [2 buffers][2 groups]
+  static constexpr int kTmemS = 0, kTmemO = 2 * NS;
+  static constexpr int kTmemCols = 2 * NS + 4 * NO <= 256 ? 256 : 512;
 };
 
 struct D8Piece {
   int row, entry, t0, n, tiles;    // entry: kv head * groups + group
-  bool whole;
 };
 // the piece at list position `cur` of a range that ends at `end`; pre[b] = tiles of one entry of the sequences before b
 __device__ __forceinline__ D8Piece d8_piece(const int* pre, int B, int entries, int cur, int end) {
@@ -149,20 +152,39 @@ __device__ __forceinline__ D8Piece d8_piece(const int* pre, int B, int entries, 
   q.entry = at / q.tiles;
   q.t0 = at - q.entry * q.tiles;
   q.n = min(q.tiles - q.t0, end - cur);
-  q.whole = q.n == q.tiles;
   return q;
 }
-__device__ __forceinline__ int d8_tiles(const Decode8Params& p, int b, int tile_tokens) {
-  return (min(max(p.seq_lens[b], 0), p.max_blocks * 64) + tile_tokens - 1) / tile_tokens;
+// the piece behind q, which begins at `cur` < end
+__device__ __forceinline__ void d8_next(const int* pre, int entries, D8Piece& q, int cur, int end) {
+  q.t0 = 0;
+  if (++q.entry == entries) {
+    q.entry = 0;
+    do q.tiles = pre[q.row + 2] - pre[q.row + 1];
+    while (++q.row, q.tiles == 0);
+  }
+  q.n = min(q.tiles, end - cur);
 }
 // ranges of the list, and the first position of one
 __device__ __forceinline__ int d8_ranges(int total, int grid) { return min(grid, max(1, total / kQ8MinTiles)); }
 __device__ __forceinline__ int d8_begin(int total, int cta, int ranges) { return (int)((long long)total * min(cta, ranges) / ranges); }
 
+template <int N>
+__device__ __forceinline__ void tmem_ld_heads(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 8) tmem_ld_32x8(taddr, r);
+  else tmem_ld_32x16(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_heads(uint32_t taddr, const uint32_t (&r)[N]) {
+  if constexpr (N == 8) tmem_st_32x8(taddr, r);
+  else tmem_st_32x16(taddr, r);
+}
+
+constexpr int kQ8Threads = 16 * 32;
+
 template <int D, int NR>
-__global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_constant__ CUtensorMap map_c, Decode8Params p) {
+__global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __grid_constant__ CUtensorMap map_c, Decode8Params p) {
   using L = D8<D, NR>;
-  constexpr int PACK = L::PACK, NST = L::kStages, BPT = L::BPT;
+  constexpr int PACK = L::PACK, NST = L::kStages, BPT = L::BPT, NQ = L::NQ;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023u) {
@@ -171,55 +193,61 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
   }
   uint8_t *sQ = smem + L::kQOff, *sP = smem + L::kPOff;
   float* s_x = reinterpret_cast<float*>(smem + L::kXOff);
-  float2* s_scale = reinterpret_cast<float2*>(smem + L::kScaleOff);
+  float4* s_block = reinterpret_cast<float4*>(smem + L::kBlockOff);
+  int4* s_piece = reinterpret_cast<int4*>(smem + L::kPieceOff);
   float2* s_red = reinterpret_cast<float2*>(smem + L::kRedOff);
   float* s_stat = reinterpret_cast<float*>(smem + L::kStatOff);
   float* s_factor = reinterpret_cast<float*>(smem + L::kFactorOff);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* v_full = k_full + NST;
   uint64_t* kv_empty = v_full + NST;
-  uint64_t* q_full = kv_empty + NST;    // pairs
-  uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_empty + 2;
+  uint64_t* q_full = kv_empty + NST;    // [NQ]
+  uint64_t* q_empty = q_full + NQ;
+  uint64_t* s_full = q_empty + NQ;      // pairs from here on
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;
   uint64_t* p_empty = p_full + 2;
-  uint64_t* o_full = p_empty + 2;       // the piece's MMAs have completed
+  uint64_t* o_full = p_empty + 2;       // the piece's MMAs have completed, its statistics are there
   uint64_t* o_empty = o_full + 2;       // the output warps have read O^T and the statistics
   uint64_t* x_full = o_empty + 2;       // second tokens' share
   uint64_t* x_empty = x_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_empty + 1);
-  volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [2]: before the first, the second vote of a tile
+  volatile int* s_fail = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [4]: by group and vote of a tile
   int* s_pre = reinterpret_cast<int*>(smem + L::kPreOff);
   int* s_tot = s_pre + kQ8Rows + 1;
+  int* s_len = s_tot + 32;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int entries = p.Hkv * p.groups, rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups;
+  // of an entry: kv head, first query head, query heads (one or two groups)
+  auto kv_head = [&](int entry) { return entry >> (p.groups - 1); };
+  auto group_of = [&](int entry) { return entry & (p.groups - 1); };
+  auto first_head = [&](int entry) { return kv_head(entry) * rep + group_of(entry) * per_group; };
+  auto heads_of = [&](int entry) { return min(per_group, rep - group_of(entry) * per_group); };
   if (tid == 0) {
     tma_prefetch_desc(&map_c);
     for (int i = 0; i < 3 * NST; ++i) mbar_init(&k_full[i], 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NQ; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 5);     // the MMAs, the four soft-max warps
+      mbar_init(&q_empty[i], 9);     // the MMAs, the soft-max warps
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&p_empty[i], 1);
-      mbar_init(&o_full[i], 5);      // the MMAs, the statistics of four warps
+      mbar_init(&o_full[i], 9);      // the MMAs, the statistics of the soft-max warps
       mbar_init(&o_empty[i], 4);
     }
     mbar_init(x_full, 2);
     mbar_init(x_empty, 2);
-    s_fail[0] = s_fail[1] = 0;
+    for (int i = 0; i < 4; ++i) s_fail[i] = 0;
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == 13) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
-  // rows of P that no head owns
-  for (int i = tid; i < 2 * L::kPBytes / 16; i += 384) reinterpret_cast<uint4*>(sP)[i] = make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -227,85 +255,92 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
   chain_sync();
   // running sum of the sequences' tiles: chunks of 32 by warp, then their totals
   const int chunks = (p.B + 31) / 32;
-  for (int c = warp; c < chunks; c += 12) {
-    const int b = c * 32 + lane;
-    int v = b < p.B ? d8_tiles(p, b, L::TT) : 0;
+  for (int c = warp; c < chunks; c += kQ8Threads / 32) {
+    const int b = c * 32 + lane, n = b < p.B ? min(max(p.seq_lens[b], 0), p.max_blocks * 64) : 0;
+    int v = (n + L::TT - 1) / L::TT;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
-    if (b < p.B) s_pre[b + 1] = v;
+    if (b < p.B) {
+      s_len[b] = n;
+      s_pre[b + 1] = v;
+    }
     if (lane == 31) s_tot[c] = v;
-  }
-  __syncthreads();
-  for (int c = warp; c < chunks; c += 12) {
-    int before = lane < c ? s_tot[lane] : 0;      // at most 32 chunks
-    before = __reduce_add_sync(0xffffffffu, before);
-    const int b = c * 32 + lane;
-    if (b < p.B) s_pre[b + 1] += before;
   }
   if (tid == 0) s_pre[0] = 0;
   __syncthreads();
+  if (chunks > 1) {
+    for (int c = warp; c < chunks; c += kQ8Threads / 32) {
+      const int before = __reduce_add_sync(0xffffffffu, lane < c ? s_tot[lane] : 0);      // at most 32 chunks
+      const int b = c * 32 + lane;
+      if (b < p.B) s_pre[b + 1] += before;
+    }
+    __syncthreads();
+  }
   const int total = s_pre[p.B] * entries, ranges = d8_ranges(total, gridDim.x);
   const int begin = d8_begin(total, blockIdx.x, ranges), end = d8_begin(total, blockIdx.x + 1, ranges);
   if (blockIdx.x == 0)
-    for (int i = tid; i <= p.B; i += 384) p.ws_pre[i] = s_pre[i];
+    for (int i = tid; i <= p.B; i += kQ8Threads) p.ws_pre[i] = s_pre[i];
 
-  if (warp == 8) {
+  if (warp == 12) {
     // ------------------------------ producer ------------------------------
     // lane i: cache block i % BPT of the tile i / BPT places on in the list
     constexpr int kAhead = 32 / BPT;
-    auto find = [&](int at, int& entry) {      // block id, or -1
-      const int cur = at + lane / BPT;
-      entry = 0;
-      if (cur >= end) return -1;
-      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
-      entry = q.entry;
-      const int j = q.t0 * BPT + lane % BPT;
-      if (j * 64 >= min(p.seq_lens[q.row], p.max_blocks * 64)) return -1;
-      const int blk = p.block_table[(size_t)q.row * p.max_blocks + j];
-      return blk < p.num_blocks ? blk : -1;
+    struct Block {
+      int id, head, left;      // left: tokens of the sequence from this block on
+      float ks, vs;
     };
-    auto scales = [&](int blk, int entry) {
-      if (blk < 0) return make_float2(0.f, 0.f);
-      const float* s = p.scales + (size_t)blk * 2 * p.Hkv + entry / p.groups;
-      return make_float2(s[0], s[p.Hkv]);
+    auto find = [&](int at) {
+      Block x = {-1, 0, 0, 0.f, 0.f};
+      const int cur = at + lane / BPT;
+      if (cur >= end) return x;
+      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      const int j = q.t0 * BPT + lane % BPT;
+      x.head = kv_head(q.entry);
+      x.left = s_len[q.row] - j * 64;
+      if (x.left > 0) x.id = p.block_table[(size_t)q.row * p.max_blocks + j];
+      return x;
+    };
+    auto scales = [&](Block& x) {
+      if (x.id < 0 || x.id >= p.num_blocks) return;
+      const float* s = p.scales + (size_t)x.id * 2 * p.Hkv + x.head;
+      x.ks = s[0];
+      x.vs = s[p.Hkv];
     };
     uint32_t tile_no = 0;
     bool ok = true;
-    int entry, entry2 = 0, blk2 = -1;
-    int blk = find(begin, entry);
-    float2 sc = scales(blk, entry), sc2 = make_float2(0.f, 0.f);
+    Block x = find(begin), y = x;
+    scales(x);
     for (int at = begin; at < end && ok; at += kAhead) {
       const int n = min(kAhead, end - at);
-      blk2 = find(at + kAhead, entry2);
+      const int seen = x.id >= 0 && x.id < p.num_blocks ? min(x.left, 64) : 0;
       for (int k = 0; k < n; ++k, ++tile_no) {
-        if (k == n / 2) sc2 = scales(blk2, entry2);
         const int stage = tile_no % NST;
         if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((tile_no / NST) & 1) ^ 1, p.status, kStatusTimeoutProducer))) {
           ok = false;
           break;
         }
-        const bool mine = lane / BPT == k, loads = mine && blk >= 0;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, loads)) * (uint32_t)(L::RPB * 128);
+        const bool mine = lane / BPT == k;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine && seen)) * (uint32_t)(L::RPB * 128);
         const int part = lane % BPT;
-        // a block that is not there: a scale that nothing else has
-        if (mine) s_scale[stage * BPT + part] = make_float2(sc.x, blk >= 0 ? log2f(sc.y) : INFINITY);
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&k_full[stage], bytes);
-          mbar_arrive_expect_tx(&v_full[stage], bytes);
-        }
-        __syncwarp();
-        if (loads) {
+        if (mine && seen) {
           uint8_t* dst = smem + stage * L::kStage + part * (L::RPB * 128);
-          const int row = (blk * 2 * p.Hkv + entry / p.groups) * L::RPB;
+          const int row = (x.id * 2 * p.Hkv + x.head) * L::RPB;
           tma_load_2d(dst, &map_c, &k_full[stage], 0, row);
           tma_load_2d(dst + 16384, &map_c, &v_full[stage], 0, row + p.Hkv * L::RPB);
         }
+        if (mine) s_block[stage * BPT + part] = make_float4(x.ks, __log2f(x.vs), __int_as_float(seen), 0.f);
+        __syncwarp();
+        if (lane == 0) {      // the copies may be there already: a phase ends with its arrival
+          mbar_arrive_expect_tx(&k_full[stage], bytes);
+          mbar_arrive_expect_tx(&v_full[stage], bytes);
+        }
+        if (k == 0) y = find(at + kAhead);
+        if (k == n / 2) scales(y);
       }
-      blk = blk2; entry = entry2; sc = sc2;
+      x = y;
     }
     if (!ok) {      // no copy may be in flight when shared memory is given back
       const uint32_t first = tile_no > (uint32_t)NST ? tile_no - NST : 0;
@@ -314,102 +349,129 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
         mbar_wait(&v_full[j % NST], (j / NST) & 1, nullptr, 0);
       }
     }
-  } else if (warp == 9) {
-    // ------------------------------ MMA issuer (the whole warp, converged; one lane issues) ------------------------------
+  } else if (warp == 13) {
+    // ------------------------------ scores (the whole warp, converged; one lane issues) ------------------------------
     const uint32_t leader = elect_one() ? 1u : 0u;
-    constexpr uint32_t idesc_s = umma_idesc_e4m3(128, L::NS, 0, 0), idesc_o = umma_idesc_e4m3(128, L::NO, 1, 0);
-    const uint64_t dk = umma_smem_desc(smem_u32(smem), 16, 1024), dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024);
-    const uint64_t dq = umma_smem_desc(smem_u32(sQ), 16, 1024), dp = umma_smem_desc(smem_u32(sP), 16, 1024);
+    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NS, 0, 0);
+    const uint64_t dk = umma_smem_desc(smem_u32(smem), 16, 1024), dq = umma_smem_desc(smem_u32(sQ), 16, 1024);
+    uint32_t piece_no = 0;
+    int left = 0, stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool r = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma));
-      tc_fence_after();
-      return r;
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
     };
-    auto tiles_at = [&](int cur) { return __shfl_sync(0xffffffffu, cur < end ? d8_piece(s_pre, p.B, entries, cur, end).n : 0, 0); };
-    // pieces and tiles left in them, of the scores and, one tile behind, of the weighted sums
-    uint32_t s_piece = 0, o_piece = 0;
-    int s_left = tiles_at(begin), o_left = s_left;
-    bool s_first = true, o_first = true;
-    for (int i = 0; i <= end - begin && ok; ++i) {
-      if (i < end - begin) {
-        const uint32_t b = i & 1, stage = i % NST, ib = s_piece & 1;
-        ok = (!s_first || wait(&q_full[ib], (s_piece >> 1) & 1)) && wait(&k_full[stage], (i / NST) & 1) &&
-             wait(&s_empty[b], ((i >> 1) & 1) ^ 1);
-        if (!ok) break;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_e4m3_ss_if(leader, tmem_base + L::kTmemS + b * L::NS, dk + stage * (L::kStage >> 4) + 2 * kk,
-                          dq + ib * (L::kQBytes >> 4) + 2 * kk, idesc_s, kk ? 1u : 0u);
-        umma_commit_if(leader, &s_full[b]);
-        s_first = --s_left == 0;
-        if (s_first) {
-          umma_commit_if(leader, &q_empty[ib]);
-          ++s_piece;
-          s_left = tiles_at(begin + i + 1);
-        }
+    for (int i = 0; i < end - begin && ok; ++i) {
+      const uint32_t b = i & 1, iq = piece_no % NQ;
+      if (left == 0) {
+        ok = wait(&q_full[iq], (piece_no / NQ) & 1);
+        left = s_piece[iq].w;
       }
-      if (i > 0) {
-        const int j = i - 1;
-        const uint32_t b = j & 1, stage = j % NST, ib = o_piece & 1;
-        ok = (!o_first || wait(&o_empty[ib], ((o_piece >> 1) & 1) ^ 1)) && wait(&v_full[stage], (j / NST) & 1) &&
-             wait(&p_full[b], (j >> 1) & 1);
-        if (!ok) break;
+      ok = ok && wait(&s_empty[b], ((i >> 1) & 1) ^ 1) && wait(&k_full[stage], phase);
+      if (!ok) break;
+      tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + ib * L::NO, dv + stage * (L::kStage >> 4) + 256 * kk,
-                          dp + b * (L::kPBytes >> 4) + 2 * kk, idesc_o, (!o_first || kk) ? 1u : 0u);
-        umma_commit_if(leader, &kv_empty[stage]);
-        umma_commit_if(leader, &p_empty[b]);
-        o_first = --o_left == 0;
-        if (o_first) {
-          umma_commit_if(leader, &o_full[ib]);
-          ++o_piece;
-          o_left = tiles_at(begin + i);
-        }
+      for (int kk = 0; kk < 4; ++kk)
+        umma_e4m3_ss_if(leader, tmem_base + L::kTmemS + b * L::NS, dk + (uint32_t)stage * (L::kStage >> 4) + 2 * kk,
+                        dq + iq * (L::kQBytes >> 4) + 2 * kk, idesc, kk ? 1u : 0u);
+      umma_commit_if(leader, &s_full[b]);
+      if (--left == 0) {
+        umma_commit_if(leader, &q_empty[iq]);
+        ++piece_no;
+      }
+      if (++stage == NST) {
+        stage = 0;
+        phase ^= 1;
       }
     }
-  } else if (warp == 10) {
-    // ------------------------------ query terms ------------------------------
+  } else if (warp == 14) {
+    // ------------------------------ weighted sums ------------------------------
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NO, 1, 0);
+    const uint64_t dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024), dp = umma_smem_desc(smem_u32(sP), 16, 1024);
+    uint32_t piece_no = 0, fresh = 3;      // fresh: groups that have not added to the piece's O^T
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
+    };
+    D8Piece q;
+    if (begin < end) q = d8_piece(s_pre, p.B, entries, begin, end);
+    int left = 0;
+    for (int i = 0; i < end - begin && ok; ++i) {
+      const uint32_t b = i & 1, ib = piece_no & 1;
+      if (left == 0) {
+        if (i) d8_next(s_pre, entries, q, begin + i, end);
+        left = __shfl_sync(0xffffffffu, q.n, 0);
+        ok = wait(&o_empty[ib], ((piece_no >> 1) & 1) ^ 1);
+      }
+      ok = ok && wait(&v_full[stage], phase) && wait(&p_full[b], (i >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t add = ~fresh >> b & 1;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + (ib * 2 + b) * L::NO, dv + (uint32_t)stage * (L::kStage >> 4) + 256 * kk,
+                        dp + b * (L::kPBytes >> 4) + 2 * kk, idesc, kk ? 1u : add);
+      umma_commit_if(leader, &kv_empty[stage]);
+      umma_commit_if(leader, &p_empty[b]);
+      fresh &= ~(1u << b);
+      if (--left == 0) {
+        umma_commit_if(leader, &o_full[ib]);
+        ++piece_no;
+        fresh = 3;
+      }
+      if (++stage == NST) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 15) {
+    // ------------------------------ query terms; the next piece's rows are asked for first ------------------------------
     constexpr int E = D / 32;       // elements of a lane
-    uint32_t piece_no = 0;
-    for (int cur = begin; cur < end; ++piece_no) {
-      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
-      cur += q.n;
-      const int ib = piece_no & 1, group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
-      const __nv_bfloat16* src = p.q + (size_t)q.row * p.row_stride + (size_t)(q.entry / p.groups * rep + group * per_group) * D + lane * E;
-      float x[NR][E];
+    auto load = [&](const D8Piece& q, uint32_t (&raw)[NR][E / 2]) {
+      const int left = heads_of(q.entry);
+      const __nv_bfloat16* src = p.q + (size_t)q.row * p.row_stride + (size_t)first_head(q.entry) * D + lane * E;
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 v = r < left ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + (size_t)r * D + e)) : make_float2(0.f, 0.f);
-          x[r][e] = v.x;
-          x[r][e + 1] = v.y;
-        }
-      if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[ib], ((piece_no >> 1) & 1) ^ 1, p.status, kStatusTimeoutProducer))) break;
-      uint8_t* dst = sQ + ib * L::kQBytes;
+        for (int e = 0; e < E / 2; ++e) raw[r][e] = r < left ? *reinterpret_cast<const uint32_t*>(src + (size_t)r * D + 2 * e) : 0u;
+    };
+    uint32_t piece_no = 0, raw[NR][E / 2], ahead[NR][E / 2];
+    D8Piece q, next;
+    if (begin < end) {
+      q = d8_piece(s_pre, p.B, entries, begin, end);
+      load(q, raw);
+    }
+    for (int cur = begin; cur < end; ++piece_no) {
+      cur += q.n;
+      if (cur < end) {
+        next = q;
+        d8_next(s_pre, entries, next, cur, end);
+        load(next, ahead);
+      }
+      const int iq = piece_no % NQ;
+      if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[iq], ((piece_no / NQ) & 1) ^ 1, p.status, kStatusTimeoutProducer))) break;
+      if (lane == 0) s_piece[iq] = make_int4(q.row, q.entry, q.t0, q.n);
+      uint8_t* dst = sQ + iq * L::kQBytes;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float top = 0.f;
+      for (int h = 0; h < NR; ++h) {
+        // largest |x| as a bf16 number's bits: infinities and NaN are the largest
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[r][e]));
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < E; ++e) odd |= !(fabsf(x[r][e]) <= 3.402823466e38f);
-        odd = __any_sync(0xffffffffu, odd);
-        top = redux_max(top);
-        // a power of two s with top / s in (224, 448] (or s = 2^-126)
-        const uint32_t u = __float_as_uint(top);
-        const int ex = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
-        const float s = __uint_as_float((uint32_t)max(ex, 1) << 23), inv = 1.f / s;
+        for (int e = 0; e < E / 2; ++e) top = max(top, max(raw[h][e] & 0x7fffu, raw[h][e] >> 16 & 0x7fffu));
+        top = __reduce_max_sync(0xffffffffu, top) << 16;
+        // a power of two s with largest / s in (224, 448] (or s = 2^-126)
+        const int ex = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
+        const float s = __uint_as_float((uint32_t)max(ex, 1) << 23), inv = __uint_as_float((uint32_t)(254 - max(ex, 1)) << 23);
         uint32_t hi = 0, lo = 0;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
-          const float a = x[r][e] * inv, b = x[r][e + 1] * inv;
-          const uint32_t h = e4m3x2(a, b);
-          const float2 f = from_e4m3x2(h);
-          hi |= h << (8 * e);
+          const float a = __uint_as_float(raw[h][e / 2] << 16) * inv, b = __uint_as_float(raw[h][e / 2] & 0xffff0000u) * inv;
+          const uint32_t c = e4m3x2(a, b);
+          const float2 f = from_e4m3x2(c);
+          hi |= c << (8 * e);
           lo |= e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (8 * e);
         }
         // row (token of the row, term, head); 16-byte pieces lie at their number xor the row's, modulo 8
@@ -417,7 +479,7 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
         for (int c = 0; c < PACK; ++c)
 #pragma unroll
           for (int term = 0; term < 2; ++term) {
-            const int row = (c * 2 + term) * NR + r;
+            const int row = (c * 2 + term) * NR + h;
 #pragma unroll
             for (int half = 0; half < PACK; ++half) {
               const int byte = half * D + lane * E;
@@ -427,126 +489,122 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
               else *reinterpret_cast<uint16_t*>(at) = (uint16_t)v;
             }
           }
-        if (lane == 0) s_factor[ib * NR + r] = odd ? __int_as_float(0x7fc00000) : s * p.scale_log2;
+        if (lane == 0) s_factor[iq * NR + h] = top >= 0x7f800000u ? __int_as_float(0x7fc00000) : s * p.scale_log2;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[ib]);
+      if (lane == 0) mbar_arrive(&q_full[iq]);
+      q = next;
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) raw[r][e] = ahead[r][e];
     }
-  } else if (warp == 11) {
-    // ------------------------------ idle slots ------------------------------
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-      if (s_pre[b + 1] > s_pre[b]) continue;
-      uint4* row = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Hq * D);
-      for (int i = lane; i < p.Hq * D / 8; i += 32) row[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-  } else if (warp < 4) {
+  } else if (warp < 8) {
     // ------------------------------ soft-max: thread = row of the tile ------------------------------
-    const int r = tid, part = r / L::RPB;
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    uint32_t tile_no = 0, piece_no = 0;
-    bool ok = true;
+    const int g = warp >> 2, quarter = warp & 3;      // g: group, parity of its tiles
+    const int r = quarter * 32 + lane, part = r / L::RPB, at = (r % L::RPB) * PACK;      // `at`: first token, in its block
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16, tmem_s = tmem_base + lane_off + L::kTmemS + g * L::NS;
+    uint8_t* dst = sP + g * L::kPBytes + (r & 15);
+    float2* red = s_red + g * 4 * NR;
+    int tn = 0;                // first tile of the piece, in the range
+    uint32_t turn = 0;         // tiles of the group so far
+    uint32_t piece_no = 0;
+    bool ok = true, gone = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutEpilogue)) != 0;
     };
-    for (int cur = begin; cur < end; ++piece_no) {
-      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
-      const int ctx = min(p.seq_lens[q.row], p.max_blocks * 64);
-      const uint32_t ib = piece_no & 1;
-      const uint32_t tmem_o = tmem_base + lane_off + L::kTmemO + ib * L::NO;
-      ok = ok && wait(&q_full[ib], (piece_no >> 1) & 1);
-      float factor[NR], m[NR], M[NR], l[NR];
+    for (; tn < end - begin && !gone; ++piece_no) {
+      const uint32_t ib = piece_no & 1, iq = piece_no % NQ;
+      const uint32_t tmem_o = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO;
+      ok = ok && wait(&q_full[iq], (piece_no / NQ) & 1);
+      const int4 piece = s_piece[iq];
+      const float* factor = s_factor + iq * NR;
+      // a warp that has given up says so in the next vote
+      const int stop = ok ? tn + piece.w : tn + 2;
+      float m[NR], M[NR], l[NR];
 #pragma unroll
       for (int h = 0; h < NR; ++h) {
-        factor[h] = s_factor[ib * NR + h];
         m[h] = M[h] = kQ8None;
         l[h] = 0.f;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[ib]);
-      bool gone = false;
-      for (int t = 0; t < q.n; ++t) {
-        const uint32_t tn = tile_no + t, b = tn & 1, stage = tn % NST;
-        ok = ok && wait(&s_full[b], (tn >> 1) & 1) && wait(&k_full[stage], (tn / NST) & 1);
-        if (!ok) s_fail[0] = 1;
+      bool first = true;
+      for (int t = tn + ((tn ^ g) & 1); t < stop; t += 2, ++turn) {
+        const uint32_t stage = (uint32_t)t % NST, round = (uint32_t)t / NST & 1;
+        ok = ok && wait(&k_full[stage], round) && wait(&s_full[g], turn & 1);
+        if (!ok) s_fail[2 * g] = 1;
         tc_fence_after();
+        const float4 block = s_block[stage * BPT + part];
+        const float lv = block.y;
+        const int seen = __float_as_int(block.z) - at;      // tokens of the row: more than 0, more than 1
         float z[PACK][NR];
-        const float2 sc = s_scale[stage * BPT + part];
-        const float lv = sc.y;
-        const int tok = ((q.t0 + t) * BPT + part) * 64 + (r % L::RPB) * PACK;   // first token of the row
-        const bool there = lv != INFINITY;
 #pragma unroll
         for (int c = 0; c < PACK; ++c) {
-          uint32_t raw[2 * NR];
-#pragma unroll
-          for (int i = 0; i < 2 * NR; i += 16) tmem_ld_32x16(tmem_base + lane_off + L::kTmemS + b * L::NS + c * 2 * NR + i, *reinterpret_cast<uint32_t(*)[16]>(raw + i));
+          uint32_t raw[2][NR];
+          tmem_ld_heads(tmem_s + (c * 2) * NR, raw[0]);
+          tmem_ld_heads(tmem_s + (c * 2 + 1) * NR, raw[1]);
           tmem_ld_wait();
-          const bool seen = there && tok + c < ctx;
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
-            const float s = fmaf(__uint_as_float(raw[NR + h]), 0.0625f, __uint_as_float(raw[h]));
-            z[c][h] = seen ? s * (sc.x * factor[h]) : -INFINITY;
+            const float s = fmaf(__uint_as_float(raw[1][h]), 0.0625f, __uint_as_float(raw[0][h]));
+            z[c][h] = seen > c ? s * (block.x * factor[h]) : -INFINITY;
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[g]);
         if constexpr (PACK == 2) {
           // The last token shares its row with what lies behind it: where that is NaN, zero times it has spoilt the sums, and
           // the scores are computed here
           bool spoilt = false;
 #pragma unroll
           for (int h = 0; h < NR; ++h) spoilt |= z[0][h] != z[0][h];
-          if (spoilt && tok + 1 == ctx) {
+          if (spoilt && seen == 1) {
             const uint8_t* k = smem + stage * L::kStage + r * 128;
-            const int group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
-            const __nv_bfloat16* src = p.q + (size_t)q.row * p.row_stride + (size_t)(q.entry / p.groups * rep + group * per_group) * D;
+            const int left = heads_of(piece.y);
+            const __nv_bfloat16* src = p.q + (size_t)piece.x * p.row_stride + (size_t)first_head(piece.y) * D;
 #pragma unroll
             for (int h = 0; h < NR; ++h) {
               float s = 0.f;
 #pragma unroll 1
               for (int d = 0; d < D && h < left; ++d)
                 s = fmaf(__bfloat162float(src[(size_t)h * D + d]), from_e4m3x2(k[(((d >> 4) ^ (r & 7)) << 4) + (d & 15)]).x, s);
-              z[0][h] = s * sc.x * p.scale_log2;
+              z[0][h] = s * block.x * p.scale_log2;
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[b]);
         // a weight beyond 2^8, or a sum that grows out of its reference's reach
-        bool raise = t == 0 || !ok;
+        bool raise = first || !ok;
 #pragma unroll
         for (int h = 0; h < NR; ++h) {
           const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
           raise |= top + lv > M[h] + 8.f || top > m[h] + 64.f;
         }
-        if (vote_128(raise)) {
+        if (vote_128(g, raise)) {
           // a wait that ran out: all four warps leave together, or the others would stay in a vote.  One flag per vote: a
           // warp may be ahead of the others by what lies between two votes
-          if (s_fail[0]) {
-            gone = true;
-            break;
-          }
+          gone = s_fail[2 * g];
+          if (gone) break;
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
             const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
             const float a = redux_max(top), v = redux_max(top == -INFINITY ? -INFINITY : top + lv);
-            if (lane == h) s_red[warp * NR + h] = make_float2(a, v);
+            if (lane == h) red[quarter * NR + h] = make_float2(a, v);
           }
-          // O^T is scaled below: the products of the tile before have to be in it
-          if (t > 0) ok = wait(&p_empty[b ^ 1], ((tn - 1) >> 1) & 1);
-          if (!ok) s_fail[1] = 1;
-          vote_128(false);
-          if (s_fail[1]) {
-            gone = true;
-            break;
-          }
-          float alpha[NR];
+          // O^T is scaled below: the products of the group's tile before have to be in it
+          if (!first) ok = wait(&p_empty[g], (turn & 1) ^ 1);
+          if (!ok) s_fail[2 * g + 1] = 1;
+          vote_128(g, false);
+          gone = s_fail[2 * g + 1];
+          if (gone) break;
           bool moved = false;
+          float alpha[NR];
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
             float a = m[h], v = M[h];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const float2 x = s_red[w * NR + h];
+              const float2 x = red[w * NR + h];
               a = fmaxf(a, x.x);
               v = fmaxf(v, x.y - 3.f);
             }
@@ -556,34 +614,31 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
             m[h] = a;
             M[h] = v;
           }
-          if (t > 0 && moved) {
+          if (!first && moved) {
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < PACK * 3; ++i) {
               uint32_t o[NR];
-              if constexpr (NR == 8) tmem_ld_32x8(tmem_o + i * NR, o);
-              else tmem_ld_32x16(tmem_o + i * NR, o);
+              tmem_ld_heads(tmem_o + i * NR, o);
               tmem_ld_wait();
 #pragma unroll
               for (int h = 0; h < NR; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * alpha[h]);
-              if constexpr (NR == 8) tmem_st_32x8(tmem_o + i * NR, o);
-              else tmem_st_32x16(tmem_o + i * NR, o);
+              tmem_st_heads(tmem_o + i * NR, o);
             }
             tmem_st_wait();
           }
         }
-        // the weighted sum of the tile two before has read this buffer
-        ok = ok && wait(&p_empty[b], ((tn >> 1) & 1) ^ 1);
-        uint8_t* dst = sP + b * L::kPBytes + (r & 15);
+        first = false;
+        // the weighted sum of the group's tile before has read this buffer
+        ok = ok && wait(&p_empty[g], (turn & 1) ^ 1);
 #pragma unroll
         for (int c = 0; c < PACK; ++c)
 #pragma unroll
           for (int h = 0; h < NR; h += 2) {
             l[h] += fast_exp2(z[c][h] - m[h]);
             l[h + 1] += fast_exp2(z[c][h + 1] - m[h + 1]);
-            const bool seen = z[c][h] != -INFINITY || z[c][h + 1] != -INFINITY;
             float2 w = make_float2(fast_exp2(z[c][h] - M[h] + lv), fast_exp2(z[c][h + 1] - M[h + 1] + lv));
-            if (!seen) w = make_float2(0.f, 0.f);      // -inf plus the mark of a block that is not there
+            if (seen <= c) w = make_float2(0.f, 0.f);      // there may be no scale
 #pragma unroll
             for (int term = 0; term < 3; ++term) {
               const uint32_t code = e4m3x2(w.x, w.y);
@@ -595,12 +650,12 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
             }
           }
         // rows behind the last token may hold anything, NaN too: zero weights alone would not do
-        if ((q.t0 + t + 1) * L::TT > ctx || !there) {
-          ok = ok && wait(&v_full[stage], (tn / NST) & 1);
+        if (__any_sync(0xffffffffu, seen < PACK)) {
+          ok = ok && wait(&v_full[stage], round);
           uint8_t* v = smem + stage * L::kStage + 16384 + r * 128;
 #pragma unroll
           for (int c = 0; c < PACK; ++c)
-            if (!there || tok + c >= ctx)
+            if (seen <= c)
 #pragma unroll
               for (int i = 0; i < 8 / PACK; ++i)
                 *reinterpret_cast<uint4*>(v + (((c * (8 / PACK) + i) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
@@ -608,14 +663,11 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) mbar_arrive(&p_full[g]);
       }
       if (gone) break;
-      tile_no += q.n;
-      cur += q.n;
+      tn = stop;
       // sums over the warp: half of the heads go to the other half of the lanes at every step
-      float* stat = s_stat + ib * 6 * NR;
-      ok = ok && wait(&o_empty[ib], ((piece_no >> 1) & 1) ^ 1);
 #pragma unroll
       for (int n = NR, o = 16; o > 0; o >>= 1) {
         if (n > 1) {
@@ -631,9 +683,11 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
           l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
         }
       }
+      float* stat = s_stat + (ib * 2 + g) * 6 * NR;
+      ok = ok && wait(&o_empty[ib], ((piece_no >> 1) & 1) ^ 1);
       constexpr int kLow = NR == 8 ? 2 : 1;      // lane bits below are copies
-      if ((lane & ((1 << kLow) - 1)) == 0) stat[warp * NR + (lane >> kLow)] = l[0];
-      if (warp == 0) {
+      if ((lane & ((1 << kLow) - 1)) == 0) stat[quarter * NR + (lane >> kLow)] = l[0];
+      if (quarter == 0) {
 #pragma unroll
         for (int h = 0; h < NR; ++h)
           if (lane == h) {
@@ -642,41 +696,62 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
           }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&o_full[ib]);
+      if (lane == 0) {
+        mbar_arrive(&q_empty[iq]);
+        mbar_arrive(&o_full[ib]);
+      }
     }
   } else {
-    // ------------------------------ output: thread = byte of a row ------------------------------
-    const int quarter = warp - 4, byte = quarter * 32 + lane, d = byte % D, c = byte / D;
+    // ------------------------------ idle slots, then output: thread = byte of a row ------------------------------
+    const int quarter = warp & 3, byte = quarter * 32 + lane, d = byte % D, c = byte / D;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    for (int b = blockIdx.x * 4 + quarter; b < p.B; b += gridDim.x * 4) {
+      if (s_len[b] > 0) continue;
+      uint4* row = reinterpret_cast<uint4*>(p.out + (size_t)b * p.Hq * D);
+      for (int i = lane; i < p.Hq * D / 8; i += 32) row[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
     uint32_t piece_no = 0;
+    D8Piece q;
+    if (begin < end) q = d8_piece(s_pre, p.B, entries, begin, end);
     for (int cur = begin; cur < end; ++piece_no) {
-      const D8Piece q = d8_piece(s_pre, p.B, entries, cur, end);
+      if (cur != begin) d8_next(s_pre, entries, q, cur, end);
       const uint32_t ib = piece_no & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(&o_full[ib], (piece_no >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
       tc_fence_after();
-      float o[NR];
-      {
-        uint32_t x[3][NR];
-        const uint32_t at = tmem_base + lane_off + L::kTmemO + ib * L::NO + c * 3 * NR;
+      // lane h: head h's factors of the two O^T, and its log-sum-exp
+      float f[2] = {0.f, 0.f}, lse = -INFINITY;
+      if (lane < NR) {
+        const float* stat = s_stat + ib * 12 * NR + lane;
+        float l[2], m = kQ8None, sum = 0.f;
 #pragma unroll
-        for (int term = 0; term < 3; ++term) {
-          if constexpr (NR == 8) tmem_ld_32x8(at + term * NR, x[term]);
-          else tmem_ld_32x16(at + term * NR, x[term]);
+        for (int g = 0; g < 2; ++g) {
+          const float* x = stat + g * 6 * NR;
+          l[g] = (x[0] + x[NR]) + (x[2 * NR] + x[3 * NR]);
+          m = fmaxf(m, x[4 * NR]);
         }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) sum += l[g] == 0.f ? 0.f : l[g] * fast_exp2(stat[(6 * g + 4) * NR] - m);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) f[g] = l[g] == 0.f ? 0.f : fast_exp2(stat[(6 * g + 5) * NR] - m) / sum;
+        lse = sum == 0.f ? -INFINITY : m + log2f(sum);
+      }
+      float o[NR];
+#pragma unroll
+      for (int h = 0; h < NR; ++h) o[h] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (q.n == 1 && g != (cur - begin & 1)) continue;      // one tile: the other group's O^T has not been written
+        uint32_t x[3][NR];
+        const uint32_t at = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO + c * 3 * NR;
+#pragma unroll
+        for (int term = 0; term < 3; ++term) tmem_ld_heads(at + term * NR, x[term]);
         tmem_ld_wait();
 #pragma unroll
-        for (int h = 0; h < NR; ++h)
-          o[h] = fmaf(fmaf(__uint_as_float(x[2][h]), 0.0625f, __uint_as_float(x[1][h])), 0.0625f, __uint_as_float(x[0][h]));
-      }
-      const float* stat = s_stat + ib * 6 * NR;
-      float lse = -INFINITY;
-#pragma unroll
-      for (int h = 0; h < NR; ++h) {
-        const float sum = (stat[h] + stat[NR + h]) + (stat[2 * NR + h] + stat[3 * NR + h]);
-        const float m = stat[4 * NR + h];
-        o[h] *= sum == 0.f ? 0.f : fast_exp2(stat[5 * NR + h] - m) / sum;
-        if (lane == h && sum > 0.f) lse = m + log2f(sum);
-        if (lane == h && sum != sum) lse = sum;
+        for (int h = 0; h < NR; ++h) {
+          const float a = fmaf(fmaf(__uint_as_float(x[2][h]), 0.0625f, __uint_as_float(x[1][h])), 0.0625f, __uint_as_float(x[0][h]));
+          const float w = __shfl_sync(0xffffffffu, f[g], h);
+          o[h] += w == 0.f ? 0.f : a * w;
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -698,25 +773,25 @@ __global__ void __launch_bounds__(384, 1) fmha_decode8_kernel(const __grid_const
         }
       }
       if (c == 0) {
-        const int group = q.entry % p.groups, left = min(per_group, rep - group * per_group);
-        const int head0 = q.entry / p.groups * rep + group * per_group;
+        const int left = heads_of(q.entry);
         const int slot = 2 * blockIdx.x + (cur == begin ? 0 : 1);
-        __nv_bfloat16* orow = p.out + ((size_t)q.row * p.Hq + head0) * D + d;
+        const bool whole = q.n == q.tiles;
+        __nv_bfloat16* orow = p.out + ((size_t)q.row * p.Hq + first_head(q.entry)) * D + d;
         float* wrow = p.ws_o + (size_t)slot * NR * D + d;
 #pragma unroll
         for (int h = 0; h < NR; ++h)
           if (h < left) {
-            if (q.whole) orow[h * D] = __float2bfloat16(o[h]);
+            if (whole) orow[h * D] = __float2bfloat16(o[h]);
             else wrow[h * D] = o[h];
           }
-        if (!q.whole && quarter == 0 && lane < NR) p.ws_lse[(size_t)slot * NR + lane] = lse;
+        if (!whole && quarter == 0 && lane < NR) p.ws_lse[(size_t)slot * NR + lane] = lse;
       }
       cur += q.n;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 13) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
   }
@@ -758,7 +833,7 @@ __global__ void __launch_bounds__(128) fmha_decode8_merge_kernel(Decode8Params p
 template <int D, int NR>
 static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int grid, cudaStream_t stream) {
   using L = D8<D, NR>;
-  static_assert(L::kStages >= 4 && L::kTotal <= kQ8Smem && 2 * (L::NS + L::NO) <= 512, "");
+  static_assert(L::kStages >= 4 && L::kTotal <= kQ8Smem && 2 * L::NS + 4 * L::NO <= 512 && L::kTotal % 4 == 0, "");
   auto kernel = fmha_decode8_kernel<D, NR>;
   static int configured = -1;
   int dev = 0;
@@ -768,7 +843,7 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
     if (e != cudaSuccess) return (int)e;
     configured = dev;
   }
-  const int rc = launch_chained(kernel, (unsigned)grid, 384, L::kTotal, stream, mc, p);
+  const int rc = launch_chained(kernel, (unsigned)grid, kQ8Threads, L::kTotal, stream, mc, p);
   if (rc || p.max_blocks <= L::BPT) return rc;      // one tile per entry: nothing is split
   return launch_chained(fmha_decode8_merge_kernel<D, NR>, dim3(p.B, p.Hkv * p.groups), 128, 0, stream, p, grid);
 }
