@@ -852,9 +852,8 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
 
 using namespace sb;
 
-// Query heads of a group (rows of a partial result): ws_o = 2 * num_sms * rows * D floats, ws_lse = 2 * num_sms * rows,
-// ws_pre = B + 1 ints.
-extern "C" int sb_kv8_decode_rows(int Hq, int Hkv) { return Hq / Hkv <= 8 ? 8 : 16; }
+// Workspaces: with rows = 8 where at most 8 query heads share a kv head, else 16, ws_o has 2 * grid * rows * D floats,
+// ws_lse 2 * grid * rows, ws_pre B + 1 ints.
 extern "C" int sb_kv8_decode_grid() { return num_sms(); }
 
 // One query row per sequence (at most 1024) against its cached context of seq_lens[b] tokens, the current one included; 0: idle

@@ -151,7 +151,6 @@ int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long long slab_
 int sb_kv8_copy_blocks(void* codes, float* scales, const int* src, const int* dst, int n_pairs, int num_blocks,
                        int per_block, long long bytes, cudaStream_t stream);
 // ---- fmha_decode8.cu ----
-int sb_kv8_decode_rows(int Hq, int Hkv);
 int sb_kv8_decode_grid();
 int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const float* scales, int num_blocks,
                   const int* seq_lens, const int* block_table, int max_blocks, void* out, float* ws_o, float* ws_lse,

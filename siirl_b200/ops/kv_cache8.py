@@ -49,33 +49,41 @@ def block_bytes(n_kv_heads: int, head_dim: int) -> int:
     return 2 * n_kv_heads * (BLOCK * head_dim + 4)
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(f"8-bit cache: {what}")
+def _refuse(what: str) -> None:
+    raise ValueError(f"8-bit cache: {what}")
 
 
-def _check(cache: Cache8, n_heads: int, n_kv_heads: int, head_dim: int, rows: torch.Tensor, *ints: torch.Tensor) -> None:
+# The checks below run before every call of a decoding step: one expression each, and words only where it fails.
+def _check(cache: Cache8, n_heads: int, n_kv_heads: int, head_dim: int, rows: torch.Tensor) -> None:
     codes, scales = cache
-    _require(codes.dtype == torch.float8_e4m3fn and scales.dtype == torch.float32, "codes are float8_e4m3fn, scales float32")
-    _require(codes.dim() == 5 and tuple(codes.shape[1:]) == (2, n_kv_heads, BLOCK, head_dim),
-             f"codes are [blocks, 2, {n_kv_heads}, {BLOCK}, {head_dim}], got {tuple(codes.shape)}")
-    _require(scales.shape == codes.shape[:3], f"scales are {tuple(codes.shape[:3])}, got {tuple(scales.shape)}")
-    _require(codes.is_contiguous() and scales.is_contiguous(), "codes and scales are contiguous")
-    _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} query heads on {n_kv_heads} kv heads")
-    dev = rows.device
-    _require(codes.device == dev and scales.device == dev, "cache and rows are on one device")
+    shape = codes.shape
+    if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
+        _refuse(f"codes are float8_e4m3fn, scales float32, got {codes.dtype}, {scales.dtype}")
+    if shape != (shape[0], 2, n_kv_heads, BLOCK, head_dim) or scales.shape != (shape[0], 2, n_kv_heads):
+        _refuse(f"codes are [blocks, 2, {n_kv_heads}, {BLOCK}, {head_dim}], scales [blocks, 2, {n_kv_heads}], got "
+                f"{tuple(codes.shape)}, {tuple(scales.shape)}")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        _refuse("codes and scales are contiguous")
+    if n_heads <= 0 or n_heads % n_kv_heads:
+        _refuse(f"{n_heads} query heads on {n_kv_heads} kv heads")
+    dev = rows.get_device()
+    if codes.get_device() != dev or scales.get_device() != dev:
+        _refuse("cache and rows are on one device")
+    if dev >= 0 and (head_dim not in HEAD_DIMS or n_heads > 32 * n_kv_heads or codes.data_ptr() % 16):
+        _refuse(f"the kernels take head widths {HEAD_DIMS}, at most 32 query heads per kv head and codes that start on a 16-byte "
+                f"boundary, not {head_dim}, {n_heads} / {n_kv_heads}, {codes.data_ptr() % 16}")
+
+
+def _check_ints(rows: torch.Tensor, *ints: torch.Tensor) -> None:
+    dev = rows.get_device()
     for t in ints:
-        _require(t.dtype == torch.int32 and t.device == dev and t.is_contiguous(),
-                 "lengths, ids, positions and block tables are contiguous int32 tensors on the rows' device")
-    if rows.is_cuda:
-        _require(head_dim in HEAD_DIMS, f"the kernels take head widths {HEAD_DIMS}, not {head_dim}")
-        _require(n_heads // n_kv_heads <= 32, f"at most 32 query heads share a kv head, not {n_heads // n_kv_heads}")
-        _require(codes.data_ptr() % 16 == 0, "codes start on a 16-byte boundary")
+        if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+            _refuse("lengths, ids, positions and block tables are contiguous int32 tensors on the rows' device")
 
 
-def _device(t: torch.Tensor):
-    """Makes the tensor's device current where it is not."""
-    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+def _device(index: int):
+    """Makes a device current where it is not."""
+    return contextlib.nullcontext() if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 # ---- appending ----------------------------------------------------------------------------------
@@ -116,26 +124,38 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
     ``bias`` is rotated and returned as bf16 rows."""
     slabs = qkv if qkv.dim() == 3 else None
     T, width = qkv.shape[-2:]
-    _require(width == (n_heads + 2 * n_kv_heads) * head_dim, f"rows are {(n_heads + 2 * n_kv_heads) * head_dim} wide, got {width}")
-    _require(seq_ids.shape == (T,) and positions.shape == (T,), f"one sequence and position for each of {T} rows")
-    _check(cache, n_heads, n_kv_heads, head_dim, qkv, seq_ids, positions, block_table)
-    if slabs is not None:
-        _require(slabs.dtype == torch.float32 and slabs.is_contiguous() and slabs.shape[0] > 0, "partial sums are contiguous float32")
-        _require(bias is None or bias.numel() == width and bias.is_contiguous() and bias.device == qkv.device and
-                 bias.dtype == torch.bfloat16, f"the bias is {width} bf16 numbers")
-    else:
-        _require(bias is None, "a bias is added to partial sums only")
+    if width != (n_heads + 2 * n_kv_heads) * head_dim:
+        _refuse(f"rows are {(n_heads + 2 * n_kv_heads) * head_dim} wide, got {width}")
+    if seq_ids.shape != (T,) or positions.shape != (T,) or block_table.dim() != 2:
+        _refuse(f"one sequence and position for each of {T} rows, and a table of blocks for each sequence")
+    _check(cache, n_heads, n_kv_heads, head_dim, qkv)
+    _check_ints(qkv, seq_ids, positions, block_table)
+    dev = qkv.get_device()
+    if slabs is None:
+        if bias is not None:
+            _refuse("a bias is added to partial sums only")
+    elif slabs.dtype is not torch.float32 or not slabs.is_contiguous() or slabs.shape[0] == 0:
+        _refuse("partial sums are contiguous float32")
+    elif bias is not None and (bias.shape != (width,) or not bias.is_contiguous() or bias.get_device() != dev or
+                               bias.dtype is not torch.bfloat16):
+        _refuse(f"the bias is {width} bf16 numbers")
     pos = cos = sin = None
     s0 = s1 = rows = 0
     if rope is not None:
         pos, cos, sin, section = rope
-        pos = pos.to(torch.int32).contiguous()
+        if pos.dtype is not torch.int32 or not pos.is_contiguous():
+            pos = pos.to(torch.int32).contiguous()
         rows = 1 if pos.dim() == 1 else pos.shape[0]
-        _require(pos.shape[-1] == T and rows in (1, 3) and pos.device == qkv.device, f"rope positions are [{T}] or [3, {T}]")
-        for t in (cos, sin):
-            _require(t.dtype == torch.float32 and t.is_contiguous() and t.shape[-1] == head_dim // 2 and t.device == qkv.device,
-                     f"cos and sin are contiguous float32 tables of width {head_dim // 2}")
+        if pos.shape[-1] != T or pos.numel() != rows * T or rows not in (1, 3) or pos.get_device() != dev:
+            _refuse(f"rope positions are [{T}] or [3, {T}]")
+        table = cos.shape
+        if len(table) != 2 or table[1] != head_dim // 2 or not table[0] or sin.shape != table or \
+                cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or not cos.is_contiguous() or \
+                not sin.is_contiguous() or cos.get_device() != dev or sin.get_device() != dev:
+            _refuse(f"cos and sin are contiguous float32 tables of width {head_dim // 2}")
         if rows == 3:
+            if section is None or len(section) < 2:
+                _refuse("positions of three axes come with the sections of the rotated pairs")
             s0, s1 = section[0], section[0] + section[1]
     if not qkv.is_cuda:
         if slabs is not None:
@@ -155,15 +175,18 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
         return qkv
     if slabs is not None:
         qkv = torch.empty(T, width, dtype=torch.bfloat16, device=slabs.device)
-    _require(qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0,
-             "rows are bf16 numbers next to one another, from an even one on")
-    with _device(qkv):
+    stride, one = qkv.stride()
+    if qkv.dtype is not torch.bfloat16 or one != 1 or stride % 2 or qkv.data_ptr() % 4 or stride < width and T > 1:
+        _refuse("rows are bf16 numbers next to one another, from an even one on, and do not overlap")
+    codes, scales = cache
+    sequences, max_blocks = block_table.shape
+    with _device(dev):
         _lib.check(_lib.get_lib().sb_kv8_append(
-            _lib.ptr(qkv), qkv.stride(0), _lib.ptr(slabs), ctypes.c_longlong(qkv.numel()), 0 if slabs is None else slabs.shape[0],
-            _lib.ptr(bias), _lib.ptr(pos), rows, s0, s1, 0 if cos is None else cos.shape[0], _lib.ptr(cos), _lib.ptr(sin),
-            _lib.ptr(seq_ids), _lib.ptr(positions), _lib.ptr(block_table), block_table.shape[0], block_table.shape[1],
-            _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0], T, n_heads, n_kv_heads, head_dim,
-            _lib.stream()), "sb_kv8_append")
+            qkv.data_ptr(), stride, 0 if slabs is None else slabs.data_ptr(), T * width,
+            0 if slabs is None else slabs.shape[0], 0 if bias is None else bias.data_ptr(), 0 if pos is None else pos.data_ptr(),
+            rows, s0, s1, 0 if cos is None else table[0], 0 if cos is None else cos.data_ptr(),
+            0 if sin is None else sin.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
+            sequences, max_blocks, codes.data_ptr(), scales.data_ptr(), codes.shape[0], T, n_heads, n_kv_heads, head_dim, _lib.stream()), "sb_kv8_append")
     return qkv
 
 
@@ -174,9 +197,11 @@ def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
         codes.view(torch.uint8)[dst.long()] = codes.view(torch.uint8)[src.long()]
         scales[dst.long()] = scales[src.long()]
         return
-    _check(cache, codes.shape[2], codes.shape[2], codes.shape[4], codes, src, dst)
-    _require(src.shape == dst.shape and src.dim() == 1, "as many sources as destinations")
-    with _device(codes):
+    _check(cache, codes.shape[2], codes.shape[2], codes.shape[4], codes)
+    _check_ints(codes, src, dst)
+    if src.shape != dst.shape or src.dim() != 1:
+        _refuse("as many sources as destinations")
+    with _device(codes.get_device()):
         _lib.check(_lib.get_lib().sb_kv8_copy_blocks(
             _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(src), _lib.ptr(dst), src.numel(), codes.shape[0], 2 * codes.shape[2],
             ctypes.c_longlong(codes[0].numel()), _lib.stream()), "sb_kv8_copy_blocks")
@@ -189,13 +214,16 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
     """:func:`siirl_b200.ops.kv_cache.decode_attention` on an 8-bit cache."""
     B, width = q_rows.shape[0], n_heads * head_dim
     scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
-    _check(cache, n_heads, n_kv_heads, head_dim, q_rows, seq_lens, block_table)
-    _require(q_rows.dim() == 2 and q_rows.shape[1] >= width and q_rows.stride(1) == 1, f"query rows are at least {width} wide")
-    _require(seq_lens.shape == (B,) and block_table.dim() == 2 and block_table.shape[0] >= B, f"a length and a row of the table for each of {B} rows")
+    _check(cache, n_heads, n_kv_heads, head_dim, q_rows)
+    _check_ints(q_rows, seq_lens, block_table)
+    if q_rows.dim() != 2 or q_rows.shape[1] < width or q_rows.stride(1) != 1:
+        _refuse(f"query rows are at least {width} wide")
+    if seq_lens.shape != (B,) or block_table.dim() != 2 or block_table.shape[0] < B:
+        _refuse(f"a length and a row of the table for each of {B} rows")
     if out is None:
         out = torch.empty(B, width, dtype=q_rows.dtype, device=q_rows.device)
-    _require(out.shape == (B, width) and out.is_contiguous() and out.dtype == q_rows.dtype and out.device == q_rows.device,
-             f"the output is a contiguous [{B}, {width}] of the rows' type")
+    elif out.shape != (B, width) or not out.is_contiguous() or out.dtype != q_rows.dtype or out.get_device() != q_rows.get_device():
+        _refuse(f"the output is a contiguous [{B}, {width}] of the rows' type")
     if not q_rows.is_cuda:
         rep = n_heads // n_kv_heads
         out.zero_()
@@ -208,27 +236,27 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
             s = torch.einsum("hd,hnd->hn", q_rows[b, :width].reshape(n_heads, head_dim).float(), k) * scale
             out[b] = torch.einsum("hn,hnd->hd", torch.softmax(s, -1), v).reshape(-1).to(out.dtype)
         return out
-    _require(q_rows.dtype == torch.bfloat16, "query rows are bf16")
+    if q_rows.dtype is not torch.bfloat16:
+        _refuse("query rows are bf16")
     if q_rows.stride(0) % 2 or q_rows.data_ptr() % 4:
         q_rows = q_rows[:, :width].contiguous()
     L = _lib.get_lib()
-    with _device(q_rows):
-        grid, rows = L.sb_kv8_decode_grid(), L.sb_kv8_decode_rows(n_heads, n_kv_heads)
+    codes, scales = cache
+    stride, max_blocks = q_rows.stride(0), block_table.shape[1]
+    with _device(q_rows.get_device()):
+        part = 2 * L.sb_kv8_decode_grid() * (8 if n_heads <= 8 * n_kv_heads else 16)
         for at in range(0, B, ROWS):
             n = min(ROWS, B - at)
             # two partial results per block of the grid, and the sequences' places in the list of tiles.  A buffer of the
             # call's own: calls on other streams and graphs that hold one write to theirs
-            ws = torch.empty(2 * grid * rows * (head_dim + 1) + n + 1, dtype=torch.float32, device=q_rows.device)
-            o, e = ws.data_ptr(), 2 * grid * rows
+            ws = torch.empty(part * (head_dim + 1) + n + 1, dtype=torch.float32, device=q_rows.device)
+            o = ws.data_ptr()
             _lib.check(L.sb_kv8_decode(
-                ctypes.c_void_p(q_rows.data_ptr() + 2 * at * q_rows.stride(0)), ctypes.c_longlong(q_rows.stride(0)),
-                _lib.ptr(cache.codes), _lib.ptr(cache.scales), cache.codes.shape[0],
-                ctypes.c_void_p(seq_lens.data_ptr() + 4 * at),
-                ctypes.c_void_p(block_table.data_ptr() + 4 * at * block_table.shape[1]), block_table.shape[1],
-                ctypes.c_void_p(out.data_ptr() + 2 * at * width), ctypes.c_void_p(o), ctypes.c_void_p(o + 4 * e * head_dim),
-                ctypes.c_void_p(o + 4 * e * (head_dim + 1)), n, n_heads, n_kv_heads, head_dim, ctypes.c_float(scale),
-                _lib.ptr(_lib.status_word(q_rows.device)), _lib.stream()), "sb_kv8_decode")
-            _lib.add_launches(int(block_table.shape[1] > 2 * 128 // head_dim))      # ranges' shares are merged
+                q_rows.data_ptr() + 2 * at * stride, stride, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+                seq_lens.data_ptr() + 4 * at, block_table.data_ptr() + 4 * at * max_blocks, max_blocks,
+                out.data_ptr() + 2 * at * width, o, o + 4 * part * head_dim, o + 4 * part * (head_dim + 1), n, n_heads,
+                n_kv_heads, head_dim, scale, _lib.status_word(q_rows.device).data_ptr(), _lib.stream()), "sb_kv8_decode")
+            _lib.add_launches(int(max_blocks > 2 * 128 // head_dim))      # ranges' shares are merged
     return out
 
 
@@ -236,12 +264,16 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
 def check_chunks(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Cache8, block_table: torch.Tensor, n_heads: int,
                  n_kv_heads: int, head_dim: int) -> None:
     """Refuses chunks that the cache or the rows cannot hold."""
-    _check(cache, n_heads, n_kv_heads, head_dim, qkv, block_table)
-    _require(len(chunk_lens) == len(prefix_lens) == len(slots), "a chunk, a prefix and a slot for each sequence")
+    _check(cache, n_heads, n_kv_heads, head_dim, qkv)
+    _check_ints(qkv, block_table)
+    if not len(chunk_lens) == len(prefix_lens) == len(slots):
+        _refuse("a chunk, a prefix and a slot for each sequence")
     rows, width = sum(chunk_lens), (n_heads + 2 * n_kv_heads) * head_dim
-    _require(qkv.dim() == 2 and qkv.shape == (rows, width), f"{rows} rows of {width} numbers, got {tuple(qkv.shape)}")
+    if qkv.shape != (rows, width):
+        _refuse(f"{rows} rows of {width} numbers, got {tuple(qkv.shape)}")
+    slots_held, tokens_held = block_table.shape[0], block_table.shape[1] * BLOCK
     for c, p, s in zip(chunk_lens, prefix_lens, slots):
-        _require(c >= 0 and p >= 0 and 0 <= s < block_table.shape[0] and c + p <= block_table.shape[1] * BLOCK,
-                 f"slot {s} of {block_table.shape[0]} with {p} + {c} tokens in {block_table.shape[1]} blocks")
-    if qkv.is_cuda:
-        _require(qkv.dtype == torch.bfloat16, "rows are bf16")
+        if c < 0 or p < 0 or not 0 <= s < slots_held or c + p > tokens_held:
+            _refuse(f"slot {s} of {slots_held} with {p} + {c} tokens of {tokens_held}")
+    if qkv.is_cuda and qkv.dtype is not torch.bfloat16:
+        _refuse("rows are bf16")

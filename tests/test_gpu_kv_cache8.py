@@ -29,7 +29,7 @@ def _gpu(cache):
 def _check_append(cache, rows, pos, section, seq, at, table, hq, hkv, d, slabs=0, bias=None, rope=True):
     """One call on the GPU against the definition.  Bounds: a rotated value is a * c - b * s in 32 bits (three roundings of
     2^-24 of |a| + |b|), sums of S partial sums add S + 1 more; bf16 rows half a step, codes half a step of e4m3."""
-    cos, sin = ref.rope_tables(d, 512, 1e4)
+    cos, sin = ref.rope_tables(d, 1600, 1e4)
     if rope is False:
         cos = sin = None
     g = _gpu(cache)
@@ -120,6 +120,26 @@ def test_append_chunks(hq, hkv, d, lens, starts):
     pos = torch.stack([at, at // 2, at // 3 + 7])
     _check_append(cache, x.bfloat16(), pos, (d // 8, d // 4, d // 8), seq, at, table, hq, hkv, d)
     _check_append(cache, x.bfloat16(), pos, None, seq, at, table, hq, hkv, d, rope=False)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(5, 1, 128), (6, 2, 64)])
+def test_append_long_batches(hq, hkv, d):
+    """More rows than the ranges of small batches, runs of every kind in one range, idle rows among them, runs of one place."""
+    lens, starts = [900, 1, 1, 7, 9, 64, 8, 1100, 70, 3], [5, 63, 0, 60, 0, 64, 10, 0, 130, 126]
+    test_append_chunks(hq, hkv, d, lens, starts)
+    n, nb = 2500, 80
+    cache = _random_cache(nb, hkv, d)
+    table = torch.randperm(nb).to(torch.int32).view(8, 10)
+    seq, at = torch.full((n,), -1, dtype=torch.int32), torch.zeros(n, dtype=torch.int32)
+    place = 0
+    for i, (b, rows) in enumerate([(0, 1), (1, 100), (2, 8), (3, 65), (4, 64), (5, 9), (6, 7), (7, 200), (8, 70)] * 4):
+        j = b + 9 * (i // 9)
+        seq[place + 2:place + 2 + rows] = j // 10
+        at[place + 2:place + 2 + rows] = j % 10 * 64 + torch.randint(0, 64, (rows,))      # places named twice
+        place += rows + 2
+    assert place < n
+    x = torch.randn(n, (hq + 2 * hkv) * d).bfloat16()
+    _check_append(cache, x, at, None, seq, at, table, hq, hkv, d)
 
 
 def test_append_odd_values_and_places_named_twice():
