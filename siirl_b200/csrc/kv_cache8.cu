@@ -141,105 +141,211 @@ struct RowLanes {
     write_back(r, x);
   }
 
-  // rows t .. end - 1, which all lie in block `blk`: one after the other, so that a place named twice gets its last values
-  __device__ __forceinline__ void append(int t, int end, int blk) const {
+  // of the head in block `blk`: its place among the scales, and its scale once the numbers of `amax` have joined; the rows that
+  // `written` does not name follow a new one
+  __device__ __forceinline__ size_t place(int blk) const {
     const int kv = head >= p.Hq + p.Hkv ? 1 : 0;
-    const size_t at = ((size_t)blk * 2 + kv) * p.Hkv + (head - p.Hq - kv * p.Hkv);
-    const float before = p.scales[at];      // asked for ahead of the rows
-    float x[4], amax = 0.f;
-    unsigned long long written = 0;
-    for (int r = t; r < end; ++r) {
-      load(r, x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(x[i]));
-      written |= 1ull << (p.cache_pos[r] % kB8);
-    }
+    return ((size_t)blk * 2 + kv) * p.Hkv + (head - p.Hq - kv * p.Hkv);
+  }
+  __device__ __forceinline__ float rescale(size_t at, float before, float amax, unsigned long long written) const {
 #pragma unroll
     for (int o = N / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-    uint8_t* dst = p.codes + at * kB8 * D;
     const bool anew = written & 1;
-    const float kept = anew ? 0.f : before;
-    const float scale = fmaxf(kept, scale_of(amax));
+    const float kept = anew ? 0.f : before, scale = fmaxf(kept, scale_of(amax));
     if (scale != kept) {
       __syncwarp(mask);      // every lane has read the old scale
       const float ratio = kept / scale;
-#pragma unroll 8
-      for (int r = 0; r < kB8; ++r) {
-        if (written >> r & 1) continue;
-        uint32_t* c = reinterpret_cast<uint32_t*>(dst + r * D) + l;
-        *c = anew ? 0u : rescaled(*c, ratio);
-      }
+      uint32_t* c = reinterpret_cast<uint32_t*>(p.codes + at * kB8 * D) + l;
+#pragma unroll 4
+      for (int r = 0; r < kB8; ++r)
+        if (!(written >> r & 1)) c[r * N] = anew ? 0u : rescaled(c[r * N], ratio);
       if (l == 0) p.scales[at] = scale;
     }
-    const float inv = 1.f / scale;
-    const bool one = end == t + 1;
+    return 1.f / scale;
+  }
+  __device__ __forceinline__ void store(size_t at, int off, const float (&x)[4], float inv) const {
+    uint8_t* c = p.codes + (at * kB8 + off) * D + 2 * l;
+    *reinterpret_cast<uint16_t*>(c) = (uint16_t)codes_of(x[0] * inv, x[1] * inv);
+    *reinterpret_cast<uint16_t*>(c + half) = (uint16_t)codes_of(x[2] * inv, x[3] * inv);
+  }
+  __device__ __forceinline__ static float largest(const float (&x)[4]) {
+    return fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+  }
+
+  // row t in block `blk`, whose scale is `before`
+  __device__ __forceinline__ void append(int t, int blk, const float (&x)[4], float before) const {
+    const int off = p.cache_pos[t] % kB8;
+    const size_t at = place(blk);
+    const float inv = rescale(at, before, largest(x), 1ull << off);
+    write_back(t, x);
+    store(at, off, x, inv);
+  }
+  // rows t .. end - 1, one after the other, so that a place named twice gets its last values
+  __device__ __forceinline__ void append(int t, int end, int blk) const {
+    const size_t at = place(blk);
+    const float before = p.scales[at];
+    float x[4], amax = 0.f;
+    unsigned long long written = 0;
+#pragma unroll 1
     for (int r = t; r < end; ++r) {
-      if (!one) load(r, x);
+      load(r, x);
+      amax = fmaxf(amax, largest(x));
+      written |= 1ull << (p.cache_pos[r] % kB8);
+    }
+    const float inv = rescale(at, before, amax, written);
+#pragma unroll 1
+    for (int r = t; r < end; ++r) {
+      load(r, x);
       write_back(r, x);
-      uint8_t* c = dst + (p.cache_pos[r] % kB8) * D + 2 * l;
-      *reinterpret_cast<uint16_t*>(c) = (uint16_t)codes_of(x[0] * inv, x[1] * inv);
-      *reinterpret_cast<uint16_t*>(c + half) = (uint16_t)codes_of(x[2] * inv, x[3] * inv);
+      store(at, p.cache_pos[r] % kB8, x, inv);
     }
   }
 };
 
-// Rows of any alignment: the lanes that meet the first of the adjacent rows of a cache block do all of them.
+// Few rows, or rows of any alignment.  A block takes 1024 / D rows of a k or v head, D / 4 lanes each; single rows, as in a
+// decoding step, are done without meeting the others: everything they read is asked for first, so that three round trips lead
+// to the store (positions; block and angles; scale).  Of a run, the block that has its first row takes all rows at once.  The
+// other blocks rotate q heads.  Short on purpose: a step's time is latency, that of fetching the code too.
 template <int D>
-__global__ void __launch_bounds__(256) append8_lanes_kernel(Append8Params p) {
+__global__ void __launch_bounds__(256) append8_rows_kernel(Append8Params p, int kv_blocks) {
+  constexpr int LPH = D / 4, S = 256 / LPH;
+  __shared__ int s_first[S], s_last[kB8];
+  __shared__ uint32_t s_same[3], s_top[8];
   chain_sync();
-  const int heads = p.Hq + 2 * p.Hkv;
-  const long long unit = (blockIdx.x * 256ll + threadIdx.x) / (D / 4);
-  if (unit >= (long long)p.T * heads) return;
-  const int t = (int)(unit / heads), head = (int)(unit % heads);
-  const RowLanes<D> lanes(p, head);
-  const int blk = head < p.Hq ? -1 : block_of(p, t);
-  if (blk < 0) {
-    lanes.turn_only(t);
+  const int tid = threadIdx.x, sub = tid / LPH;
+  if ((int)blockIdx.x >= kv_blocks) {
+    const long long unit = (blockIdx.x - kv_blocks) * (long long)S + sub;
+    if (unit < (long long)p.T * p.Hq) RowLanes<D>(p, (int)(unit % p.Hq)).turn_only((int)(unit / p.Hq));
     return;
   }
-  if (t > 0 && block_of(p, t - 1) == blk) return;
-  int end = t + 1;
-  while (end < p.T && block_of(p, end) == blk) ++end;
-  lanes.append(t, end, blk);
-}
-
-// ---------------------------------------------------------------------------------------
-// Rows on 16-byte boundaries.  The first blocks of the grid take k and v heads: one head of `range` rows, of which those that
-// are the first of a cache block's adjacent rows count (the block that has the first has all of them, up to 64, also where
-// they reach beyond its range).  Runs of few rows go to D / 4 lanes each; of longer ones every thread holds a quarter of a row
-// in registers while the block finds the largest value, so that rows are read once.  The other blocks rotate q heads: a thread
-// keeps the eight angles of its pairs for `per` heads.
-//
-// Bound by memory: 28 / 4 heads, D = 128, 8992 rows of prompts: NOTE us for 170 MB.
-// ---------------------------------------------------------------------------------------
-constexpr int kRun = 8;      // rows from which on a run takes the whole block
-
-// eight pairs from element i0 on of one head of row r: the sum of the partial sums, or the row; not rotated
-template <int D>
-__device__ __forceinline__ void load_pairs(const Append8Params& p, int r, int head, int i0, float (&x)[8], float (&y)[8]) {
-  if (p.slabs) {
-    const float* src = p.slabs + ((size_t)r * (p.Hq + 2 * p.Hkv) + head) * D + i0;
-    slab_sum8(src, p.slab_stride, p.splits, x);
-    slab_sum8(src + D / 2, p.slab_stride, p.splits, y);
-    if (p.bias) {
-      const __nv_bfloat16* b = p.bias + head * D + i0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[k] += __bfloat162float(b[k]);
-        y[k] += __bfloat162float(b[D / 2 + k]);
-      }
+  const int hd = blockIdx.x % (2 * p.Hkv), r0 = blockIdx.x / (2 * p.Hkv) * S, t = r0 + sub;
+  const RowLanes<D> lanes(p, p.Hq + hd);
+  bool several = false;
+  if (t < p.T) {
+    float x[4];
+    const int blk = block_of(p, t), prev = t > 0 ? block_of(p, t - 1) : -1, next = t + 1 < p.T ? block_of(p, t + 1) : -1;
+    if (blk < 0 || (blk != prev && blk != next)) {
+      lanes.load(t, x);
+      if (blk < 0) lanes.write_back(t, x);
+      else lanes.append(t, blk, x, p.scales[lanes.place(blk)]);
     }
-  } else {
-    const __nv_bfloat16* src = p.qkv + (size_t)r * p.row_stride + (size_t)head * D + i0;
-    const uint4 a = *reinterpret_cast<const uint4*>(src), b = *reinterpret_cast<const uint4*>(src + D / 2);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w}, v[4] = {b.x, b.y, b.z, b.w};
+    several = blk >= 0 && blk != prev && blk == next;
+  }
+  if (tid % LPH == 0) s_first[sub] = several ? t : -1;
+  if (!__syncthreads_or(several)) return;
+  for (int i = 0; i < S; ++i) {
+    const int first = s_first[i];
+    if (first < 0) continue;
+    const int blk = block_of(p, first);
+    __syncthreads();      // the run before has been done
+    if (tid < 96) {
+      const int r = first + tid;
+      const uint32_t same = __ballot_sync(0xffffffffu, tid <= kB8 && r < p.T && block_of(p, r) == blk);
+      if ((tid & 31) == 0) s_same[tid >> 5] = same;
+    }
+    if (tid < kB8) s_last[tid] = -1;
+    __syncthreads();
+    // rows of the run: up to the first that is elsewhere
+    const int n = ~s_same[0] ? __ffs(~s_same[0]) - 1 : ~s_same[1] ? 31 + __ffs(~s_same[1]) : 63 + __ffs(~s_same[2]);
+    if (n > kB8) {        // some place is named twice, and the last row counts
+      if (sub == 0) {
+        int end = first + n;
+        while (end < p.T && block_of(p, end) == blk) ++end;
+        lanes.append(first, end, blk);
+      }
+      continue;
+    }
+    const size_t at = lanes.place(blk);
+    const float before = p.scales[at];
+    constexpr int M = kB8 / S;
+    float x[M][4], amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-      y[2 * k] = __uint_as_float(v[k] << 16); y[2 * k + 1] = __uint_as_float(v[k] & 0xffff0000u);
+    for (int k = 0; k < M; ++k) {
+      const int row = k * S + sub;
+      if (row >= n) continue;
+      lanes.load(first + row, x[k]);
+      amax = fmaxf(amax, lanes.largest(x[k]));
+      if (tid % LPH == 0) atomicMax(&s_last[p.cache_pos[first + row] % kB8], row);
+    }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));      // of numbers >= 0, bits order as they do
+    if ((tid & 31) == 0) s_top[tid >> 5] = top;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all = max(all, s_top[w]);
+    const bool anew = s_last[0] >= 0;
+    const float kept = anew ? 0.f : before, scale = fmaxf(kept, scale_of(__uint_as_float(all))), inv = 1.f / scale;
+    if (scale != kept) {
+      uint32_t* c = reinterpret_cast<uint32_t*>(p.codes + at * kB8 * D) + lanes.l;
+#pragma unroll 4
+      for (int r = sub; r < kB8; r += S)
+        if (s_last[r] < 0) c[r * LPH] = anew ? 0u : rescaled(c[r * LPH], kept / scale);
+      if (tid == 0) p.scales[at] = scale;
+    }
+#pragma unroll
+    for (int k = 0; k < M; ++k) {
+      const int row = k * S + sub;
+      if (row >= n) continue;
+      lanes.write_back(first + row, x[k]);
+      const int off = p.cache_pos[first + row] % kB8;
+      if (s_last[off] == row) lanes.store(at, off, x[k], inv);
     }
   }
 }
+
+// ---------------------------------------------------------------------------------------
+// Rows on 16-byte boundaries.  The first blocks of the grid take k and v heads: some heads of 64 rows, of which those that
+// are the first of a cache block's adjacent rows count (the block that has the first has all of them, up to 64, also where
+// they reach beyond its range).  Single rows go to D / 4 lanes each; of more, every thread holds eight pairs in registers
+// while the block finds the largest value, so that rows are read once.  The other blocks rotate q heads: a thread
+// keeps the eight angles of its pairs for `per` heads.
+//
+// Bound by memory: 28 / 4 heads, D = 128, 8992 rows of 24 prompts (170 MB): 48 us; 32 / 8 heads, 32653 rows (819 MB): 177 us,
+// 4.6 TB/s.
+// ---------------------------------------------------------------------------------------
+
+// Eight pairs from element i0 on of one head of a row, as they are asked for: bf16 numbers, or (SLABS) the sum of the partial
+// sums and the bias; not rotated
+template <int D, bool SLABS>
+struct Pairs {
+  uint4 a, b;
+  float x[SLABS ? 8 : 1], y[SLABS ? 8 : 1];
+  __device__ __forceinline__ void load(const Append8Params& p, int r, int head, int i0) {
+    if constexpr (SLABS) {
+      const float* src = p.slabs + ((size_t)r * (p.Hq + 2 * p.Hkv) + head) * D + i0;
+      slab_sum8(src, p.slab_stride, p.splits, x);
+      slab_sum8(src + D / 2, p.slab_stride, p.splits, y);
+      if (p.bias) {
+        const __nv_bfloat16* v = p.bias + head * D + i0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          x[k] += __bfloat162float(v[k]);
+          y[k] += __bfloat162float(v[D / 2 + k]);
+        }
+      }
+    } else {
+      const __nv_bfloat16* src = p.qkv + (size_t)r * p.row_stride + (size_t)head * D + i0;
+      a = *reinterpret_cast<const uint4*>(src);
+      b = *reinterpret_cast<const uint4*>(src + D / 2);
+    }
+  }
+  __device__ __forceinline__ void get(float (&u)[8], float (&v)[8]) const {
+    if constexpr (SLABS) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        u[k] = x[k];
+        v[k] = y[k];
+      }
+    } else {
+      const uint32_t c[4] = {a.x, a.y, a.z, a.w}, d[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u[2 * k] = __uint_as_float(c[k] << 16); u[2 * k + 1] = __uint_as_float(c[k] & 0xffff0000u);
+        v[2 * k] = __uint_as_float(d[k] << 16); v[2 * k + 1] = __uint_as_float(d[k] & 0xffff0000u);
+      }
+    }
+  }
+};
 template <int D>
 __device__ __forceinline__ void load_angles(const Append8Params& p, int r, int i0, float (&c)[8], float (&s)[8]) {
   if (p.pos_rows == 3) {
@@ -278,36 +384,44 @@ __device__ __forceinline__ uint2 codes_of8(const float (&x)[8], float inv) {
                     codes_of(x[4] * inv, x[5] * inv) | codes_of(x[6] * inv, x[7] * inv) << 16);
 }
 
-template <int D>
-__global__ void __launch_bounds__(256) append8_kernel(Append8Params p, int kv_blocks, int range, int per) {
+template <int D, bool SLABS>
+__global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_kernel(Append8Params p, int kv_blocks, int per_kv,
+                                                                                   int per_q) {
+  constexpr int range = kB8;              // rows of a block
   __shared__ int s_blk[2 * kB8 + 2];      // cache blocks of rows r0 - 1 .. r0 + range + 63
   __shared__ int s_last[kB8];             // last row of the run at each offset
-  __shared__ uint32_t s_begin[5], s_top[8];
+  __shared__ uint32_t s_begin[5], s_top[2][D / 8];
+  constexpr int TPR = D / 16;             // threads of a row, eight pairs each
   chain_sync();
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x >= kv_blocks) {
+  const int tid = threadIdx.x, q = tid % TPR, i0 = q * 8;
+  // blocks of the two kinds take turns, so that the ones that wait and the ones that stream share the SMs
+  const int i_kv = (int)((long long)blockIdx.x * kv_blocks / gridDim.x);
+  if ((int)((long long)(blockIdx.x + 1) * kv_blocks / gridDim.x) == i_kv) {
     // ------------------------------ q heads ------------------------------
-    constexpr int TPR = D / 16, ROWS = 256 / TPR;
-    const int b = blockIdx.x - kv_blocks, parts = (p.Hq + per - 1) / per;
-    const int r = b / parts * ROWS + tid / TPR, h0 = b % parts * per, i0 = tid % TPR * 8;
+    const int b = blockIdx.x - i_kv, parts = (p.Hq + per_q - 1) / per_q;
+    const int r = b / parts * 64 + tid / TPR, h0 = b % parts * per_q;
     if (r >= p.T) return;
     float c[8], s[8];
     if (p.rope_pos) load_angles<D>(p, r, i0, c, s);
-#pragma unroll 4
-    for (int h = h0; h < min(h0 + per, p.Hq); ++h) {
+#pragma unroll 2
+    for (int h = h0; h < min(h0 + per_q, p.Hq); ++h) {
+      Pairs<D, SLABS> pairs;
+      pairs.load(p, r, h, i0);
       float x[8], y[8];
-      load_pairs<D>(p, r, h, i0, x, y);
+      pairs.get(x, y);
       if (p.rope_pos) turn_pairs(x, y, c, s);
       store_pairs<D>(p, r, h, i0, x, y);
     }
     return;
   }
-  // ------------------------------ k and v heads ------------------------------
-  const int kv_heads = 2 * p.Hkv, hd = blockIdx.x % kv_heads, r0 = blockIdx.x / kv_heads * range;
-  const int head = p.Hq + hd, rows = min(range, p.T - r0);
-  for (int i = tid; i < range + kB8 + 1; i += 256) {
-    const int t = r0 - 1 + i;
-    s_blk[i] = t >= 0 && t < p.T ? block_of(p, t) : -1;
+  // ------------------------------ k or v heads ------------------------------
+  const int parts = (p.Hkv + per_kv - 1) / per_kv, kv = i_kv % (2 * parts) / parts;
+  const int g0 = i_kv % parts * per_kv, g1 = min(g0 + per_kv, p.Hkv);                    // kv heads
+  const int r0 = i_kv / (2 * parts) * range, rows = min(range, p.T - r0);
+  const int head0 = p.Hq + kv * p.Hkv;
+  if (tid < range + kB8 + 1) {
+    const int t = r0 - 1 + tid;
+    s_blk[tid] = t >= 0 && t < p.T ? block_of(p, t) : -1;
   }
   __syncthreads();
   // bit i: row r0 + i lies in another block than the one before
@@ -323,85 +437,91 @@ __global__ void __launch_bounds__(256) append8_kernel(Append8Params p, int kv_bl
     while (!bits && ++w < 5) bits = s_begin[w];
     return bits ? w * 32 + __ffs(bits) - 1 : range + kB8;
   };
-  const RowLanes<D> lanes(p, head);
-  constexpr int LPH = D / 4;
-  for (int i = tid / LPH; i < rows; i += 256 / LPH) {
+  // single rows, and runs that name a place twice
+  for (int i = tid / (D / 4); i < rows; i += 16) {
     const int blk = s_blk[i + 1], t = r0 + i;
-    if (blk < 0) {
-      lanes.turn_only(t);
-      continue;
+    int end = t;
+    if (blk >= 0) {
+      if (s_blk[i] == blk) continue;
+      end = r0 + next(i + 1);
+      if (end - t > 1 && end - t <= kB8) continue;
+      if (end - t > kB8)
+        while (end < p.T && block_of(p, end) == blk) ++end;
     }
-    if (s_blk[i] == blk) continue;
-    int end = r0 + next(i + 1);
-    if (end - t >= kRun && end - t <= kB8) continue;
-    if (end - t > kB8)      // some place is named twice
-      while (end < p.T && block_of(p, end) == blk) ++end;
-    lanes.append(t, end, blk);
+    for (int g = g0; g < g1; ++g) {
+      const RowLanes<D> lanes(p, head0 + g);
+      if (blk < 0) {
+        lanes.turn_only(t);
+      } else if (end > t + 1) {
+        lanes.append(t, end, blk);
+      } else {
+        float x[4];
+        lanes.load(t, x);
+        lanes.append(t, blk, x, p.scales[lanes.place(blk)]);
+      }
+    }
   }
-  const int kv = hd >= p.Hkv ? 1 : 0;
   const bool turns = p.rope_pos && !kv;
   for (int i = next(0), e; i < rows; i = e) {
     e = next(i + 1);
     const int blk = s_blk[i + 1], t = r0 + i, n = e - i;
-    if (blk < 0 || n < kRun || n > kB8) continue;
-    // a quarter of a row per thread: 16 pairs (D = 128) or 8
-    constexpr int U = D / 64;
-    const int row = tid >> 2, q = tid & 3, r = t + row;
+    if (blk < 0 || n < 2 || n > kB8) continue;
+    const int row = tid / TPR, r = t + row;
     const bool mine = row < n;
-    const size_t at = ((size_t)blk * 2 + kv) * p.Hkv + (hd - kv * p.Hkv);
-    const float before = p.scales[at];
-    if (tid < kB8) s_last[tid] = -1;
-    float x[U][8], y[U][8], amax = 0.f;
+    const size_t at0 = ((size_t)blk * 2 + kv) * p.Hkv;
+    Pairs<D, SLABS> ahead;
+    float c[8], s[8], before = p.scales[at0 + g0];
     int off = 0;
     if (mine) {
       off = p.cache_pos[r] % kB8;
-#pragma unroll
-      for (int u = 0; u < U; ++u) load_pairs<D>(p, r, head, (u * 4 + q) * 8, x[u], y[u]);
-      if (turns) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float c[8], s[8];
-          load_angles<D>(p, r, (u * 4 + q) * 8, c, s);
-          turn_pairs(x[u], y[u], c, s);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fmaxf(finite_abs(x[u][k]), finite_abs(y[u][k])));
+      ahead.load(p, r, head0 + g0, i0);
+      if (turns) load_angles<D>(p, r, i0, c, s);
     }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));      // of numbers >= 0, bits order as they do
-    if ((tid & 31) == 0) s_top[tid >> 5] = top;
+    __syncthreads();      // the run before has been done
+    if (tid < kB8) s_last[tid] = -1;
     __syncthreads();
     if (mine && q == 0) atomicMax(&s_last[off], row);
-    __syncthreads();
-    uint32_t all = 0;
+    for (int g = g0; g < g1; ++g) {
+      float x[8], y[8], amax = 0.f;
+      if (mine) {
+        ahead.get(x, y);
+        if (turns) turn_pairs(x, y, c, s);
 #pragma unroll
-    for (int w = 0; w < 8; ++w) all = max(all, s_top[w]);
-    const bool anew = s_last[0] >= 0;
-    const float kept = anew ? 0.f : before, scale = fmaxf(kept, scale_of(__uint_as_float(all))), inv = 1.f / scale;
-    uint8_t* dst = p.codes + at * kB8 * D;
-    if (scale != kept) {
-      if (s_last[row] < 0) {      // thread's quarter of the row at this offset
-        const float ratio = kept / scale;
-        uint32_t* c = reinterpret_cast<uint32_t*>(dst + row * D) + q * (D / 16);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) c[k] = anew ? 0u : rescaled(c[k], ratio);
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fmaxf(finite_abs(x[k]), finite_abs(y[k])));
       }
-      if (tid == 0) p.scales[at] = scale;
-    }
-    if (mine) {
+      // of numbers >= 0, bits order as they do
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+      if ((tid & 31) == 0) s_top[g & 1][tid >> 5] = top;
+      const float now = before;
+      if (g + 1 < g1) {      // the next head's, while this one's largest value is found
+        before = p.scales[at0 + g + 1];
+        if (mine) ahead.load(p, r, head0 + g + 1, i0);
+      }
+      __syncthreads();
+      uint32_t all = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i0 = (u * 4 + q) * 8;
-        if (s_last[off] == row) {
-          *reinterpret_cast<uint2*>(dst + off * D + i0) = codes_of8(x[u], inv);
-          *reinterpret_cast<uint2*>(dst + off * D + D / 2 + i0) = codes_of8(y[u], inv);
+      for (int w = 0; w < D / 8; ++w) all = max(all, s_top[g & 1][w]);
+      const bool anew = s_last[0] >= 0;
+      const float kept = anew ? 0.f : now, scale = fmaxf(kept, scale_of(__uint_as_float(all))), inv = 1.f / scale;
+      uint8_t* dst = p.codes + (at0 + g) * kB8 * D;
+      if (scale != kept) {
+        if (s_last[row] < 0) {      // the row at this offset is not the call's
+          const float ratio = kept / scale;
+          uint4* to = reinterpret_cast<uint4*>(dst + row * D) + q;
+          const uint4 v = *to;
+          *to = anew ? make_uint4(0u, 0u, 0u, 0u)
+                     : make_uint4(rescaled(v.x, ratio), rescaled(v.y, ratio), rescaled(v.z, ratio), rescaled(v.w, ratio));
         }
-        if (turns || p.slabs) store_pairs<D>(p, r, head, i0, x[u], y[u]);
+        if (tid == 0) p.scales[at0 + g] = scale;
+      }
+      if (mine) {
+        if (s_last[off] == row) {
+          *reinterpret_cast<uint2*>(dst + off * D + i0) = codes_of8(x, inv);
+          *reinterpret_cast<uint2*>(dst + off * D + D / 2 + i0) = codes_of8(y, inv);
+        }
+        if (turns || SLABS) store_pairs<D>(p, r, head0 + g, i0, x, y);
       }
     }
-    __syncthreads();
   }
 }
 
@@ -439,16 +559,28 @@ extern "C" int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long
   p.block_table = block_table; p.sequences = sequences; p.max_blocks = max_blocks; p.codes = (uint8_t*)codes;
   p.scales = scales; p.num_blocks = num_blocks; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
   auto on = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  if (row_stride % 8 || !on(qkv) || !on(slabs) || slab_stride % 4 || !on(cos_tab) || !on(sin_tab)) {
-    const long long blocks = ((long long)T * (Hq + 2 * Hkv) * (D / 4) + 255) / 256;
-    if (blocks > 0x7fffffffll) return -4;
-    return launch_chained(D == 128 ? append8_lanes_kernel<128> : append8_lanes_kernel<64>, (unsigned)blocks, 256, 0, stream, p);
+  // At most as many rows as sequences: a decoding step, if it is anything, and then the second kernel would go from row to row
+  // (256 rows, 28 / 4 heads, D = 128: 7.4 us against 22.7; 1000: 24 against 28).  More rows come in runs (825 rows of three prompts:
+  // 21.5 against 10.7; 60 rows of one: 7.9 either way).
+  if (T <= 128 || T <= sequences || row_stride % 8 || !on(qkv) || !on(slabs) || slab_stride % 4 || !on(cos_tab) || !on(sin_tab)) {
+    const int rows = 1024 / D;
+    const long long kv = (long long)((T + rows - 1) / rows) * 2 * Hkv;
+    const long long q = rope_pos || slabs ? ((long long)T * Hq + rows - 1) / rows : 0;
+    if (kv + q > 0x7fffffffll) return -4;
+    return launch_chained(D == 128 ? append8_rows_kernel<128> : append8_rows_kernel<64>, (unsigned)(kv + q), 256, 0, stream, p, (int)kv);
   }
-  const int range = T <= 2048 ? 8 : kB8, per = T <= 2048 ? 1 : 4, rows = 256 / (D / 16);
-  const long long kv = (long long)((T + range - 1) / range) * 2 * Hkv;
-  const long long q = rope_pos || slabs ? (long long)((T + rows - 1) / rows) * ((Hq + per - 1) / per) : 0;
+  // several heads for what a block finds out about its rows, as long as every SM gets blocks
+  const int ranges = (T + kB8 - 1) / kB8;
+  auto blocks_of = [](long long n, int heads, int per) { return n * ((heads + per - 1) / per); };
+  int per_kv = 4, per_q = 8;
+  while (per_kv > 1 && blocks_of(2 * ranges, Hkv, per_kv) < 4 * num_sms()) per_kv /= 2;
+  while (per_q > 1 && blocks_of(ranges, Hq, per_q) < 4 * num_sms()) per_q /= 2;
+  const long long kv = blocks_of(2 * ranges, Hkv, per_kv);
+  const long long q = rope_pos || slabs ? blocks_of(ranges, Hq, per_q) : 0;
   if (kv + q > 0x7fffffffll) return -4;
-  return launch_chained(D == 128 ? append8_kernel<128> : append8_kernel<64>, (unsigned)(kv + q), 256, 0, stream, p, (int)kv, range, per);
+  auto kernel = D == 128 ? (slabs ? append8_kernel<128, true> : append8_kernel<128, false>)
+                         : (slabs ? append8_kernel<64, true> : append8_kernel<64, false>);
+  return launch_chained(kernel, (unsigned)(kv + q), 4 * D, 0, stream, p, (int)kv, per_kv, per_q);
 }
 
 extern "C" int sb_kv8_copy_blocks(void* codes, float* scales, const int* src, const int* dst, int n_pairs, int num_blocks,
