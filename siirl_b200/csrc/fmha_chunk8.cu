@@ -1,0 +1,530 @@
+// Attention of chunks of prompts against a paged cache of e4m3 codes (kv_cache8.cu): row i of a chunk behind a prefix of P
+// tokens sees tokens 0 .. P + i.
+//
+// unpack8_kernel writes the visible tokens' keys and values once as bf16 rows [2, Hkv, rows, D] (code times scale, exact where
+// the scale is a power of two), every sequence from a multiple of 128 rows on, zeros behind its last token.  It moves 5 bytes per
+// cached number, against 4 * Hq / Hkv * chunk flops per number that the products take; converting in every block of the product
+// kernel instead would cost it shared memory bandwidth, of which its operands take three quarters.
+//
+// fmha_chunk_kernel: one block takes one or two tiles of 128 rows of one kv head, a row being (position, query head of the kv
+// head): heads that share keys share a tile, so that short chunks fill it, too, and keys are fetched once for all of them.
+//   S = Q K_j^T      tcgen05.mma 128 x KV x D -> TMEM
+//   soft-max         one warpgroup per tile, thread = row; weights (bf16) replace the scores in TMEM, in two halves, each
+//                    handed to the products at once
+//   O += P V_j       tcgen05.mma 128 x D x KV, P from TMEM, V through an MN-major descriptor
+// The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.  Of the
+// exponentials, which would take as long as the products (16 a cycle and SM), every fourth pair is computed on the
+// fused-multiply-add units: 2^x = 2^n 2^f with n the nearest integer and a cubic in f, |f| <= 1/2, fitted for the smallest largest
+// relative error (7.5e-5, an eighth of a bf16 step) by iteratively reweighted least squares.
+// Where there are fewer blocks than fit the SMs, the key tiles are split over several, whose results chunk_merge_kernel joins.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "launchers.h"
+
+namespace sb {
+
+constexpr int kChunkSeqs = 128;      // sequences of one launch
+
+struct ChunkSeqs {
+  int n, rows, tiles;                // rows: of the unpacked keys; tiles: of `span` positions, over all sequences
+  int slot[kChunkSeqs], total[kChunkSeqs], prefix[kChunkSeqs];
+  int q_row[kChunkSeqs];             // first row of the chunk
+  int kv_row[kChunkSeqs], tile[kChunkSeqs];      // first unpacked row, first tile
+};
+// last i with first[i] <= x
+__device__ __forceinline__ int find_seq(const int* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint2 bf16_of(uint32_t codes, float scale) {
+  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
+  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return make_uint2(pack_bf16x2(a.x * scale, a.y * scale), pack_bf16x2(b.x * scale, b.y * scale));
+}
+
+// block x: 64 rows; block y: k and v heads
+template <int D>
+__global__ void __launch_bounds__(256) unpack8_kernel(const __grid_constant__ ChunkSeqs q, const uint8_t* codes, const float* scales,
+                                                      int num_blocks, const int* block_table, int max_blocks, int Hkv,
+                                                      __nv_bfloat16* out) {
+  chain_sync();
+  const int row = blockIdx.x * 64, i = find_seq(q.kv_row, q.n, row), t0 = row - q.kv_row[i], left = q.total[i] - t0;
+  const int hd = blockIdx.y, kv = hd >= Hkv;
+  int blk = left > 0 ? block_table[(size_t)q.slot[i] * max_blocks + t0 / 64] : -1;
+  if (blk >= num_blocks) blk = -1;
+  const size_t at = blk < 0 ? 0 : ((size_t)blk * 2 + kv) * Hkv + (hd - kv * Hkv);
+  const float scale = blk < 0 ? 0.f : scales[at];
+  const uint4* src = reinterpret_cast<const uint4*>(codes + at * 64 * D);
+  uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)hd * q.rows + row) * D);
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    const int u = k * 256 + threadIdx.x;      // 16 numbers
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (blk >= 0 && u * 16 / D < left) {
+      const uint4 c = src[u];
+      const uint2 p0 = bf16_of(c.x, scale), p1 = bf16_of(c.y, scale), p2 = bf16_of(c.z, scale), p3 = bf16_of(c.w, scale);
+      a = make_uint4(p0.x, p0.y, p1.x, p1.y);
+      b = make_uint4(p2.x, p2.y, p3.x, p3.y);
+    }
+    dst[2 * u] = a;
+    dst[2 * u + 1] = b;
+  }
+}
+
+struct ChunkParams {
+  __nv_bfloat16* out;      // [chunk rows, Hq * D]
+  float* ws_o;             // [tile, kv head, split, query tile, 128, D], where splits > 1
+  float* ws_lse;           // [.., 128]
+  int Hq, Hkv, rep, span, splits;      // span: positions of 128 rows
+  float scale_log2;
+  int* status;
+};
+
+template <int D, int KV, int QT>
+struct ChunkSmem {
+  static constexpr int kQBytes = 128 * D * 2, kKvBytes = KV * D * 2;
+  static constexpr int kStages = QT == 1 ? 4 : D == 128 ? 5 : 6;
+  static constexpr int kRingOff = QT * kQBytes;
+  static constexpr int kBarOff = kRingOff + kStages * kKvBytes;  // q[2], s_full[2], p_full[2][2], o_full[2], full[], empty[]
+  static constexpr int kTotal = kBarOff + (10 + 2 * kStages) * 8 + 16;
+};
+
+// two of 2^x, x >= -126: see above
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 big = make_float2(12582912.f, 12582912.f), small = make_float2(-12582912.f, -12582912.f);      // 1.5 * 2^23
+  const float2 t = add_f32x2(x, big), n = add_f32x2(t, small), minus = make_float2(-1.f, -1.f);
+  const float2 f = fma_f32x2(n, minus, x);
+  float2 p = fma_f32x2(f, make_float2(0.0551716817f, 0.0551716817f), make_float2(0.24261115979f, 0.24261115979f));
+  p = fma_f32x2(p, f, make_float2(0.69326098678f, 0.69326098678f));
+  p = fma_f32x2(p, f, make_float2(0.99992807130f, 0.99992807130f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// KV: keys of a tile; QT: query tiles; CTAS: blocks of an SM.
+// Four warps for the soft-max of each query tile (thread = row), then one for TMA and the MMA issuer.
+template <int D, int KV, int QT, int CTAS>
+__global__ void __launch_bounds__(QT * 128 + 64, CTAS)
+fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
+                  const __grid_constant__ ChunkSeqs seqs, ChunkParams p) {
+  using L = ChunkSmem<D, KV, QT>;
+  constexpr int kDChunks = D / 64, kStages = L::kStages, kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1;
+  constexpr uint32_t kTmemCols = QT * (KV + D) <= 128 ? 128 : QT * (KV + D) <= 256 ? 256 : 512;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw;
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, (int)kStatusBadArgument);
+    return;
+  }
+  uint8_t* sQ = smem;
+  uint8_t* ring = smem + L::kRingOff;
+  uint64_t* bar_q = reinterpret_cast<uint64_t*>(smem + L::kBarOff);  // [2]
+  uint64_t* s_full = bar_q + 2;                                      // [2] scores are in TMEM
+  uint64_t* p_full = bar_q + 4;                                      // [2][2] halves of the weights have replaced the scores
+  uint64_t* o_full = bar_q + 8;                                      // [2] the output is complete
+  uint64_t* full = bar_q + 10;                                       // [kStages] ring of K and V tiles
+  uint64_t* empty = full + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + kStages);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_kv);
+    for (int i = 0; i < 10; ++i) mbar_init(&bar_q[i], i >= 4 && i < 8 ? 4 : 1);
+    for (int i = 0; i < 2 * kStages; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_sync();
+  // block -> (tile, kv head, share of the keys); a sequence's last tiles, which see most, first
+  const int split = (int)(blockIdx.x % p.splits), g = (int)(blockIdx.x / p.splits % p.Hkv);
+  const int tile = (int)(blockIdx.x / p.splits / p.Hkv), seq = find_seq(seqs.tile, seqs.n, tile);
+  const int prefix = seqs.prefix[seq], total = seqs.total[seq];
+  const int tile_end = seq + 1 < seqs.n ? seqs.tile[seq + 1] : seqs.tiles;
+  const int c0 = (tile_end - 1 - tile) * QT * p.span;      // first position, in the chunk
+  // key tiles that query tile w walks over: first .. key_tiles(w) - 1
+  auto key_tiles = [&](int w) {
+    const int from = prefix + c0 + w * p.span;
+    return from >= total ? 0 : (min(from + p.span, total) + KV - 1) / KV;
+  };
+  const int all = max(key_tiles(0), QT == 2 ? key_tiles(1) : 0);
+  const int j0 = (int)((long long)all * split / p.splits), j1 = (int)((long long)all * (split + 1) / p.splits);
+  const int n0 = max(0, min(key_tiles(0), j1) - j0), n1 = QT == 2 ? max(0, min(key_tiles(1), j1) - j0) : 0;
+  const int n_max = max(n0, n1);
+
+  if (warp == kTmaWarp) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0 && n_max > 0) {
+      const int q_row = seqs.q_row[seq] + c0;
+      const int k_row = g * seqs.rows + seqs.kv_row[seq] + j0 * KV, v_row = k_row + p.Hkv * seqs.rows;
+      auto load_q = [&](int w) {
+        mbar_arrive_expect_tx(&bar_q[w], (uint32_t)(kDChunks * p.rep * p.span * 128));
+#pragma unroll
+        for (int c = 0; c < kDChunks; ++c)
+          tma_load_3d(sQ + w * L::kQBytes + c * 16384, &map_q, &bar_q[w], c * 64, g * p.rep, q_row + w * p.span);
+      };
+      load_q(0);
+      int i = 0;
+      for (; i < 2 * n_max; ++i) {  // K0 V0 K1 V1 ...
+        const int st = i % kStages;
+        if (!mbar_wait(&empty[st], ((i / kStages) & 1) ^ 1, p.status, kStatusTimeoutProducer)) break;
+        uint8_t* dst = ring + st * L::kKvBytes;
+        const int row = ((i & 1) ? v_row : k_row) + (i >> 1) * KV;
+        mbar_arrive_expect_tx(&full[st], L::kKvBytes);
+#pragma unroll
+        for (int c = 0; c < kDChunks; ++c) tma_load_2d(dst + c * (KV * 128), &map_kv, &full[st], c * 64, row);
+        if (i == 0 && n1 > 0) load_q(1);
+      }
+      if (i < 2 * n_max) {  // gave up: no copy may land in shared memory that has been handed on
+        mbar_wait(&bar_q[0], 0, nullptr, 0);
+        if (n1 > 0 && i > 0) mbar_wait(&bar_q[1], 0, nullptr, 0);
+        for (int k = max(0, i - kStages); k < i; ++k) mbar_wait(&full[k % kStages], (k / kStages) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------ MMA issuer (converged; lane 0 issues) ------------------------------
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, KV, 0, 0);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 0, 1);
+    const uint32_t leader = lane == 0;
+    const uint32_t aq = smem_u32(sQ), ar = smem_u32(ring);
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma));
+      tc_fence_after();
+      return ok;
+    };
+    auto wait_ring = [&](int i) { return wait(&full[i % kStages], (i / kStages) & 1); };
+    auto scores = [&](int w, int j) {
+      const uint32_t bk = ar + ((2 * j) % kStages) * L::kKvBytes;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        umma_bf16_ss_if(leader, tmem_base + w * KV,
+                        umma_smem_desc(aq + w * L::kQBytes + (kk / 4) * 16384 + (kk % 4) * 32, 16, 1024),
+                        umma_smem_desc(bk + (kk / 4) * (KV * 128) + (kk % 4) * 32, 16, 1024), idesc_s, kk ? 1u : 0u);
+      umma_commit_if(leader, &s_full[w]);
+    };
+    bool ok = n_max > 0 && wait(&bar_q[0], 0) && wait_ring(0);
+    if (ok) {
+      if (n0 > 0) scores(0, 0);
+      if (n1 > 0) {
+        ok = wait(&bar_q[1], 0);
+        if (ok) scores(1, 0);
+      }
+      umma_commit_if(leader, &empty[0]);
+    }
+    for (int j = 0; j < n_max && ok; ++j) {
+      ok = wait_ring(2 * j + 1);
+#pragma unroll
+      for (int w = 0; w < QT; ++w) {
+        const int n = w ? n1 : n0;
+        if (ok && j < n) {
+          const uint32_t bv = ar + ((2 * j + 1) % kStages) * L::kKvBytes;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            ok = ok && wait(&p_full[2 * w + part], j & 1);
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < KV / 32; ++k) {
+              const int kk = part * (KV / 32) + k;
+              umma_bf16_ts_if(leader, tmem_base + QT * KV + w * D, tmem_base + w * KV + kk * 8,
+                              umma_smem_desc(bv + kk * 2048, KV * 128, 1024), idesc_o, (j | kk) ? 1u : 0u);
+            }
+          }
+          if (ok && j + 1 == n) umma_commit_if(leader, &o_full[w]);
+        }
+        if (w == QT - 1) umma_commit_if(leader, &empty[(2 * j + 1) % kStages]);
+        if (ok && j + 1 < n) {
+          ok = wait_ring(2 * j + 2);
+          if (ok) scores(w, j + 1);
+        }
+      }
+      if (j + 1 < n_max) umma_commit_if(leader, &empty[(2 * j + 2) % kStages]);
+    }
+  } else {
+    // ------------------------------ softmax and output: thread = row ------------------------------
+    const int w = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tmem_s = tmem_base + lane_off + w * KV;
+    const uint32_t tmem_o = tmem_base + lane_off + QT * KV + w * D;
+    const int first = prefix + c0 + w * p.span, at = row / p.rep, head = row - at * p.rep;
+    const int qpos = first + at;      // position within the sequence
+    const int n = w ? n1 : n0;
+    const float sc = p.scale_log2;
+    float m_ref = -INFINITY;          // reference of the weights, scaled
+    float2 l_run[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[w], j & 1, p.status, kStatusTimeoutEpilogue));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[KV / 32][32];
+#pragma unroll
+      for (int c = 0; c < KV / 32; ++c) tmem_ld_32x32(tmem_s + c * 32, s[c]);
+      tmem_ld_wait();
+      const int kv0 = (j0 + j) * KV;
+      if (kv0 + KV - 1 > first) {
+        const int visible = min(qpos + 1, total) - kv0;
+#pragma unroll
+        for (int i = 0; i < KV; ++i)
+          if (i >= visible) s[i / 32][i % 32] = 0xff800000u;  // -inf
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < KV; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i / 32][i % 32]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+      if (__any_sync(0xffffffffu, top > m_ref + 8.f)) {
+        // The barrier of the scores also said that P V of the previous tile is done
+        const float m_new = fmaxf(m_ref, top), alpha = fast_exp2(m_ref - (m_new == -INFINITY ? 0.f : m_new));
+        m_ref = m_new;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          l_run[i].x *= alpha;
+          l_run[i].y *= alpha;
+        }
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 8; ++c) {      // few columns at a time: the scores hold most registers
+            uint32_t r[8];
+            tmem_ld_32x8(tmem_o + c * 8, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st_32x8(tmem_o + c * 8, r);
+          }
+        }
+      }
+      const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+      const float2 sc2 = make_float2(sc, sc), neg = make_float2(-ref, -ref);
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+#pragma unroll
+        for (int i0 = part * (KV / 2); i0 < (part + 1) * (KV / 2); i0 += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = i0; i < i0 + 32; i += 2) {
+            float2 x = make_float2(__uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
+            x = fma_f32x2(x, sc2, neg);
+            if (i % 8 == 6) {
+              x = poly_exp2(x);
+            } else {
+              x.x = fast_exp2(x.x);
+              x.y = fast_exp2(x.y);
+            }
+            l_run[i / 2 & 1] = add_f32x2(l_run[i / 2 & 1], x);
+            pk[(i - i0) / 2] = pack_bf16x2(x.x, x.y);
+          }
+          tmem_st_32x16(tmem_s + i0 / 2, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * w + part]);
+      }
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[w], 0, p.status, kStatusTimeoutEpilogue));
+    // ---- O / l -> bf16, or the share's normalised result (TMEM loads are warp-collective; only the stores are predicated) ----
+    if (ok) {
+      tc_fence_after();
+      const bool row_valid = at < p.span && qpos < total;
+      const float l = m_ref == -INFINITY ? 0.f : (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
+      const float inv_l = l != 0.f ? 1.f / l : 0.f;
+      const size_t part = ((((size_t)tile * p.Hkv + g) * p.splits + split) * QT + w) * 128 + row;
+      const size_t out_row = (size_t)seqs.q_row[seq] + (row_valid ? qpos - prefix : 0);
+      __nv_bfloat16* orow = p.out + out_row * (size_t)(p.Hq * D) + (size_t)(g * p.rep + head) * D;
+      if (n > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32(tmem_o + c * 32, r);
+          tmem_ld_wait();
+          if (!row_valid) continue;
+          if (p.splits > 1) {
+            float4* wrow = reinterpret_cast<float4*>(p.ws_o + part * D + c * 32);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              wrow[q] = make_float4(__uint_as_float(r[4 * q]) * inv_l, __uint_as_float(r[4 * q + 1]) * inv_l,
+                                    __uint_as_float(r[4 * q + 2]) * inv_l, __uint_as_float(r[4 * q + 3]) * inv_l);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 o;
+              o.x = pack_bf16x2(__uint_as_float(r[q * 8 + 0]) * inv_l, __uint_as_float(r[q * 8 + 1]) * inv_l);
+              o.y = pack_bf16x2(__uint_as_float(r[q * 8 + 2]) * inv_l, __uint_as_float(r[q * 8 + 3]) * inv_l);
+              o.z = pack_bf16x2(__uint_as_float(r[q * 8 + 4]) * inv_l, __uint_as_float(r[q * 8 + 5]) * inv_l);
+              o.w = pack_bf16x2(__uint_as_float(r[q * 8 + 6]) * inv_l, __uint_as_float(r[q * 8 + 7]) * inv_l);
+              *reinterpret_cast<uint4*>(orow + c * 32 + q * 8) = o;
+            }
+          }
+        }
+      }
+      if (p.splits > 1 && row_valid) p.ws_lse[part] = l != 0.f ? m_ref + log2f(l) : -INFINITY;      // NaN stays NaN
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// mean of the shares' results, weighted by 2^(log-sum-exp); a warp per row
+template <int D>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkSeqs seqs, ChunkParams p, int qt) {
+  chain_sync();
+  const int unit = blockIdx.x / 16, row = blockIdx.x % 16 * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int w = unit % qt, g = unit / qt % p.Hkv, tile = unit / qt / p.Hkv, seq = find_seq(seqs.tile, seqs.n, tile);
+  const int tile_end = seq + 1 < seqs.n ? seqs.tile[seq + 1] : seqs.tiles;
+  const int at = row / p.rep, pos = ((tile_end - 1 - tile) * qt + w) * p.span + at;
+  if (at >= p.span || pos >= seqs.total[seq] - seqs.prefix[seq]) return;
+  constexpr int N = D / 32;
+  float top = -INFINITY, sum = 0.f, acc[N] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const size_t part = ((((size_t)tile * p.Hkv + g) * p.splits + s) * qt + w) * 128 + row;
+    const float lse = p.ws_lse[part];
+    if (lse == -INFINITY) continue;      // its share may not have been written
+    const float now = fmaxf(top, lse), f = exp2f(top - now), e = exp2f(lse - now);
+    top = now;
+    sum = sum * f + e;
+    const float* o = p.ws_o + part * D + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = acc[i] * f + e * o[i];
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  __nv_bfloat16* out = p.out + (size_t)(seqs.q_row[seq] + pos) * (p.Hq * D) + (size_t)(g * p.rep + row - at * p.rep) * D + lane * N;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// What a call does, from the host's lists alone
+struct ChunkPlan {
+  ChunkSeqs s;
+  int qt, kv, ctas, span, splits;
+};
+static int make_chunk_plan(ChunkPlan& c, const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D) {
+  const int rep = Hq / Hkv;
+  c.span = 128 / rep;
+  int order[kChunkSeqs], first[kChunkSeqs];
+  long long rows = 0, positions = 0;
+  int live = 0;
+  for (int i = 0; i < n; ++i) {
+    first[i] = (int)positions;
+    positions += chunk[i];
+    if (chunk[i] > 0) order[live++] = i;
+  }
+  // those that see most first
+  std::sort(order, order + live, [&](int a, int b) { return prefix[a] + chunk[a] > prefix[b] + chunk[b]; });
+  auto tiles_of = [&](int span) {
+    long long t = 0;
+    for (int k = 0; k < live; ++k) t += (chunk[order[k]] + span - 1) / span;
+    return t;
+  };
+  const long long ones = tiles_of(c.span), twos = tiles_of(2 * c.span);
+  // two tiles share their keys; one alone leaves room for a second block on the SM
+  c.qt = ones * Hkv <= 2 * num_sms() || twos * 2 * 100 > ones * 110 ? 1 : 2;
+  c.kv = c.qt == 2 && D == 128 ? 128 : 64;
+  c.ctas = c.qt == 2 ? (D == 128 ? 1 : 2) : (D == 128 ? 2 : 3);
+  c.s.n = live;
+  int tiles = 0, longest = 0;
+  for (int k = 0; k < live; ++k) {
+    const int i = order[k], total = prefix[i] + chunk[i];
+    c.s.slot[k] = slot[i]; c.s.total[k] = total; c.s.prefix[k] = prefix[i]; c.s.q_row[k] = first[i];
+    c.s.kv_row[k] = (int)rows; c.s.tile[k] = tiles;
+    rows += (total + 127) / 128 * 128;
+    tiles += (chunk[i] + c.qt * c.span - 1) / (c.qt * c.span);
+    longest = std::max(longest, (total + c.kv - 1) / c.kv);
+    if (rows * 2 * Hkv > 0x7fffffffll) return -4;
+  }
+  c.s.rows = (int)rows;
+  c.s.tiles = tiles;
+  const long long blocks = (long long)tiles * Hkv, room = (long long)num_sms() * c.ctas;
+  c.splits = blocks ? (int)std::max(1ll, std::min({room / blocks, (long long)longest / 4, 32ll})) : 1;
+  if (blocks * c.splits > 0x7fffffffll / 32) return -4;
+  return 0;
+}
+
+template <int D, int KV, int QT, int CTAS>
+static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mkv, const ChunkPlan& c, const ChunkParams& p, cudaStream_t stream) {
+  using L = ChunkSmem<D, KV, QT>;
+  auto kernel = fmha_chunk_kernel<D, KV, QT, CTAS>;
+  static int configured = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured != dev) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e != cudaSuccess) return (int)e;
+    configured = dev;
+  }
+  const unsigned blocks = (unsigned)(c.s.tiles * p.Hkv * c.splits);
+  const int rc = launch_chained(kernel, blocks, QT * 128 + 64, L::kTotal, stream, mq, mkv, c.s, p);
+  if (rc || c.splits == 1) return rc;
+  return launch_chained(chunk_merge_kernel<D>, (unsigned)(c.s.tiles * p.Hkv * QT * 16), 256, 0, stream, c.s, p, QT);
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int sb_kv8_chunk_seqs() { return kChunkSeqs; }
+
+// Sizes of a call's workspaces: sizes[0] bf16 numbers of unpacked keys and values, sizes[1] floats (0: the result is written at
+// once).  The lists are the host's, of at most kChunkSeqs sequences.
+extern "C" int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D, long long* sizes) {
+  if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32) return -3;
+  ChunkPlan c;
+  const int rc = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
+  sizes[0] = 2ll * Hkv * c.s.rows * D;
+  sizes[1] = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * (D + 1) : 0;
+  return rc;
+}
+
+// Rows of n chunks, one behind the other in `qkv` (q heads first, row_stride apart), whose keys and values are in the cache.
+extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, const void* codes, const float* scales, int num_blocks,
+                             const int* block_table, int max_blocks, const int* chunk, const int* prefix, const int* slot, int n,
+                             void* kv, float* ws, void* out, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream) {
+  if (D != 64 && D != 128) return -2;
+  if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32 || row_stride % 8 || reinterpret_cast<uintptr_t>(qkv) % 16 || !(scale > 0.f)) return -3;
+  static thread_local bool tl_context_bound = false;
+  if (!tl_context_bound) {
+    cudaFree(0);
+    tl_context_bound = true;
+  }
+  ChunkPlan c;
+  int r = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
+  if (r || c.s.tiles == 0) return r;
+  long long rows = 0;
+  for (int i = 0; i < n; ++i) rows += chunk[i];
+  CUtensorMap mq, mkv;
+  r = make_tensor_map_bf16_3d(&mq, qkv, D, Hq, rows, D, row_stride, 64, Hq / Hkv, c.span);
+  if (r) return r;
+  r = make_tensor_map_bf16_2d(&mkv, kv, D, 2ll * Hkv * c.s.rows, D, 64, c.kv);
+  if (r) return r;
+  r = launch_chained(D == 128 ? unpack8_kernel<128> : unpack8_kernel<64>, dim3(c.s.rows / 64, 2 * Hkv), 256, 0, stream, c.s,
+                     (const uint8_t*)codes, scales, num_blocks, block_table, max_blocks, Hkv, (__nv_bfloat16*)kv);
+  if (r) return r;
+  ChunkParams p;
+  p.out = (__nv_bfloat16*)out; p.ws_o = ws;
+  p.ws_lse = ws + (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * D;
+  p.Hq = Hq; p.Hkv = Hkv; p.rep = Hq / Hkv; p.span = c.span; p.splits = c.splits;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  if (c.qt == 1) return D == 128 ? launch_chunk<128, 64, 1, 2>(mq, mkv, c, p, stream) : launch_chunk<64, 64, 1, 3>(mq, mkv, c, p, stream);
+  return D == 128 ? launch_chunk<128, 128, 2, 1>(mq, mkv, c, p, stream) : launch_chunk<64, 64, 2, 2>(mq, mkv, c, p, stream);
+}

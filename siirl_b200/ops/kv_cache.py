@@ -186,6 +186,9 @@ def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, sl
     chunk rows, and the chunk rows of the result are returned ``[sum(chunk_lens), Hq*D]``."""
     from .attention import SeqInfo, attention_packed
     if isinstance(cache_layer, Cache8):
+        if qkv.is_cuda:
+            return kv_cache8.chunk_attention(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads,
+                                             head_dim)
         kv_cache8.check_chunks(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads, head_dim)
     dev = qkv.device
     qw, kw = n_heads * head_dim, n_kv_heads * head_dim

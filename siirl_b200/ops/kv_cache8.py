@@ -271,9 +271,47 @@ def check_chunks(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Cache
     rows, width = sum(chunk_lens), (n_heads + 2 * n_kv_heads) * head_dim
     if qkv.shape != (rows, width):
         _refuse(f"{rows} rows of {width} numbers, got {tuple(qkv.shape)}")
+    if block_table.dim() != 2:
+        _refuse("a table of blocks for each sequence")
     slots_held, tokens_held = block_table.shape[0], block_table.shape[1] * BLOCK
     for c, p, s in zip(chunk_lens, prefix_lens, slots):
         if c < 0 or p < 0 or not 0 <= s < slots_held or c + p > tokens_held:
             _refuse(f"slot {s} of {slots_held} with {p} + {c} tokens of {tokens_held}")
     if qkv.is_cuda and qkv.dtype is not torch.bfloat16:
         _refuse("rows are bf16")
+
+
+def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Cache8, block_table: torch.Tensor, n_heads: int,
+                    n_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """:func:`siirl_b200.ops.kv_cache.prefill_attention_with_prefix` on an 8-bit cache, on the GPU.  The visible keys and values
+    are unpacked to bf16 once per call: ``4 * Hkv * D`` bytes for every token up to the next multiple of 128, beside the
+    output."""
+    chunk_lens, prefix_lens, slots = ([int(x) for x in v] for v in (chunk_lens, prefix_lens, slots))
+    check_chunks(qkv, chunk_lens, prefix_lens, slots, cache, block_table, n_heads, n_kv_heads, head_dim)
+    rows = qkv.shape[0]
+    out = torch.empty(rows, n_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
+    if rows == 0:
+        return out
+    stride, one = qkv.stride()
+    if one != 1 or stride % 8 or qkv.data_ptr() % 16:
+        qkv = qkv.contiguous()
+        stride = qkv.shape[1]
+    L = _lib.get_lib()
+    with _device(qkv.get_device()):
+        most, at = L.sb_kv8_chunk_seqs(), 0
+        for i in range(0, len(slots), most):
+            ints = ctypes.c_int * len(slots[i:i + most])
+            lists = [ints(*v[i:i + most]) for v in (chunk_lens, prefix_lens, slots)]
+            n = len(lists[0])
+            sizes = (ctypes.c_longlong * 2)()
+            _lib.check(L.sb_kv8_chunk_sizes(*lists, n, n_heads, n_kv_heads, head_dim, sizes), "sb_kv8_chunk_sizes")
+            # buffers of the call's own, as for single tokens
+            ws = torch.empty(2 * sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=qkv.device)
+            _lib.check(L.sb_kv8_chunks(
+                qkv.data_ptr() + 2 * at * stride, stride, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.codes.shape[0],
+                block_table.data_ptr(), block_table.shape[1], *lists, n, ws.data_ptr(), ws.data_ptr() + 2 * sizes[0],
+                out.data_ptr() + 2 * at * out.shape[1], n_heads, n_kv_heads, head_dim, 1.0 / math.sqrt(head_dim),
+                _lib.status_word(qkv.device).data_ptr(), _lib.stream()), "sb_kv8_chunks")
+            _lib.add_launches(int(sizes[1] > 0))        # shares of the keys are joined
+            at += sum(lists[0])
+    return out

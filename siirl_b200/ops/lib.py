@@ -24,14 +24,16 @@ _status_words: dict[int, torch.Tensor] = {}
 _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_rows": 0, "sb_ppo_token_loss": 2,
                      "sb_fmha_bwd": 3, "sb_kk_partition": 0, "sb_rmsnorm_bwd_blocks": 0, "sb_colsum_blocks": 0,
                      "sb_colsum_bf16": 2, "sb_gemm_set_pair_kernel": 0, "sb_fmha_decode_chunk_tiles": 0,
-                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_recurrence_prefill": 2, "sb_attn_window_decode": 2, "sb_latent_decode": 2,
+                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_kv8_chunk_seqs": 0, "sb_kv8_chunk_sizes": 0,
+                     "sb_kv8_chunks": 2, "sb_recurrence_prefill": 2, "sb_attn_window_decode": 2, "sb_latent_decode": 2,
                      "sb_delta_prefill": 3}
 
 
 # Arguments of entry points that single steps call most, one letter each (p: address, i: int, l: 64 bits, f: float): they are
 # then passed as plain numbers, which saves an object for each.
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
-_ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp"}
+_ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
+              "sb_kv8_chunk_sizes": "pppiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
 
 
 class _CountingLib:
