@@ -12,10 +12,11 @@
 //   soft-max         one warpgroup per tile, thread = row; weights (bf16) replace the scores in TMEM, in two halves, each
 //                    handed to the products at once
 //   O += P V_j       tcgen05.mma 128 x D x KV, P from TMEM, V through an MN-major descriptor
-// The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.  Of the
-// exponentials, which would take as long as the products (16 a cycle and SM), every fourth pair is computed on the
-// fused-multiply-add units: 2^x = 2^n 2^f with n the nearest integer and a cubic in f, |f| <= 1/2, fitted for the smallest largest
-// relative error (7.5e-5, an eighth of a bf16 step) by iteratively reweighted least squares.
+// The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.  At D = 64
+// the exponentials (16 a cycle and SM) take twice as long as the products, and every fourth pair is computed on the
+// fused-multiply-add units (4 sequences of up to 2000 rows, 14 / 2 heads: 262 us, 283 without; at D = 128 it costs what it
+// saves): 2^x = 2^n 2^f with n the nearest integer and a cubic in f, |f| <= 1/2, fitted for the smallest largest relative error
+// (7.5e-5, a fiftieth of a bf16 step) by iteratively reweighted least squares.
 // Where there are fewer blocks than fit the SMs, the key tiles are split over several, whose results chunk_merge_kernel joins.
 #include <cuda_fp8.h>
 
@@ -113,6 +114,28 @@ __device__ __forceinline__ float2 poly_exp2(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
+// One thread's MMAs, of operands whose descriptors have the high word of 128-byte swizzle and 1024 bytes between groups of eight
+// rows.  A in shared memory, and in TMEM
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_bf16_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHigh), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts_lo(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(kDescHigh), "r"(accumulate)
+      : "memory");
+}
+
 // KV: keys of a tile; QT: query tiles; CTAS: blocks of an SM.
 // Four warps for the soft-max of each query tile (thread = row), then one for TMA and the MMA issuer.
 template <int D, int KV, int QT, int CTAS>
@@ -201,63 +224,72 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
   } else if (warp == kMmaWarp) {
-    // ------------------------------ MMA issuer (converged; lane 0 issues) ------------------------------
-    constexpr uint32_t idesc_s = umma_idesc_bf16(128, KV, 0, 0);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 0, 1);
-    const uint32_t leader = lane == 0;
-    const uint32_t aq = smem_u32(sQ), ar = smem_u32(ring);
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma));
+    // ------------------------------ MMA issuer: one thread ------------------------------
+    // The soft-max warps leave it few issue slots: descriptors differ in their low words only, which are kept and stepped
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, KV, 0, 0);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 0, 1);
+      constexpr uint32_t kStep = L::kKvBytes >> 4;
+      const uint32_t q_lo = (uint32_t)umma_smem_desc(smem_u32(sQ), 16, 1024), k_lo = (uint32_t)umma_smem_desc(smem_u32(ring), 16, 1024);
+      const uint32_t v_lo = (uint32_t)umma_smem_desc(smem_u32(ring), KV * 128, 1024);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, p.status, kStatusTimeoutMma); };
+      auto scores = [&](int w, int stage) {
+        const uint32_t a = q_lo + w * (L::kQBytes >> 4), b = k_lo + stage * kStep;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16_ss_lo(tmem_base + w * KV, a + (kk / 4) * 1024 + (kk % 4) * 2, b + (kk / 4) * (KV * 8) + (kk % 4) * 2, idesc_s, kk > 0);
+        umma_commit(&s_full[w]);
+      };
+      int ks = 0, vs = 1;                  // ring places of K_j and V_j
+      uint32_t k_phase = 0, v_phase = 0;
+      auto step = [&](int& at, uint32_t& phase) {
+        at += 2;
+        if (at >= kStages) {
+          at -= kStages;
+          phase ^= 1;
+        }
+      };
+      bool ok = n_max > 0 && wait(&bar_q[0], 0) && wait(&full[0], 0);
       tc_fence_after();
-      return ok;
-    };
-    auto wait_ring = [&](int i) { return wait(&full[i % kStages], (i / kStages) & 1); };
-    auto scores = [&](int w, int j) {
-      const uint32_t bk = ar + ((2 * j) % kStages) * L::kKvBytes;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        umma_bf16_ss_if(leader, tmem_base + w * KV,
-                        umma_smem_desc(aq + w * L::kQBytes + (kk / 4) * 16384 + (kk % 4) * 32, 16, 1024),
-                        umma_smem_desc(bk + (kk / 4) * (KV * 128) + (kk % 4) * 32, 16, 1024), idesc_s, kk ? 1u : 0u);
-      umma_commit_if(leader, &s_full[w]);
-    };
-    bool ok = n_max > 0 && wait(&bar_q[0], 0) && wait_ring(0);
-    if (ok) {
-      if (n0 > 0) scores(0, 0);
-      if (n1 > 0) {
-        ok = wait(&bar_q[1], 0);
-        if (ok) scores(1, 0);
+      if (ok) {
+        if (n0 > 0) scores(0, 0);
+        if (n1 > 0) {
+          ok = wait(&bar_q[1], 0);
+          if (ok) scores(1, 0);
+        }
+        umma_commit(&empty[0]);
       }
-      umma_commit_if(leader, &empty[0]);
-    }
-    for (int j = 0; j < n_max && ok; ++j) {
-      ok = wait_ring(2 * j + 1);
+      for (int j = 0; j < n_max && ok; ++j) {
+        step(ks, k_phase);
+        ok = wait(&full[vs], v_phase) && (j + 1 >= n_max || wait(&full[ks], k_phase));
 #pragma unroll
-      for (int w = 0; w < QT; ++w) {
-        const int n = w ? n1 : n0;
-        if (ok && j < n) {
-          const uint32_t bv = ar + ((2 * j + 1) % kStages) * L::kKvBytes;
+        for (int w = 0; w < QT; ++w) {
+          const int n = w ? n1 : n0;
+          if (j < n) {
+            const uint32_t v = v_lo + vs * kStep;
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            ok = ok && wait(&p_full[2 * w + part], j & 1);
-            if (!ok) break;
+            for (int part = 0; part < 2; ++part) {
+              ok = ok && wait(&p_full[2 * w + part], j & 1);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < KV / 32; ++k) {
-              const int kk = part * (KV / 32) + k;
-              umma_bf16_ts_if(leader, tmem_base + QT * KV + w * D, tmem_base + w * KV + kk * 8,
-                              umma_smem_desc(bv + kk * 2048, KV * 128, 1024), idesc_o, (j | kk) ? 1u : 0u);
+              for (int k = 0; k < KV / 32; ++k) {
+                const int kk = part * (KV / 32) + k;
+                umma_bf16_ts_lo(tmem_base + QT * KV + w * D, tmem_base + w * KV + kk * 8, v + kk * 128, idesc_o, kk > 0 || j > 0);
+              }
             }
+            if (ok && j + 1 < n) scores(w, ks);
+            else if (ok) umma_commit(&o_full[w]);
           }
-          if (ok && j + 1 == n) umma_commit_if(leader, &o_full[w]);
+          if (w == QT - 1) {
+            umma_commit(&empty[vs]);
+            if (j + 1 < n_max) umma_commit(&empty[ks]);
+          }
         }
-        if (w == QT - 1) umma_commit_if(leader, &empty[(2 * j + 1) % kStages]);
-        if (ok && j + 1 < n) {
-          ok = wait_ring(2 * j + 2);
-          if (ok) scores(w, j + 1);
-        }
+        step(vs, v_phase);
       }
-      if (j + 1 < n_max) umma_commit_if(leader, &empty[(2 * j + 2) % kStages]);
     }
+    __syncwarp();
   } else {
     // ------------------------------ softmax and output: thread = row ------------------------------
     const int w = warp >> 2, row = (warp & 3) * 32 + lane;
@@ -322,7 +354,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int i = i0; i < i0 + 32; i += 2) {
             float2 x = make_float2(__uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
             x = fma_f32x2(x, sc2, neg);
-            if (i % 8 == 6) {
+            if (D == 64 && i % 8 == 6) {
               x = poly_exp2(x);
             } else {
               x.x = fast_exp2(x.x);

@@ -184,7 +184,6 @@ def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, sl
     ``slots[i]`` with ``prefix_lens[i]`` earlier tokens.  K/V of all ``prefix + chunk`` positions are read back from
     the paged cache into one packed buffer, the packed-attention kernel computes only the query tiles that contain
     chunk rows, and the chunk rows of the result are returned ``[sum(chunk_lens), Hq*D]``."""
-    from .attention import SeqInfo, attention_packed
     if isinstance(cache_layer, Cache8):
         if qkv.is_cuda:
             return kv_cache8.chunk_attention(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads,
