@@ -5,23 +5,26 @@
 // e4m3 terms that are columns of one product and are added up afterwards:
 //   * a query row, divided by a power of two, into two terms, the second 16 times enlarged: 4 + 4 bits hold all that a bf16
 //     number has, down to 2^-22 of the row's largest;
-//   * a weight into three terms (each remainder 16 times enlarged): off by at most 2^-12 of itself or 2^-21 of the largest.
+//   * a weight of 2^-4 and more into two terms, the second 16 times enlarged, a smaller one likewise, in two other columns and
+//     4096 times enlarged: off by at most 2^-9 of itself, half of what rounding it to bf16 would cost, or 2^-31 of the largest
+//     weight.  Such a range is needed: thousands of small weights may stand beside one large one whose value is near zero.
 // The block's scales go into the score and into the weight, in 32 bits.
 //
 // A tile is 128 rows of 128 bytes: two cache blocks at D = 128; at D = 64, where a row holds two tokens, four.
 //   S^T[row, (token of the row, term, head)] = K Q^T     A = the K tile, B = the terms of all query heads of a kv head
-//   O^T[byte of a row, (token of the row, term, head)] += V^T W^T    A = the V tile through an MN-major descriptor
+//   O^T[byte of a row, (token of the row, term, head)] += V^T W^T    A = the V tile, B = the weights' terms, a tile row's side by
+//                                                        side as its thread writes them, both through MN-major descriptors
 // The tile fills the 128 rows of the MMA whatever the number of heads, and shared memory is read once per product.  At D = 64
 // only the diagonal (token of the row) blocks of O^T mean something; the query terms of the other token's half are zeros.
 //
-// The tiles of all (sequence, kv head, group of at most 16 query heads) form one list, and every CTA of a persistent grid of
+// The tiles of all (sequence, kv head, group of at most NR query heads) form one list, and every CTA of a persistent grid of
 // one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry; a piece that is not
 // the whole entry leaves a normalised partial result and its log-sum-exp in a workspace, two slots per CTA, and a small
 // kernel merges them.  The warps:
 //   0..7   soft-max, thread = row of the tile.  Four warps take the even tiles of the range, four the odd ones, each with an
 //          O^T and weights' references of its own, so that two tiles are under way and nobody waits for the other four.  A
 //          vote of the four per tile says whether a reference has to be raised (a weight above 2^8; a fresh one puts the
-//          largest weight at 2^3)
+//          largest weight at 2^5)
 //   8..11  output: joins the two O^T of a piece while the next piece's tiles are under way (double-buffered)
 //   12     producer: a ring of K and V tiles, ids and scales of the next 32 cache blocks of the list in registers
 //   13, 14 MMA issuers: scores; weighted sums
@@ -38,6 +41,15 @@ constexpr int kQ8Smem = 227 * 1024;
 constexpr int kQ8MinTiles = 2;       // tiles of a range, where there are so few that not every SM gets as many
 constexpr float kQ8None = -3.0e38f;  // reference before anything has been seen
 
+// mbar_wait() with all but the first look in one place: sixteen warps run seven programs here, and what each of them takes of the
+// instruction cache counts
+__device__ __noinline__ bool bar_wait_on(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return mbar_wait(bar, parity, status, code);
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return mbar_try_wait(bar, parity) || bar_wait_on(bar, parity, status, code);
+}
+
 __device__ __forceinline__ void umma_e4m3_ss_if(uint32_t leader, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
                                                 uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -51,6 +63,11 @@ __device__ __forceinline__ void umma_e4m3_ss_if(uint32_t leader, uint32_t tmem_d
 // kind::f8f6f4 with e4m3 operands and fp32 accumulation
 __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int a_mn, int b_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// descriptor of an MN-major tile whose rows have 32 or 64 bytes: 32- or 64-byte swizzle, groups of eight rows one behind the other
+__device__ __forceinline__ uint64_t umma_desc_rows(uint32_t smem_addr, int row_bytes) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(row_bytes * 8 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)(row_bytes == 32 ? 6 : 4) << 61;
 }
 // largest of a warp
 __device__ __forceinline__ float redux_max(float x) {
@@ -94,7 +111,7 @@ struct Decode8Params {
   int* status;
 };
 
-// NR: query heads of a group (rows of a piece), 8 or 16
+// NR: query heads of a group (rows of a piece), 8 or, at D = 128, 16
 template <int D, int NR>
 struct D8 {
   static constexpr int PACK = 128 / D;             // tokens of a 128-byte row
@@ -102,7 +119,7 @@ struct D8 {
   static constexpr int BPT = 2 * PACK;             // cache blocks of a tile
   static constexpr int TT = 64 * BPT;              // tokens of a tile
   static constexpr int NS = PACK * 2 * NR;         // columns of S^T
-  static constexpr int NO = (PACK * 3 * NR + 15) / 16 * 16;   // columns of O^T: a legal N of the MMA
+  static constexpr int NO = PACK * 4 * NR;         // columns of O^T, bytes of a row of the weights' terms: 32 or 64
   static constexpr int NQ = NS <= 32 ? 4 : 2;      // query buffers
   static constexpr int kQBytes = NS * 128, kPBytes = NO * 128, kStage = 32768;
   static constexpr int kXBytes = PACK == 2 ? 64 * NR * 4 : 0; // the second tokens' share of a result
@@ -168,6 +185,15 @@ __device__ __forceinline__ void tmem_st_heads(uint32_t taddr, const uint32_t (&r
   else tmem_st_32x16(taddr, r);
 }
 
+// a query row times the first D codes of row r of a K tile, in 32 bits
+template <int D>
+__device__ __noinline__ float d8_dot(const __nv_bfloat16* q, const uint8_t* k, int r) {
+  float s = 0.f;
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) s = fmaf(__bfloat162float(q[d]), from_e4m3x2(k[(((d >> 4) ^ (r & 7)) << 4) + (d & 15)]).x, s);
+  return s;
+}
+
 constexpr int kQ8Threads = 16 * 32;
 
 template <int D, int NR>
@@ -208,9 +234,9 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int entries = p.Hkv * p.groups, rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups;
-  // of an entry: kv head, first query head, query heads (one or two groups)
-  auto kv_head = [&](int entry) { return entry >> (p.groups - 1); };
-  auto group_of = [&](int entry) { return entry & (p.groups - 1); };
+  // of an entry: kv head, first query head, query heads
+  auto kv_head = [&](int entry) { return entry / p.groups; };
+  auto group_of = [&](int entry) { return entry % p.groups; };
   auto first_head = [&](int entry) { return kv_head(entry) * rep + group_of(entry) * per_group; };
   auto heads_of = [&](int entry) { return min(per_group, rep - group_of(entry) * per_group); };
   if (tid == 0) {
@@ -307,7 +333,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       const int seen = x.id >= 0 && x.id < p.num_blocks ? min(x.left, 64) : 0;
       for (int k = 0; k < n; ++k, ++tile_no) {
         const int stage = tile_no % NST;
-        if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((tile_no / NST) & 1) ^ 1, p.status, kStatusTimeoutProducer))) {
+        if (!__all_sync(0xffffffffu, bar_wait(&kv_empty[stage], ((tile_no / NST) & 1) ^ 1, p.status, kStatusTimeoutProducer))) {
           ok = false;
           break;
         }
@@ -334,8 +360,8 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     if (!ok) {      // no copy may be in flight when shared memory is given back
       const uint32_t first = tile_no > (uint32_t)NST ? tile_no - NST : 0;
       for (uint32_t j = first; j < tile_no; ++j) {
-        mbar_wait(&k_full[j % NST], (j / NST) & 1, nullptr, 0);
-        mbar_wait(&v_full[j % NST], (j / NST) & 1, nullptr, 0);
+        bar_wait(&k_full[j % NST], (j / NST) & 1, nullptr, 0);
+        bar_wait(&v_full[j % NST], (j / NST) & 1, nullptr, 0);
       }
     }
   } else if (warp == 13) {
@@ -348,7 +374,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     uint32_t phase = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
+      return __all_sync(0xffffffffu, bar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
     };
     for (int i = 0; i < end - begin && ok; ++i) {
       const uint32_t b = i & 1, iq = piece_no % NQ;
@@ -376,14 +402,14 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   } else if (warp == 14) {
     // ------------------------------ weighted sums ------------------------------
     const uint32_t leader = elect_one() ? 1u : 0u;
-    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NO, 1, 0);
-    const uint64_t dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024), dp = umma_smem_desc(smem_u32(sP), 16, 1024);
+    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NO, 1, 1);
+    const uint64_t dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024), dp = umma_desc_rows(smem_u32(sP), L::NO);
     uint32_t piece_no = 0, fresh = 3;      // fresh: groups that have not added to the piece's O^T
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
+      return __all_sync(0xffffffffu, bar_wait(bar, parity, p.status, kStatusTimeoutMma)) != 0;
     };
     D8Piece q;
     if (begin < end) q = d8_piece(s_pre, p.B, entries, begin, end);
@@ -402,7 +428,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + (ib * 2 + b) * L::NO, dv + (uint32_t)stage * (L::kStage >> 4) + 256 * kk,
-                        dp + b * (L::kPBytes >> 4) + 2 * kk, idesc, kk ? 1u : add);
+                        dp + b * (L::kPBytes >> 4) + kk * (32 * L::NO >> 4), idesc, kk ? 1u : add);
       umma_commit_if(leader, &kv_empty[stage]);
       umma_commit_if(leader, &p_empty[b]);
       fresh &= ~(1u << b);
@@ -441,7 +467,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
         load(next, ahead);
       }
       const int iq = piece_no % NQ;
-      if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[iq], ((piece_no / NQ) & 1) ^ 1, p.status, kStatusTimeoutProducer))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(&q_empty[iq], ((piece_no / NQ) & 1) ^ 1, p.status, kStatusTimeoutProducer))) break;
       if (lane == 0) s_piece[iq] = make_int4(q.row, q.entry, q.t0, q.n);
       uint8_t* dst = sQ + iq * L::kQBytes;
 #pragma unroll
@@ -494,14 +520,15 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     const int g = warp >> 2, quarter = warp & 3;      // g: group, parity of its tiles
     const int r = quarter * 32 + lane, part = r / L::RPB, at = (r % L::RPB) * PACK;      // `at`: first token, in its block
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16, tmem_s = tmem_base + lane_off + L::kTmemS + g * L::NS;
-    uint8_t* dst = sP + g * L::kPBytes + (r & 15);
+    uint8_t* dst = sP + g * L::kPBytes + r * L::NO;
+    const int twist = L::NO == 32 ? r >> 2 & 1 : r >> 1 & 3;      // 16-byte pieces lie at their number xor this
     float2* red = s_red + g * 4 * NR;
     int tn = 0;                // first tile of the piece, in the range
     uint32_t turn = 0;         // tiles of the group so far
     uint32_t piece_no = 0;
     bool ok = true, gone = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, kStatusTimeoutEpilogue)) != 0;
+      return __all_sync(0xffffffffu, bar_wait(bar, parity, p.status, kStatusTimeoutEpilogue)) != 0;
     };
     for (; tn < end - begin && !gone; ++piece_no) {
       const uint32_t ib = piece_no & 1, iq = piece_no % NQ;
@@ -553,13 +580,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
             const int left = heads_of(piece.y);
             const __nv_bfloat16* src = p.q + (size_t)piece.x * p.row_stride + (size_t)first_head(piece.y) * D;
 #pragma unroll
-            for (int h = 0; h < NR; ++h) {
-              float s = 0.f;
-#pragma unroll 1
-              for (int d = 0; d < D && h < left; ++d)
-                s = fmaf(__bfloat162float(src[(size_t)h * D + d]), from_e4m3x2(k[(((d >> 4) ^ (r & 7)) << 4) + (d & 15)]).x, s);
-              z[0][h] = s * block.x * p.scale_log2;
-            }
+            for (int h = 0; h < NR; ++h) z[0][h] = h < left ? d8_dot<D>(src + (size_t)h * D, k, r) * block.x * p.scale_log2 : 0.f;
           }
         }
         // a weight beyond 2^8, or a sum that grows out of its reference's reach
@@ -595,7 +616,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
             for (int w = 0; w < 4; ++w) {
               const float2 x = red[w * NR + h];
               a = fmaxf(a, x.x);
-              v = fmaxf(v, x.y - 3.f);
+              v = fmaxf(v, x.y - 5.f);
             }
             l[h] *= fast_exp2(m[h] - a);
             alpha[h] = fast_exp2(M[h] - v);
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
           if (!first && moved) {
             tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < PACK * 3; ++i) {
+            for (int i = 0; i < PACK * 4; ++i) {
               uint32_t o[NR];
               tmem_ld_heads(tmem_o + i * NR, o);
               tmem_ld_wait();
@@ -623,19 +644,35 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
 #pragma unroll
         for (int c = 0; c < PACK; ++c)
 #pragma unroll
-          for (int h = 0; h < NR; h += 2) {
-            l[h] += fast_exp2(z[c][h] - m[h]);
-            l[h + 1] += fast_exp2(z[c][h + 1] - m[h + 1]);
-            float2 w = make_float2(fast_exp2(z[c][h] - M[h] + lv), fast_exp2(z[c][h + 1] - M[h + 1] + lv));
-            if (seen <= c) w = make_float2(0.f, 0.f);      // there may be no scale
+          for (int h8 = 0; h8 < NR; h8 += 8) {
+            uint32_t hi[4], lo[4], low[4];      // codes of two heads, and where they belong to the small ones
 #pragma unroll
-            for (int term = 0; term < 3; ++term) {
-              const uint32_t code = e4m3x2(w.x, w.y);
-              const int row = (c * 3 + term) * NR + h;
-              dst[row * 128 + (((r >> 4) ^ (row & 7)) << 4)] = (uint8_t)code;
-              dst[(row + 1) * 128 + (((r >> 4) ^ ((row + 1) & 7)) << 4)] = (uint8_t)(code >> 8);
-              const float2 f = from_e4m3x2(code);
-              w = make_float2((w.x - f.x) * 16.f, (w.y - f.y) * 16.f);
+            for (int i = 0; i < 4; ++i) {
+              const int h = h8 + 2 * i;
+              l[h] += fast_exp2(z[c][h] - m[h]);
+              l[h + 1] += fast_exp2(z[c][h + 1] - m[h + 1]);
+              float2 w = make_float2(fast_exp2(z[c][h] - M[h] + lv), fast_exp2(z[c][h + 1] - M[h + 1] + lv));
+              if (seen <= c) w = make_float2(0.f, 0.f);      // there may be no scale
+              const bool a = w.x < 0.0625f, b = w.y < 0.0625f;
+              w.x *= a ? 4096.f : 1.f;
+              w.y *= b ? 4096.f : 1.f;
+              low[i] = (a ? 0xffu : 0u) | (b ? 0xff00u : 0u);
+              hi[i] = e4m3x2(w.x, w.y);
+              const float2 f = from_e4m3x2(hi[i]);
+              lo[i] = e4m3x2((w.x - f.x) * 16.f, (w.y - f.y) * 16.f);
+            }
+            auto join = [](uint32_t a, uint32_t b) { return a | b << 16; };
+            const uint2 hi8 = make_uint2(join(hi[0], hi[1]), join(hi[2], hi[3])), lo8 = make_uint2(join(lo[0], lo[1]), join(lo[2], lo[3]));
+            const uint2 low8 = make_uint2(join(low[0], low[1]), join(low[2], low[3]));
+            const uint2 out[4] = {make_uint2(hi8.x & ~low8.x, hi8.y & ~low8.y), make_uint2(lo8.x & ~low8.x, lo8.y & ~low8.y),
+                                  make_uint2(hi8.x & low8.x, hi8.y & low8.y), make_uint2(lo8.x & low8.x, lo8.y & low8.y)};
+            if constexpr (NR == 8) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<uint4*>(dst + ((c * 2 + i) ^ twist) * 16) = make_uint4(out[2 * i].x, out[2 * i].y, out[2 * i + 1].x, out[2 * i + 1].y);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + (i ^ twist) * 16 + h8) = out[i];
             }
           }
         // rows behind the last token may hold anything, NaN too: zero weights alone would not do
@@ -705,7 +742,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     for (int cur = begin; cur < end; ++piece_no) {
       if (cur != begin) d8_next(s_pre, entries, q, cur, end);
       const uint32_t ib = piece_no & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&o_full[ib], (piece_no >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
+      if (!__all_sync(0xffffffffu, bar_wait(&o_full[ib], (piece_no >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
       tc_fence_after();
       // lane h: head h's factors of the two O^T, and its log-sum-exp
       float f[2] = {0.f, 0.f}, lse = -INFINITY;
@@ -730,14 +767,15 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         if (q.n == 1 && g != (cur - begin & 1)) continue;      // one tile: the other group's O^T has not been written
-        uint32_t x[3][NR];
-        const uint32_t at = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO + c * 3 * NR;
+        uint32_t x[4][NR];
+        const uint32_t at = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO + c * 4 * NR;
 #pragma unroll
-        for (int term = 0; term < 3; ++term) tmem_ld_heads(at + term * NR, x[term]);
+        for (int term = 0; term < 4; ++term) tmem_ld_heads(at + term * NR, x[term]);
         tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < NR; ++h) {
-          const float a = fmaf(fmaf(__uint_as_float(x[2][h]), 0.0625f, __uint_as_float(x[1][h])), 0.0625f, __uint_as_float(x[0][h]));
+          const float large = fmaf(__uint_as_float(x[1][h]), 0.0625f, __uint_as_float(x[0][h]));
+          const float a = fmaf(fmaf(__uint_as_float(x[3][h]), 0.0625f, __uint_as_float(x[2][h])), 1.f / 4096.f, large);
           const float w = __shfl_sync(0xffffffffu, f[g], h);
           o[h] += w == 0.f ? 0.f : a * w;
         }
@@ -748,13 +786,13 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       if constexpr (PACK == 2) {
         // the odd tokens' warps hand their share to the even tokens'
         if (c == 1) {
-          if (!__all_sync(0xffffffffu, mbar_wait(x_empty, (piece_no & 1) ^ 1, p.status, kStatusTimeoutEpilogue))) break;
+          if (!__all_sync(0xffffffffu, bar_wait(x_empty, (piece_no & 1) ^ 1, p.status, kStatusTimeoutEpilogue))) break;
 #pragma unroll
           for (int h = 0; h < NR; ++h) s_x[h * 64 + d] = o[h];
           __syncwarp();
           if (lane == 0) mbar_arrive(x_full);
         } else {
-          if (!__all_sync(0xffffffffu, mbar_wait(x_full, piece_no & 1, p.status, kStatusTimeoutEpilogue))) break;
+          if (!__all_sync(0xffffffffu, bar_wait(x_full, piece_no & 1, p.status, kStatusTimeoutEpilogue))) break;
 #pragma unroll
           for (int h = 0; h < NR; ++h) o[h] += s_x[h * 64 + d];
           __syncwarp();
@@ -841,7 +879,7 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
 
 using namespace sb;
 
-// Workspaces: with rows = 8 where at most 8 query heads share a kv head, else 16, ws_o has 2 * grid * rows * D floats,
+// Workspaces: with rows = 8 where at most 8 query heads share a kv head or D = 64, else 16, ws_o has 2 * grid * rows * D floats,
 // ws_lse 2 * grid * rows, ws_pre B + 1 ints.
 extern "C" int sb_kv8_decode_grid() { return num_sms(); }
 
@@ -854,7 +892,7 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || max_blocks < 1 || num_blocks < 1) return -3;
-  const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (long long)(max_blocks + 1) / 2 * B * Hkv * 2;
+  const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (long long)(max_blocks + 1) / 2 * B * Hkv * 4;
   if (rows > 0x7fffffffll || tiles > 0x7fffffffll) return -4;
   static thread_local bool tl_context_bound = false;
   if (!tl_context_bound) {
@@ -868,10 +906,11 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   Decode8Params p;
   p.q = (const __nv_bfloat16*)q; p.row_stride = row_stride; p.scales = scales; p.seq_lens = seq_lens;
   p.block_table = block_table; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
-  p.groups = Hq / Hkv > 16 ? 2 : 1;
+  const int most = Hq / Hkv <= 8 || D == 64 ? 8 : 16;
+  p.groups = (Hq / Hkv + most - 1) / most;
   p.out = (__nv_bfloat16*)out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.ws_pre = ws_pre;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   const int grid = num_sms();
-  if (Hq / Hkv <= 8) return D == 128 ? launch_decode8<128, 8>(mc, p, grid, stream) : launch_decode8<64, 8>(mc, p, grid, stream);
-  return D == 128 ? launch_decode8<128, 16>(mc, p, grid, stream) : launch_decode8<64, 16>(mc, p, grid, stream);
+  if (D == 64) return launch_decode8<64, 8>(mc, p, grid, stream);
+  return most == 8 ? launch_decode8<128, 8>(mc, p, grid, stream) : launch_decode8<128, 16>(mc, p, grid, stream);
 }

@@ -244,7 +244,7 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
     codes, scales = cache
     stride, max_blocks = q_rows.stride(0), block_table.shape[1]
     with _device(q_rows.get_device()):
-        part = 2 * L.sb_kv8_decode_grid() * (8 if n_heads <= 8 * n_kv_heads else 16)
+        part = 2 * L.sb_kv8_decode_grid() * (8 if n_heads <= 8 * n_kv_heads or head_dim == 64 else 16)
         for at in range(0, B, ROWS):
             n = min(ROWS, B - at)
             # two partial results per block of the grid, and the sequences' places in the list of tiles.  A buffer of the
