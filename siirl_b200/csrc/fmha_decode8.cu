@@ -2,12 +2,11 @@
 //
 // o = sum_t softmax(scale q . k_t)_t v_t with k_t = ks * code, v_t = vs * code, one ks and vs per cache block and head.  Both
 // products run on codes as they lie in the cache: nothing is converted on the way.  What meets the codes is split instead, into
-// e4m3 terms that are columns of one product and are added up afterwards:
-//   * a query row, divided by a power of two, into two terms, the second 16 times enlarged: 4 + 4 bits hold all that a bf16
+// 8-bit terms that are columns of one product and are added up afterwards:
+//   * a query row, divided by a power of two, into two e4m3 terms, the second 16 times enlarged: 4 + 4 bits hold all that a bf16
 //     number has, down to 2^-22 of the row's largest;
-//   * a weight of 2^-4 and more into two terms, the second 16 times enlarged, a smaller one likewise, in two other columns and
-//     4096 times enlarged: off by at most 2^-9 of itself, half of what rounding it to bf16 would cost, or 2^-31 of the largest
-//     weight.  Such a range is needed: thousands of small weights may stand beside one large one whose value is near zero.
+//   * a weight into three e5m2 terms, each remainder 16 times enlarged: off by at most 2^-11 of itself or 2^-36 of the largest
+//     weight.  e5m2 for its range: thousands of small weights may stand beside one large one whose value is near zero.
 // The block's scales go into the score and into the weight, in 32 bits.
 //
 // A tile is 128 rows of 128 bytes: two cache blocks at D = 128; at D = 64, where a row holds two tokens, four.
@@ -21,10 +20,10 @@
 // one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry; a piece that is not
 // the whole entry leaves a normalised partial result and its log-sum-exp in a workspace, two slots per CTA, and a small
 // kernel merges them.  The warps:
-//   0..7   soft-max, thread = row of the tile.  Four warps take the even tiles of the range, four the odd ones, each with an
-//          O^T and weights' references of its own, so that two tiles are under way and nobody waits for the other four.  A
-//          vote of the four per tile says whether a reference has to be raised (a weight above 2^8; a fresh one puts the
-//          largest weight at 2^5)
+//   0..7   soft-max in two groups, each with an O^T and weights' references of its own.  D = 128: thread = row of the tile, the
+//          first four warps take the even tiles of the range, the others the odd ones, so that two tiles are under way.
+//          D = 64: the groups take the first and the second tokens of every tile's rows.  A vote of the group per tile says
+//          whether a reference has to be raised (a weight above 2^14; a fresh one puts the largest weight at 2^11)
 //   8..11  output: joins the two O^T of a piece while the next piece's tiles are under way (double-buffered)
 //   12     producer: a ring of K and V tiles, ids and scales of the next 32 cache blocks of the list in registers
 //   13, 14 MMA issuers: scores; weighted sums
@@ -60,9 +59,9 @@ __device__ __forceinline__ void umma_e4m3_ss_if(uint32_t leader, uint32_t tmem_d
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-// kind::f8f6f4 with e4m3 operands and fp32 accumulation
-__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int a_mn, int b_mn) {
-  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+// kind::f8f6f4 with e4m3 operands, or B in e5m2, and fp32 accumulation
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int a_mn, int b_mn, int b_e5m2) {
+  return (1u << 4) | ((uint32_t)b_e5m2 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // descriptor of an MN-major tile whose rows have 32 or 64 bytes: 32- or 64-byte swizzle, groups of eight rows one behind the other
 __device__ __forceinline__ uint64_t umma_desc_rows(uint32_t smem_addr, int row_bytes) {
@@ -74,6 +73,11 @@ __device__ __forceinline__ float redux_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
 }
 // whether `any` is set in one of the 128 threads of four soft-max warps
 __device__ __forceinline__ bool vote_128(int group, bool any) {
@@ -93,6 +97,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
 }
 __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+__device__ __forceinline__ uint32_t e5m2x2(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E5M2);
+}
+__device__ __forceinline__ float2 from_e5m2x2(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E5M2);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
@@ -119,7 +131,8 @@ struct D8 {
   static constexpr int BPT = 2 * PACK;             // cache blocks of a tile
   static constexpr int TT = 64 * BPT;              // tokens of a tile
   static constexpr int NS = PACK * 2 * NR;         // columns of S^T
-  static constexpr int NO = PACK * 4 * NR;         // columns of O^T, bytes of a row of the weights' terms: 32 or 64
+  static constexpr int NO = PACK * 4 * NR;         // columns of O^T, bytes of a row of the weights' terms: 32 or 64, the last
+                                                   // quarter of a token's unused
   static constexpr int NQ = NS <= 32 ? 4 : 2;      // query buffers
   static constexpr int kQBytes = NS * 128, kPBytes = NO * 128, kStage = 32768;
   static constexpr int kXBytes = PACK == 2 ? 64 * NR * 4 : 0; // the second tokens' share of a result
@@ -135,9 +148,10 @@ struct D8 {
   static constexpr int kBars = 3 * kStages + 2 * NQ + 14;
   static constexpr int kPreOff = kBarOff + kBars * 8 + 24;
   static constexpr int kTotal = kPreOff + (2 * kQ8Rows + 1 + 32) * 4;
-  // TMEM columns: S^T of the two groups, O^T [2 buffers][2 groups]
+  // TMEM columns: S^T of two tiles, O^T of two pieces
   static constexpr int kTmemS = 0, kTmemO = 2 * NS;
-  static constexpr int kTmemCols = 2 * NS + 4 * NO <= 256 ? 256 : 512;
+  static constexpr int kOBuffer = (3 - PACK) * NO;                     // columns of O^T of a piece: each group's own
+  static constexpr int kTmemCols = 2 * (NS + kOBuffer) <= 256 ? 256 : 512;
 };
 
 struct D8Piece {
@@ -235,8 +249,8 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int entries = p.Hkv * p.groups, rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups;
   // of an entry: kv head, first query head, query heads
-  auto kv_head = [&](int entry) { return entry / p.groups; };
-  auto group_of = [&](int entry) { return entry % p.groups; };
+  auto kv_head = [&](int entry) { return p.groups == 1 ? entry : entry / p.groups; };
+  auto group_of = [&](int entry) { return p.groups == 1 ? 0 : entry % p.groups; };
   auto first_head = [&](int entry) { return kv_head(entry) * rep + group_of(entry) * per_group; };
   auto heads_of = [&](int entry) { return min(per_group, rep - group_of(entry) * per_group); };
   if (tid == 0) {
@@ -248,8 +262,8 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 4);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&s_empty[i], 4 * PACK);
+      mbar_init(&p_full[i], 4 * PACK);
       mbar_init(&p_empty[i], 1);
       mbar_init(&o_full[i], 9);      // the MMAs, the statistics of the soft-max warps
       mbar_init(&o_empty[i], 4);
@@ -263,6 +277,8 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
+  if (NR == 16)      // the unused quarters
+    for (int i = tid; i < 2 * L::kPBytes / 16; i += kQ8Threads) reinterpret_cast<uint4*>(sP)[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -346,7 +362,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
           tma_load_2d(dst, &map_c, &k_full[stage], 0, row);
           tma_load_2d(dst + 16384, &map_c, &v_full[stage], 0, row + p.Hkv * L::RPB);
         }
-        if (mine) s_block[stage * BPT + part] = make_float4(x.ks, __log2f(x.vs), __int_as_float(seen), 0.f);
+        if (mine) s_block[stage * BPT + part] = make_float4(x.ks, seen ? __log2f(x.vs) : 0.f, __int_as_float(seen), 0.f);
         __syncwarp();
         if (lane == 0) {      // the copies may be there already: a phase ends with its arrival
           mbar_arrive_expect_tx(&k_full[stage], bytes);
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   } else if (warp == 13) {
     // ------------------------------ scores (the whole warp, converged; one lane issues) ------------------------------
     const uint32_t leader = elect_one() ? 1u : 0u;
-    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NS, 0, 0);
+    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NS, 0, 0, 0);
     const uint64_t dk = umma_smem_desc(smem_u32(smem), 16, 1024), dq = umma_smem_desc(smem_u32(sQ), 16, 1024);
     uint32_t piece_no = 0;
     int left = 0, stage = 0;
@@ -402,9 +418,9 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   } else if (warp == 14) {
     // ------------------------------ weighted sums ------------------------------
     const uint32_t leader = elect_one() ? 1u : 0u;
-    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NO, 1, 1);
+    constexpr uint32_t idesc = umma_idesc_e4m3(128, L::NO, 1, 1, 1);
     const uint64_t dv = umma_smem_desc(smem_u32(smem) + 16384, 16384, 1024), dp = umma_desc_rows(smem_u32(sP), L::NO);
-    uint32_t piece_no = 0, fresh = 3;      // fresh: groups that have not added to the piece's O^T
+    uint32_t piece_no = 0, fresh = 3;      // fresh: parts of the piece's O^T that nothing has been added to
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -424,14 +440,14 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       ok = ok && wait(&v_full[stage], phase) && wait(&p_full[b], (i >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t add = ~fresh >> b & 1;
+      const uint32_t part = PACK == 1 ? b : 0, add = ~fresh >> part & 1;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + (ib * 2 + b) * L::NO, dv + (uint32_t)stage * (L::kStage >> 4) + 256 * kk,
+        umma_e4m3_ss_if(leader, tmem_base + L::kTmemO + ib * L::kOBuffer + part * L::NO, dv + (uint32_t)stage * (L::kStage >> 4) + 256 * kk,
                         dp + b * (L::kPBytes >> 4) + kk * (32 * L::NO >> 4), idesc, kk ? 1u : add);
       umma_commit_if(leader, &kv_empty[stage]);
       umma_commit_if(leader, &p_empty[b]);
-      fresh &= ~(1u << b);
+      fresh &= ~(1u << part);
       if (--left == 0) {
         umma_commit_if(leader, &o_full[ib]);
         ++piece_no;
@@ -516,15 +532,16 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
         for (int e = 0; e < E / 2; ++e) raw[r][e] = ahead[r][e];
     }
   } else if (warp < 8) {
-    // ------------------------------ soft-max: thread = row of the tile ------------------------------
-    const int g = warp >> 2, quarter = warp & 3;      // g: group, parity of its tiles
-    const int r = quarter * 32 + lane, part = r / L::RPB, at = (r % L::RPB) * PACK;      // `at`: first token, in its block
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16, tmem_s = tmem_base + lane_off + L::kTmemS + g * L::NS;
-    uint8_t* dst = sP + g * L::kPBytes + r * L::NO;
-    const int twist = L::NO == 32 ? r >> 2 & 1 : r >> 1 & 3;      // 16-byte pieces lie at their number xor this
+    // ------------------------------ soft-max ------------------------------
+    const int g = warp >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane, part = r / L::RPB;                     // row of the tile, its cache block
+    const int at = (r % L::RPB) * PACK + (PACK == 2 ? g : 0);                 // the thread's token, in its block
+    const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16), col = PACK == 2 ? g * 2 * NR : 0;
+    const int twist = L::NO == 32 ? r >> 2 & 1 : r >> 1 & 3;      // 16-byte pieces of a row of the weights lie at their number xor this
     float2* red = s_red + g * 4 * NR;
     int tn = 0;                // first tile of the piece, in the range
-    uint32_t turn = 0;         // tiles of the group so far
+    int stage = PACK == 1 ? g : 0;      // ring place of the group's next tile, and its turn
+    uint32_t round = 0;
     uint32_t piece_no = 0;
     bool ok = true, gone = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -532,168 +549,201 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     };
     for (; tn < end - begin && !gone; ++piece_no) {
       const uint32_t ib = piece_no & 1, iq = piece_no % NQ;
-      const uint32_t tmem_o = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO;
+      const uint32_t tmem_o = tmem + L::kTmemO + ib * L::kOBuffer + g * 4 * NR;
       ok = ok && wait(&q_full[iq], (piece_no / NQ) & 1);
       const int4 piece = s_piece[iq];
-      const float* factor = s_factor + iq * NR;
+      const float2* factor = reinterpret_cast<const float2*>(s_factor + iq * NR);
       // a warp that has given up says so in the next vote
       const int stop = ok ? tn + piece.w : tn + 2;
-      float m[NR], M[NR], l[NR];
+      // two heads in each: references of the sums and of the weights, with their signs turned, and the sums
+      float2 m[NR / 2], M[NR / 2], l[NR / 2];
 #pragma unroll
-      for (int h = 0; h < NR; ++h) {
-        m[h] = M[h] = kQ8None;
-        l[h] = 0.f;
+      for (int i = 0; i < NR / 2; ++i) {
+        m[i] = M[i] = make_float2(-kQ8None, -kQ8None);
+        l[i] = make_float2(0.f, 0.f);
       }
       bool first = true;
-      for (int t = tn + ((tn ^ g) & 1); t < stop; t += 2, ++turn) {
-        const uint32_t stage = (uint32_t)t % NST, round = (uint32_t)t / NST & 1;
-        ok = ok && wait(&k_full[stage], round) && wait(&s_full[g], turn & 1);
-        if (!ok) s_fail[2 * g] = 1;
+      for (int t = PACK == 1 ? tn + ((tn ^ g) & 1) : tn; t < stop; t += 3 - PACK) {
+        const uint32_t b = t & 1, phase = t >> 1 & 1;
+        ok = ok && wait(&s_full[b], phase);
         tc_fence_after();
-        const float4 block = s_block[stage * BPT + part];
-        const float lv = block.y;
-        const int seen = __float_as_int(block.z) - at;      // tokens of the row: more than 0, more than 1
-        float z[PACK][NR];
-#pragma unroll
-        for (int c = 0; c < PACK; ++c) {
+        float4 block;
+        int left;      // tokens of the block from this one on
+        float2 z[NR / 2];
+        {
           uint32_t raw[2][NR];
-          tmem_ld_heads(tmem_s + (c * 2) * NR, raw[0]);
-          tmem_ld_heads(tmem_s + (c * 2 + 1) * NR, raw[1]);
+          tmem_ld_heads(tmem + L::kTmemS + b * L::NS + col, raw[0]);
+          tmem_ld_heads(tmem + L::kTmemS + b * L::NS + col + NR, raw[1]);
+          // meanwhile: the tile's scales (its keys' barrier has long turned), and the weighted sum of the tile two before, which
+          // has read the buffer that the weights go to
+          ok = ok && wait(&k_full[stage], round) && wait(&p_empty[b], phase ^ 1);
+          if (!ok) s_fail[2 * g] = 1;
+          block = s_block[stage * BPT + part];
+          left = __float_as_int(block.z) - at;
           tmem_ld_wait();
 #pragma unroll
-          for (int h = 0; h < NR; ++h) {
-            const float s = fmaf(__uint_as_float(raw[1][h]), 0.0625f, __uint_as_float(raw[0][h]));
-            z[c][h] = seen > c ? s * (block.x * factor[h]) : -INFINITY;
+          for (int i = 0; i < NR / 2; ++i) {
+            const float2 hi = make_float2(__uint_as_float(raw[0][2 * i]), __uint_as_float(raw[0][2 * i + 1]));
+            const float2 lo = make_float2(__uint_as_float(raw[1][2 * i]), __uint_as_float(raw[1][2 * i + 1]));
+            z[i] = mul_f32x2(fma_f32x2(lo, make_float2(0.0625f, 0.0625f), hi), mul_f32x2(factor[i], make_float2(block.x, block.x)));
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[g]);
+        if (lane == 0) mbar_arrive(&s_empty[b]);
+        const float lv = block.y;
+        const bool seen = left > 0, whole = __all_sync(0xffffffffu, seen);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < NR / 2; ++i)
+            if (!seen) z[i] = make_float2(-INFINITY, -INFINITY);
+        }
         if constexpr (PACK == 2) {
-          // The last token shares its row with what lies behind it: where that is NaN, zero times it has spoilt the sums, and
-          // the scores are computed here
-          bool spoilt = false;
+          if (g == 0 && __any_sync(0xffffffffu, left == 1)) {
+            // The last token shares its row with what lies behind it: where that is NaN, zero times it has spoilt the sums, and
+            // the scores are computed here
+            bool spoilt = false;
 #pragma unroll
-          for (int h = 0; h < NR; ++h) spoilt |= z[0][h] != z[0][h];
-          if (spoilt && seen == 1) {
-            const uint8_t* k = smem + stage * L::kStage + r * 128;
-            const int left = heads_of(piece.y);
-            const __nv_bfloat16* src = p.q + (size_t)piece.x * p.row_stride + (size_t)first_head(piece.y) * D;
+            for (int i = 0; i < NR / 2; ++i) spoilt |= z[i].x != z[i].x || z[i].y != z[i].y;
+            if (spoilt && left == 1) {
+              const uint8_t* k = smem + stage * L::kStage + r * 128;
+              const int heads = heads_of(piece.y);
+              const __nv_bfloat16* src = p.q + (size_t)piece.x * p.row_stride + (size_t)first_head(piece.y) * D;
+              const float f = block.x * p.scale_log2;
 #pragma unroll
-            for (int h = 0; h < NR; ++h) z[0][h] = h < left ? d8_dot<D>(src + (size_t)h * D, k, r) * block.x * p.scale_log2 : 0.f;
+              for (int i = 0; i < NR / 2; ++i)
+                z[i] = make_float2(2 * i < heads ? d8_dot<D>(src + (size_t)(2 * i) * D, k, r) * f : 0.f,
+                                   2 * i + 1 < heads ? d8_dot<D>(src + (size_t)(2 * i + 1) * D, k, r) * f : 0.f);
+            }
           }
         }
-        // a weight beyond 2^8, or a sum that grows out of its reference's reach
-        bool raise = first || !ok;
+        // exponents of the sums' and of the weights' terms
+        float2 e[NR / 2], d[NR / 2];
+        float top_e = -INFINITY, top_d = -INFINITY;
+        auto exponents = [&]() {
 #pragma unroll
-        for (int h = 0; h < NR; ++h) {
-          const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
-          raise |= top + lv > M[h] + 8.f || top > m[h] + 64.f;
+          for (int i = 0; i < NR / 2; ++i) {
+            e[i] = add_f32x2(z[i], m[i]);
+            d[i] = add_f32x2(add_f32x2(z[i], M[i]), make_float2(lv, lv));
+          }
+        };
+        exponents();
+#pragma unroll
+        for (int i = 0; i < NR / 2; ++i) {
+          top_e = fmaxf(top_e, fmaxf(e[i].x, e[i].y));
+          top_d = fmaxf(top_d, fmaxf(d[i].x, d[i].y));
         }
-        if (vote_128(g, raise)) {
+        // a weight beyond 2^14, or a sum that grows out of its reference's reach
+        if (vote_128(g, first || !ok || top_d > 14.f || top_e > 64.f)) {
           // a wait that ran out: all four warps leave together, or the others would stay in a vote.  One flag per vote: a
           // warp may be ahead of the others by what lies between two votes
           gone = s_fail[2 * g];
           if (gone) break;
+          float top = -INFINITY;
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
-            const float top = PACK == 2 ? fmaxf(z[0][h], z[PACK - 1][h]) : z[0][h];
-            const float a = redux_max(top), v = redux_max(top == -INFINITY ? -INFINITY : top + lv);
-            if (lane == h) red[quarter * NR + h] = make_float2(a, v);
+            const float a = redux_max(h & 1 ? z[h / 2].y : z[h / 2].x);
+            if (lane == h) top = a;
           }
+          if (lane < NR) red[quarter * NR + lane] = make_float2(top, top + lv);      // the warp's rows lie in one cache block
           // O^T is scaled below: the products of the group's tile before have to be in it
-          if (!first) ok = wait(&p_empty[g], (turn & 1) ^ 1);
+          if (PACK == 2 && !first) ok = wait(&p_empty[b ^ 1], (t - 1) >> 1 & 1);
           if (!ok) s_fail[2 * g + 1] = 1;
           vote_128(g, false);
           gone = s_fail[2 * g + 1];
           if (gone) break;
-          bool moved = false;
-          float alpha[NR];
-#pragma unroll
-          for (int h = 0; h < NR; ++h) {
-            float a = m[h], v = M[h];
+          // lane h: head h's new references (0 where there is none to turn)
+          float a = -kQ8None, v = -kQ8None;
+          if (lane < NR) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const float2 x = red[w * NR + h];
-              a = fmaxf(a, x.x);
-              v = fmaxf(v, x.y - 5.f);
+              const float2 x = red[w * NR + lane];
+              a = fminf(a, -x.x);
+              v = fminf(v, 11.f - x.y);
             }
-            l[h] *= fast_exp2(m[h] - a);
-            alpha[h] = fast_exp2(M[h] - v);
-            moved |= v != M[h];
-            m[h] = a;
-            M[h] = v;
           }
-          if (!first && moved) {
-            tc_fence_after();
+          bool moved = false;
+          float2 alpha[NR / 2];
 #pragma unroll
-            for (int i = 0; i < PACK * 4; ++i) {
+          for (int i = 0; i < NR / 2; ++i) {
+            const float2 m2 = make_float2(fminf(m[i].x, __shfl_sync(0xffffffffu, a, 2 * i)), fminf(m[i].y, __shfl_sync(0xffffffffu, a, 2 * i + 1)));
+            const float2 M2 = make_float2(fminf(M[i].x, __shfl_sync(0xffffffffu, v, 2 * i)), fminf(M[i].y, __shfl_sync(0xffffffffu, v, 2 * i + 1)));
+            if (!first) {
+              l[i].x *= fast_exp2(m2.x - m[i].x);
+              l[i].y *= fast_exp2(m2.y - m[i].y);
+              alpha[i] = make_float2(fast_exp2(M2.x - M[i].x), fast_exp2(M2.y - M[i].y));
+              moved |= M2.x != M[i].x || M2.y != M[i].y;
+            }
+            m[i] = m2;
+            M[i] = M2;
+          }
+          if (moved) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < 3; ++i) {
               uint32_t o[NR];
               tmem_ld_heads(tmem_o + i * NR, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < NR; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * alpha[h]);
+              for (int h = 0; h < NR; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * (h & 1 ? alpha[h / 2].y : alpha[h / 2].x));
               tmem_st_heads(tmem_o + i * NR, o);
             }
             tmem_st_wait();
           }
+          exponents();
         }
         first = false;
-        // the weighted sum of the group's tile before has read this buffer
-        ok = ok && wait(&p_empty[g], (turn & 1) ^ 1);
+        uint8_t* dst = sP + b * L::kPBytes + r * L::NO;
 #pragma unroll
-        for (int c = 0; c < PACK; ++c)
+        for (int h8 = 0; h8 < NR; h8 += 8) {
+          uint32_t code[3][4];      // of two heads each
 #pragma unroll
-          for (int h8 = 0; h8 < NR; h8 += 8) {
-            uint32_t hi[4], lo[4], low[4];      // codes of two heads, and where they belong to the small ones
+          for (int i = 0; i < 4; ++i) {
+            const int j = h8 / 2 + i;
+            l[j] = add_f32x2(l[j], make_float2(fast_exp2(e[j].x), fast_exp2(e[j].y)));
+            float2 w = make_float2(fast_exp2(d[j].x), fast_exp2(d[j].y));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int h = h8 + 2 * i;
-              l[h] += fast_exp2(z[c][h] - m[h]);
-              l[h + 1] += fast_exp2(z[c][h + 1] - m[h + 1]);
-              float2 w = make_float2(fast_exp2(z[c][h] - M[h] + lv), fast_exp2(z[c][h + 1] - M[h + 1] + lv));
-              if (seen <= c) w = make_float2(0.f, 0.f);      // there may be no scale
-              const bool a = w.x < 0.0625f, b = w.y < 0.0625f;
-              w.x *= a ? 4096.f : 1.f;
-              w.y *= b ? 4096.f : 1.f;
-              low[i] = (a ? 0xffu : 0u) | (b ? 0xff00u : 0u);
-              hi[i] = e4m3x2(w.x, w.y);
-              const float2 f = from_e4m3x2(hi[i]);
-              lo[i] = e4m3x2((w.x - f.x) * 16.f, (w.y - f.y) * 16.f);
-            }
-            auto join = [](uint32_t a, uint32_t b) { return a | b << 16; };
-            const uint2 hi8 = make_uint2(join(hi[0], hi[1]), join(hi[2], hi[3])), lo8 = make_uint2(join(lo[0], lo[1]), join(lo[2], lo[3]));
-            const uint2 low8 = make_uint2(join(low[0], low[1]), join(low[2], low[3]));
-            const uint2 out[4] = {make_uint2(hi8.x & ~low8.x, hi8.y & ~low8.y), make_uint2(lo8.x & ~low8.x, lo8.y & ~low8.y),
-                                  make_uint2(hi8.x & low8.x, hi8.y & low8.y), make_uint2(lo8.x & low8.x, lo8.y & low8.y)};
-            if constexpr (NR == 8) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<uint4*>(dst + ((c * 2 + i) ^ twist) * 16) = make_uint4(out[2 * i].x, out[2 * i].y, out[2 * i + 1].x, out[2 * i + 1].y);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(dst + (i ^ twist) * 16 + h8) = out[i];
+            for (int term = 0; term < 3; ++term) {
+              code[term][i] = e5m2x2(w.x, w.y);
+              w = fma_f32x2(from_e5m2x2(code[term][i]), make_float2(-16.f, -16.f), mul_f32x2(w, make_float2(16.f, 16.f)));
             }
           }
-        // rows behind the last token may hold anything, NaN too: zero weights alone would not do
-        if (__any_sync(0xffffffffu, seen < PACK)) {
+          auto join = [](const uint32_t (&x)[4]) { return make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16); };
+          const uint2 a = join(code[0]), b = join(code[1]), c = join(code[2]);
+          if constexpr (NR == 8) {
+            *reinterpret_cast<uint4*>(dst + ((PACK == 2 ? g * 2 : 0) ^ twist) * 16) = make_uint4(a.x, a.y, b.x, b.y);
+            *reinterpret_cast<uint4*>(dst + (((PACK == 2 ? g * 2 : 0) + 1) ^ twist) * 16) = make_uint4(c.x, c.y, 0u, 0u);
+          } else {
+            *reinterpret_cast<uint2*>(dst + (0 ^ twist) * 16 + h8) = a;
+            *reinterpret_cast<uint2*>(dst + (1 ^ twist) * 16 + h8) = b;
+            *reinterpret_cast<uint2*>(dst + (2 ^ twist) * 16 + h8) = c;
+          }
+        }
+        // what lies behind the last token may be anything, NaN too: zero weights alone would not do
+        if (!whole) {
           ok = ok && wait(&v_full[stage], round);
           uint8_t* v = smem + stage * L::kStage + 16384 + r * 128;
+          if (!seen)
 #pragma unroll
-          for (int c = 0; c < PACK; ++c)
-            if (seen <= c)
-#pragma unroll
-              for (int i = 0; i < 8 / PACK; ++i)
-                *reinterpret_cast<uint4*>(v + (((c * (8 / PACK) + i) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8 / PACK; ++i)
+              *reinterpret_cast<uint4*>(v + ((((PACK == 2 ? g * 4 : 0) + i) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g]);
+        if (lane == 0) mbar_arrive(&p_full[b]);
+        stage += 3 - PACK;
+        if (stage >= NST) {
+          stage -= NST;
+          round ^= 1;
+        }
       }
       if (gone) break;
       tn = stop;
       // sums over the warp: half of the heads go to the other half of the lanes at every step
+      float sum[NR];
+#pragma unroll
+      for (int h = 0; h < NR; ++h) sum[h] = h & 1 ? l[h / 2].y : l[h / 2].x;
 #pragma unroll
       for (int n = NR, o = 16; o > 0; o >>= 1) {
         if (n > 1) {
@@ -702,23 +752,23 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
           for (int i = 0; i < NR / 2; ++i)
             if (i < n) {
               const bool up = lane & o;
-              const float mine = up ? l[i + n] : l[i], other = up ? l[i] : l[i + n];
-              l[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+              const float mine = up ? sum[i + n] : sum[i], other = up ? sum[i] : sum[i + n];
+              sum[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
             }
         } else {
-          l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+          sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
         }
       }
       float* stat = s_stat + (ib * 2 + g) * 6 * NR;
       ok = ok && wait(&o_empty[ib], ((piece_no >> 1) & 1) ^ 1);
       constexpr int kLow = NR == 8 ? 2 : 1;      // lane bits below are copies
-      if ((lane & ((1 << kLow) - 1)) == 0) stat[quarter * NR + (lane >> kLow)] = l[0];
+      if ((lane & ((1 << kLow) - 1)) == 0) stat[quarter * NR + (lane >> kLow)] = sum[0];
       if (quarter == 0) {
 #pragma unroll
-        for (int h = 0; h < NR; ++h)
-          if (lane == h) {
-            stat[4 * NR + h] = m[h];
-            stat[5 * NR + h] = M[h];
+        for (int i = 0; i < NR / 2; ++i)
+          if (lane == i) {
+            *reinterpret_cast<float2*>(stat + 4 * NR + 2 * i) = make_float2(-m[i].x, -m[i].y);
+            *reinterpret_cast<float2*>(stat + 5 * NR + 2 * i) = make_float2(-M[i].x, -M[i].y);
           }
       }
       __syncwarp();
@@ -764,19 +814,19 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       float o[NR];
 #pragma unroll
       for (int h = 0; h < NR; ++h) o[h] = 0.f;
+      // D = 128: both groups' O^T; D = 64: of the tokens that stand where the thread's byte does
+#pragma unroll 1
+      for (int g = PACK == 2 ? c : 0; g < (PACK == 2 ? c + 1 : 2); ++g) {
+        if (PACK == 1 && q.n == 1 && g != (cur - begin & 1)) continue;      // one tile: the other group's has not been written
+        uint32_t x[3][NR];
+        const uint32_t at = tmem_base + lane_off + L::kTmemO + ib * L::kOBuffer + g * 4 * NR;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (q.n == 1 && g != (cur - begin & 1)) continue;      // one tile: the other group's O^T has not been written
-        uint32_t x[4][NR];
-        const uint32_t at = tmem_base + lane_off + L::kTmemO + (ib * 2 + g) * L::NO + c * 4 * NR;
-#pragma unroll
-        for (int term = 0; term < 4; ++term) tmem_ld_heads(at + term * NR, x[term]);
+        for (int term = 0; term < 3; ++term) tmem_ld_heads(at + term * NR, x[term]);
         tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < NR; ++h) {
-          const float large = fmaf(__uint_as_float(x[1][h]), 0.0625f, __uint_as_float(x[0][h]));
-          const float a = fmaf(fmaf(__uint_as_float(x[3][h]), 0.0625f, __uint_as_float(x[2][h])), 1.f / 4096.f, large);
-          const float w = __shfl_sync(0xffffffffu, f[g], h);
+          const float a = fmaf(fmaf(__uint_as_float(x[2][h]), 0.0625f, __uint_as_float(x[1][h])), 0.0625f, __uint_as_float(x[0][h]));
+          const float w = __shfl_sync(0xffffffffu, g ? f[1] : f[0], h);
           o[h] += w == 0.f ? 0.f : a * w;
         }
       }
@@ -860,7 +910,7 @@ __global__ void __launch_bounds__(128) fmha_decode8_merge_kernel(Decode8Params p
 template <int D, int NR>
 static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int grid, cudaStream_t stream) {
   using L = D8<D, NR>;
-  static_assert(L::kStages >= 4 && L::kTotal <= kQ8Smem && 2 * L::NS + 4 * L::NO <= 512 && L::kTotal % 4 == 0, "");
+  static_assert(L::kStages >= 4 && L::kTotal <= kQ8Smem && 2 * (L::NS + L::kOBuffer) <= 512 && L::kTotal % 4 == 0, "");
   auto kernel = fmha_decode8_kernel<D, NR>;
   static int configured = -1;
   int dev = 0;

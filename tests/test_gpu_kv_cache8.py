@@ -90,6 +90,16 @@ def test_append_single_rows(hq, hkv, d, rows):
     _check_append(cache, x.bfloat16(), at.clamp(min=0) + 5, None, seq, at, table, hq, hkv, d)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 128), (6, 1, 64)])
+def test_append_partial_sums_of_chunks(hq, hkv, d):
+    lens, width = (150, 70, 1), (hq + 2 * hkv) * d
+    cache = _random_cache(8, hkv, d)
+    table = torch.tensor([[0, 1, 2, 3], [4, 5, -1, -1], [6, 7, -1, -1]], dtype=torch.int32)
+    seq = torch.repeat_interleave(torch.arange(3, dtype=torch.int32), torch.tensor(lens))
+    at = torch.cat([torch.arange(s, s + n, dtype=torch.int32) for n, s in zip(lens, (40, 0, 64))])
+    _check_append(cache, torch.randn(2, sum(lens), width), at, None, seq, at, table, hq, hkv, d, 2, torch.randn(width).bfloat16())
+
+
 @pytest.mark.parametrize("hq,hkv,d,slabs,bias", [(28, 4, 128, 3, True), (14, 2, 64, 1, False), (2, 2, 64, 5, True)])
 def test_append_partial_sums(hq, hkv, d, slabs, bias):
     rows, width = 13, (hq + 2 * hkv) * d
@@ -184,8 +194,10 @@ def _decode(lens, hq, hkv, d, max_blocks, spread=1.0, q_scale=1.0, stride=0):
 
 
 def _check_decode(cache, table, q, lens, hq, hkv, d, scale=None):
-    """Bounds: the output is rounded to bf16; weights carry at most 2^-11 of their value or 2^-18 of the largest weight (three e4m3
-    terms), scores 2^-22 sum |q k| and 2^-20 of themselves; sums of 32 bits over n tokens stay below that."""
+    """Bounds: the output is rounded to bf16.  A weight of 2^e to 2^(e + 1) is kept as three e5m2 terms: the first is off by at most
+    2^(e - 3), so that the second is below 2^(e - 3) and off by at most 2^(e - 7), and the third, likewise, by 2^(e - 11): 2^-11 of
+    the weight, or 2^-36 of the largest one.  Scores carry 2^-22 sum |q k| and 2^-20 of themselves; these and sums of 32 bits
+    over n tokens stay below 2^-11 together."""
     g = _gpu(cache)
     out = kvc.decode_attention(q.to(DEV), g, lens.to(DEV), table.to(DEV), hq, hkv, d, scale)
     lib.check_status()
@@ -194,8 +206,10 @@ def _check_decode(cache, table, q, lens, hq, hkv, d, scale=None):
     for b, n in enumerate(lens.tolist()):
         want, size = oracle.attention(q[b:b + 1, :hq * d], *cache, table[b, :-(-n // 64)].long(), [n], hq, hkv, d,
                                       d ** -0.5 if scale is None else scale)
+        x = cache.dequantize(table[b, :-(-n // 64)].long(), torch.float64)[:, 1].transpose(0, 1).reshape(hkv, -1, d)[:, :n]
+        least = 2.0 ** -36 * x.abs().sum(1).repeat_interleave(hq // hkv, 0).reshape(-1)
         err = (out[b].cpu().double() - want[0]).abs()
-        assert bool((err <= BF16 * want[0].abs() + 2.0 ** -10 * size[0]).all()), (b, n, float((err / (size[0] + 1e-300)).max()))
+        assert bool((err <= least + BF16 * want[0].abs() + 2.0 ** -10 * size[0]).all()), (b, n, float((err / (size[0] + 1e-300)).max()))
 
 
 HEADS = [(28, 4, 128), (14, 2, 64), (4, 4, 128), (32, 1, 128), (9, 1, 64), (24, 2, 128)]
@@ -223,6 +237,30 @@ def test_decode_attention_of_sharp_scores_and_unlike_scales(hq, hkv, d):
     cache.scales[table[0, 3].long(), 1] = 2.0 ** -126
     cache.scales[table[1, 0].long(), 0] = 2.0 ** -126
     _check_decode(cache, table, q, lens, hq, hkv, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64)])
+def test_decode_attention_of_many_small_weights_beside_a_large_one(hq, hkv, d):
+    """A first token that takes nearly all weight and has values near zero: the result is what thousands of tokens add, each with
+    less than a millionth of the largest weight."""
+    n = 6000
+    cache, table, q, lens = _decode([n], hq, hkv, d, 100)
+    cache.codes[:, 0] = (torch.randn(len(cache.codes), hkv, 64, d) * 30).to(torch.float8_e4m3fn)
+    cache.scales[:, 0] = 2.0 ** -9
+    q[0, :hq * d] = (0.1 * torch.randn(hq * d)).bfloat16()
+    sink = table[0, 0].long()
+    for h in range(hkv):
+        mean = q[0, :hq * d].float().view(hkv, hq // hkv, d)[h].mean(0)
+        cache.codes[sink, 0, h, 0] = (440 * torch.sign(mean)).to(torch.float8_e4m3fn)
+        cache.scales[sink, 0, h] = 2.0 ** -3
+        cache.codes[sink, 0, h, 1:] = 0
+    cache.codes[sink, 1, :, 0] = 0
+    want, _ = oracle.attention(q[:, :hq * d], *cache, table[0, :-(-n // 64)].long(), [n], hq, hkv, d, d ** -0.5)
+    x = cache.dequantize(table[0, :-(-n // 64)].long())
+    lead = torch.einsum("hrd,hd->hr", q[0, :hq * d].float().view(hkv, hq // hkv, d), x[0, 0, :, 0]) * d ** -0.5
+    assert float(lead.max()) > 14       # 2^-20 of the largest weight and less for the others
+    _check_decode(cache, table, q, lens, hq, hkv, d)
+    assert float(want.abs().max()) > 0
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (32, 2, 128)])
