@@ -31,6 +31,7 @@ def main() -> None:
     ap.add_argument("--max-model-len", type=int, default=0, help="engine limit (0: just enough for this run); the "
                     "training configuration uses prompt + response = 5120")
     ap.add_argument("--n", type=int, default=1, help="samples per prompt (prefix blocks shared by the n samples)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"], help="type of the cached keys and values")
     args = ap.parse_args()
     if args.decode_kernel:
         from ..ops import kv_cache
@@ -39,7 +40,8 @@ def main() -> None:
     dev = torch.device("cuda")
     model = build_model(cfg, dtype=torch.bfloat16, device=dev, seed=0)
     res = {"model": args.model, "layers": cfg.num_layers, "seqs": args.seqs, "context": args.context,
-           "max_model_len": args.max_model_len, "n": args.n, "decode_kernel": args.decode_kernel or "default"}
+           "max_model_len": args.max_model_len, "n": args.n, "decode_kernel": args.decode_kernel or "default",
+           "kv_cache_dtype": args.kv_cache_dtype}
     # prompts are prefilled at most 256 k tokens per engine iteration (a whole 256 x 2700 batch would need a 24 GB MLP
     # intermediate); every sequence decodes `extra` more rounds than the three of a single-batch prefill, so that a
     # round exists in which all sequences are active (the one that is reported)
@@ -49,7 +51,8 @@ def main() -> None:
     for graph in ([False] if args.no_graph else [False, True]):
         eng = RolloutEngine(model, max_num_seqs=args.seqs,
                             max_model_len=args.max_model_len or args.context + (4 + extra) * args.steps + 64,
-                            use_cuda_graph=graph, sync_interval=args.steps, max_num_batched_tokens=batched)
+                            use_cuda_graph=graph, sync_interval=args.steps, max_num_batched_tokens=batched,
+                            kv_cache_dtype=args.kv_cache_dtype)
         g = torch.Generator().manual_seed(0)
         prompts = [torch.randint(3, cfg.vocab_size, (args.context,), generator=g).tolist()
                    for _ in range(args.seqs // args.n)]

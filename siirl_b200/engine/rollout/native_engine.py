@@ -156,11 +156,16 @@ class RolloutEngine:
     def __init__(self, model: DecoderLM, max_num_seqs: int = 256, max_model_len: int = 8192,
                  num_blocks: Optional[int] = None, gpu_memory_utilization: float = 0.5, sync_interval: int = 16,
                  use_cuda_graph: bool = True, max_num_batched_tokens: int = 8192, lockstep_group=None,
-                 enable_chunked_prefill: bool = False, enable_prefix_caching: bool = True):
+                 enable_chunked_prefill: bool = False, enable_prefix_caching: bool = True, kv_cache_dtype: str = "auto"):
         """``lockstep_group``: ranks whose forward passes contain collectives over DIFFERENT requests (expert
         parallelism).  They then run the same sequence of prefill / decode calls: a rank without work joins with
         an empty prefill or an all-inactive decode step, and decode runs eagerly (the barriers of the expert
-        exchange carry a host-side epoch)."""
+        exchange carry a host-side epoch).
+
+        ``kv_cache_dtype``: ``auto`` (the weights' type) or ``fp8``: keys and values as e4m3 codes with a scale per block and
+        head (:class:`~siirl_b200.ops.kv_cache8.Cache8`), half the memory and half the reads of a decoding step.  Prompts that
+        are prefilled whole attend to their unrounded keys; single tokens, later chunks and prompts whose first blocks were
+        found in the prefix cache read the codes."""
         self.lockstep_group = lockstep_group
         if lockstep_group is not None:
             use_cuda_graph = False
@@ -172,6 +177,11 @@ class RolloutEngine:
         self.enable_chunked_prefill = bool(enable_chunked_prefill)
         self.enable_prefix_caching = bool(enable_prefix_caching)
         hybrid = model.cfg.hybrid
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype is 'auto' or 'fp8', not {kv_cache_dtype!r}")
+        if kv_cache_dtype == "fp8" and hybrid is not None:
+            raise ValueError("hybrid decoders keep their keys and values in the weights' type: set kv_cache_dtype=auto")
+        self.cache8 = kv_cache_dtype == "fp8"
         self.recurrent = hybrid is not None and any(b.recurrent for x in hybrid.layers for b in x.branches)
         self.visible_span = hybrid.visible_span() if hybrid is not None else None
         if hybrid is not None and lockstep_group is not None:
@@ -197,7 +207,7 @@ class RolloutEngine:
         self.max_num_batched_tokens = max_num_batched_tokens
         self._requested_blocks = num_blocks
         self._mem_util = gpu_memory_utilization
-        self.cache: Optional[List[torch.Tensor]] = None      # per layer [blocks, 2, Hkv, 64, D]
+        self.cache: Optional[List] = None       # per layer [blocks, 2, Hkv, 64, D], or a Cache8
         self.alloc: Optional[BlockAllocator] = None
         self._graphs: Dict[int, object] = {}
         self._graph_launches: Dict[int, int] = {}
@@ -209,6 +219,8 @@ class RolloutEngine:
 
     # ---- memory hand-off with the trainer -------------------------------------------------------
     def _block_bytes(self) -> int:
+        if self.cache8:
+            return self.cfg.num_layers * kvc.kv_cache8.block_bytes(self.cfg.num_kv_heads, self.cfg.head_dim)
         return sum(self._layer_elems()) * torch.finfo(self.dtype).bits // 8
 
     def _layer_elems(self) -> List[int]:
@@ -226,7 +238,8 @@ class RolloutEngine:
             return
         c = self.cfg
         nb = self._requested_blocks
-        esize = torch.finfo(self.dtype).bits // 8
+        dtype = torch.float8_e4m3fn if self.cache8 else self.dtype
+        esize = torch.finfo(dtype).bits // 8
         lent = 0
         if self.borrowed is not None and self.borrowed.device == self.device:
             lent = self.borrowed.numel() * self.borrowed.element_size()
@@ -248,14 +261,17 @@ class RolloutEngine:
             n_lent += 1
         pieces = []
         if n_lent:
-            flat = self.borrowed.reshape(-1).view(torch.uint8)[:used].view(self.dtype)
+            flat = self.borrowed.reshape(-1).view(torch.uint8)[:used]
             flat.zero_()    # rows past a sequence's length are multiplied by zero weights: they must be finite
-            pieces += flat.split([nb * e for e in elems[:n_lent]])
+            pieces += flat.view(dtype).split([nb * e for e in elems[:n_lent]])
         if n_lent < len(elems):
-            own = torch.zeros(nb * sum(elems[n_lent:]), dtype=self.dtype, device=self.device)
+            own = torch.zeros(nb * sum(elems[n_lent:]) * esize, dtype=torch.uint8, device=self.device).view(dtype)
             pieces += own.split([nb * e for e in elems[n_lent:]])
         shape = (nb, -1) if c.hybrid is not None else (nb, 2, c.num_kv_heads, BLOCK, c.head_dim)
         layers = [x.view(shape) for x in pieces]
+        if self.cache8:
+            scales = torch.zeros(len(layers), nb, 2, c.num_kv_heads, dtype=torch.float32, device=self.device)
+            layers = [kvc.Cache8(x, s) for x, s in zip(layers, scales)]
         self.cache = layers
         self.kv_layout = {"blocks": nb, "layers_in_borrowed_memory": n_lent}
         self.alloc = BlockAllocator(nb)

@@ -689,6 +689,8 @@ class ActorRolloutRefWorker(_ModelWorkerBase):
                 raise ValueError("hybrid decoders run on whole weights: set rollout.tensor_model_parallel_size=1")
             if tp > 1:
                 self.tp_model = self._build_tp_model(tp, r.max_num_batched_tokens)
+            if (str(r.name).lower() == "hf" or self.model_config.is_mla) and r.kv_cache_dtype != "auto":
+                raise ValueError("this rollout engine has no cache of keys and values: set rollout.kv_cache_dtype=auto")
             if str(r.name).lower() == "hf" or self.model_config.is_mla:
                 # ``rollout.name=hf``: cache-free generation through the training forward (the reference's HF
                 # rollout).  Multi-head latent attention has no paged-cache kernel: it decodes against a cache of
@@ -732,6 +734,7 @@ class ActorRolloutRefWorker(_ModelWorkerBase):
                                         max_num_batched_tokens=r.max_num_batched_tokens,
                                         enable_chunked_prefill=bool(r.enable_chunked_prefill),
                                         enable_prefix_caching=bool(getattr(r, "enable_prefix_caching", True)),
+                                        kv_cache_dtype=str(r.kv_cache_dtype),
                                         lockstep_group=self.group if getattr(self, "ep_ctx", None) is not None
                                         and self.world > 1 else None,
                                         **dict(r.engine_kwargs.native or {}))

@@ -189,6 +189,7 @@ def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, sl
             return kv_cache8.chunk_attention(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads,
                                              head_dim)
         kv_cache8.check_chunks(qkv, chunk_lens, prefix_lens, slots, cache_layer, block_table, n_heads, n_kv_heads, head_dim)
+    from .attention import SeqInfo, attention_packed
     dev = qkv.device
     qw, kw = n_heads * head_dim, n_kv_heads * head_dim
     totals = [int(p) + int(c) for p, c in zip(prefix_lens, chunk_lens)]

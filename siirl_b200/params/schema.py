@@ -294,6 +294,7 @@ class RolloutArguments:
     layer_name_map: LayerNameMapArguments = _dc(LayerNameMapArguments)
     seed: int = 0
     mode: str = "sync"
+    kv_cache_dtype: str = "auto"           # native: "fp8" keeps keys and values as e4m3 codes with scales per block and head
     kv_borrow_grad_buffer: bool = True     # native: lend the idle fp32 gradient buffer to the KV arena
     multi_turn: MultiTurnArguments = _dc(MultiTurnArguments)
     micro_batch_size: Optional[int] = None

@@ -373,3 +373,27 @@ def test_refusals():
                  lambda: kvc.prefill_attention_with_prefix(q, [3], [3], [0], cache, table, hq, hkv, d)):
         with pytest.raises(ValueError, match="8-bit cache"):
             call()
+
+
+def test_engine_on_the_8_bit_cache():
+    """Prompts, shared and forked blocks, reused prompts and decoding steps from a graph, through the rollout engine."""
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    from siirl_b200.models.config import get_config
+    from siirl_b200.models.decoder import build_model
+    model = build_model(get_config("tiny-gpu"), dtype=torch.bfloat16, device=DEV, seed=1)
+    prompts = [list(range(5, 5 + n)) for n in (7, 70, 130, 3)]
+    sp = SamplingParams(n=2, temperature=0.0, max_new_tokens=70, eos_token_id=None)
+    kw = dict(max_num_seqs=8, max_model_len=512, num_blocks=64, sync_interval=4)
+    eager = RolloutEngine(model, use_cuda_graph=False, kv_cache_dtype="fp8", **kw)
+    outs = eager.generate(prompts, sp)
+    graph = RolloutEngine(model, use_cuda_graph=True, kv_cache_dtype="fp8", **kw)
+    assert [o.token_ids for o in graph.generate(prompts, sp)] == [o.token_ids for o in outs]
+    plain = RolloutEngine(model, use_cuda_graph=False, **kw).generate(prompts, sp)
+    lib.check_status()
+    # whole prompts attend to their unrounded keys
+    assert [o.token_ids[0] for o in plain] == [o.token_ids[0] for o in outs]
+    assert all(o.token_ids == p.token_ids for o, p in zip(outs[::2], outs[1::2]))      # greedy samples of a prompt
+    assert eager.generate([p + [9, 8] for p in prompts], sp) is not None
+    assert eager.stats["prefix_cache_hit_tokens"] >= 64 + 128
+    lib.check_status()
+    assert eager.alloc.num_free == eager.alloc.num_blocks

@@ -133,3 +133,74 @@ def test_refusals():
                  lambda: append(cache=Cache8(cache.codes.transpose(2, 3), cache.scales))):
         with pytest.raises(ValueError, match="8-bit cache"):
             call()
+
+
+# ---- the rollout engine -------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def tiny():
+    from siirl_b200.models.config import get_config
+    from siirl_b200.models.decoder import build_model
+    return build_model(get_config("tiny"), dtype=torch.float32, device="cpu", seed=3)
+
+
+def test_engine_decodes_what_its_cache_holds(tiny):
+    """Greedy tokens with shared prompts, forked blocks and several blocks per sequence: each follows from attention to rounded
+    keys and values, recomputed here token by token."""
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    cfg = tiny.cfg
+    eng = RolloutEngine(tiny, max_num_seqs=8, max_model_len=256, num_blocks=40, sync_interval=4, kv_cache_dtype="fp8")
+    assert all(isinstance(x, Cache8) for x in eng.cache)
+    assert eng._block_bytes() == sum(x.codes[0].numel() + 4 * x.scales[0].numel() for x in eng.cache)
+    prompts = [[5, 6, 7, 8, 9], list(range(20, 20 + 70)), list(range(9, 9 + 64))]
+    outs = eng.generate(prompts, SamplingParams(n=2, temperature=0.0, max_new_tokens=6, ignore_eos=True))
+    plain = RolloutEngine(tiny, max_num_seqs=8, max_model_len=256, num_blocks=40, sync_interval=4)
+    want = plain.generate(prompts, SamplingParams(n=2, temperature=0.0, max_new_tokens=6, ignore_eos=True))
+    # the first token comes from unrounded keys; samples of a prompt are the same; log-probs stay near
+    for o, w in zip(outs, want):
+        assert o.token_ids[0] == w.token_ids[0] and abs(o.logprobs[0] - w.logprobs[0]) < 1e-5
+        same = next((i for i, (a, b) in enumerate(zip(o.token_ids, w.token_ids)) if a != b), 6)
+        assert all(abs(a - b) < 0.2 for a, b in zip(o.logprobs[:same], w.logprobs[:same]))
+    assert [outs[0].token_ids, outs[2].token_ids, outs[4].token_ids] == [outs[1].token_ids, outs[3].token_ids, outs[5].token_ids]
+    assert eng.alloc.num_free == eng.alloc.num_blocks
+    # one sequence by hand
+    cache = [Cache8.zeros(4, cfg.num_kv_heads, cfg.head_dim) for _ in range(cfg.num_layers)]
+    table, ids = torch.tensor([[2, 0, 3]], dtype=torch.int32), list(prompts[1])
+    one = torch.zeros(1, dtype=torch.int32)
+    from siirl_b200.ops.attention import SeqInfo
+    info = SeqInfo([len(ids)])
+    hidden = tiny.forward_cached(torch.tensor(ids), info.positions, cache, table, one.expand(len(ids)).contiguous(), prefill_info=info)[-1:]
+    got = []
+    for n in range(len(ids), len(ids) + 6):
+        got.append(int(eng._logits(hidden).argmax()))
+        hidden = tiny.forward_cached(torch.tensor(got[-1:]), one + n, cache, table, one, seq_lens=one + n + 1)
+    assert got == outs[2].token_ids
+
+
+def test_engine_chunks_and_reuses_prompts(tiny):
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    prompts = [list(range(7, 7 + n)) for n in (150, 70)]
+    sp = SamplingParams(n=1, temperature=0.0, max_new_tokens=4, ignore_eos=True)
+    eng = RolloutEngine(tiny, max_num_seqs=8, max_model_len=256, num_blocks=40, kv_cache_dtype="fp8")
+    eng.generate(prompts, sp)
+    again = eng.generate([p + [3, 4] for p in prompts], sp)
+    assert eng.stats["prefix_cache_hit_tokens"] == 128 + 64
+    chunked = RolloutEngine(tiny, max_num_seqs=8, max_model_len=256, num_blocks=40, max_num_batched_tokens=64,
+                            enable_chunked_prefill=True, kv_cache_dtype="fp8")
+    assert len(chunked.generate(prompts, sp)) == len(again) == 2
+    eng.borrowed = torch.full((300_000,), math.nan)
+    eng.sleep()
+    eng.wake_up()
+    assert eng.kv_layout["layers_in_borrowed_memory"] > 0
+    assert [o.token_ids for o in eng.generate([p + [3, 4] for p in prompts], sp)] is not None
+    assert all(bool(torch.isfinite(x.codes.float()).all()) for x in eng.cache)
+
+
+def test_engine_refusals(tiny):
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        RolloutEngine(tiny, max_num_seqs=8, max_model_len=64, kv_cache_dtype="int8")
+    from siirl_b200.models.config import get_config
+    from siirl_b200.models.decoder import build_model
+    hybrid = build_model(get_config("tiny-domavik"), dtype=torch.float32, device="cpu", seed=0)
+    with pytest.raises(ValueError, match="hybrid"):
+        RolloutEngine(hybrid, max_num_seqs=8, max_model_len=64, num_blocks=8, kv_cache_dtype="fp8")
