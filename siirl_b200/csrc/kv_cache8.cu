@@ -300,17 +300,33 @@ __global__ void __launch_bounds__(256) append8_rows_kernel(Append8Params p, int 
 // while the block finds the largest value, so that rows are read once.  The other blocks rotate q heads: a thread
 // keeps the eight angles of its pairs for `per` heads.
 //
-// Bound by memory: 28 / 4 heads, D = 128, 8992 rows of 24 prompts (170 MB): 48 us; 32 / 8 heads, 32653 rows (819 MB): 177 us,
-// 4.6 TB/s.
+// Bound by memory: 32 / 8 heads, D = 128, 32653 rows (819 MB): 145 us, 5.6 TB/s (with rows held in registers instead of asked for
+// four heads ahead, 177); 28 / 4 heads, 8992 rows of 24 prompts (170 MB): 38 us.
 // ---------------------------------------------------------------------------------------
 
-// Eight pairs from element i0 on of one head of a row, as they are asked for: bf16 numbers, or (SLABS) the sum of the partial
-// sums and the bias; not rotated
+// Eight pairs from element i0 on of one head of a row, not rotated.  bf16 rows are asked for several heads ahead: a thread's
+// own places in shared memory take what would need registers, and nobody else reads them.  Partial sums (SLABS) are added up
+// when they are needed.
+constexpr int kAheadHeads = 4;
 template <int D, bool SLABS>
 struct Pairs {
-  uint4 a, b;
-  float x[SLABS ? 8 : 1], y[SLABS ? 8 : 1];
-  __device__ __forceinline__ void load(const Append8Params& p, int r, int head, int i0) {
+  static constexpr int kThreads = 4 * D;
+  static constexpr int kBytes = SLABS ? 0 : kAheadHeads * 2 * kThreads * 16;
+  uint4* own;      // [kAheadHeads][2][threads], from this thread's place on
+  __device__ __forceinline__ void ask(const Append8Params& p, int slot, bool any, int r, int head, int i0) const {
+    if constexpr (!SLABS) {
+      if (any) {
+        const __nv_bfloat16* src = p.qkv + (size_t)r * p.row_stride + (size_t)head * D + i0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(own + (slot * 2 + half) * kThreads)), "l"(src + half * (D / 2))
+                       : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  // what was asked for kAheadHeads calls of ask() ago, or before
+  __device__ __forceinline__ void get(const Append8Params& p, int slot, int r, int head, int i0, float (&x)[8], float (&y)[8]) const {
     if constexpr (SLABS) {
       const float* src = p.slabs + ((size_t)r * (p.Hq + 2 * p.Hkv) + head) * D + i0;
       slab_sum8(src, p.slab_stride, p.splits, x);
@@ -324,24 +340,13 @@ struct Pairs {
         }
       }
     } else {
-      const __nv_bfloat16* src = p.qkv + (size_t)r * p.row_stride + (size_t)head * D + i0;
-      a = *reinterpret_cast<const uint4*>(src);
-      b = *reinterpret_cast<const uint4*>(src + D / 2);
-    }
-  }
-  __device__ __forceinline__ void get(float (&u)[8], float (&v)[8]) const {
-    if constexpr (SLABS) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        u[k] = x[k];
-        v[k] = y[k];
-      }
-    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAheadHeads - 1) : "memory");
+      const uint4 a = own[slot * 2 * kThreads], b = own[(slot * 2 + 1) * kThreads];
       const uint32_t c[4] = {a.x, a.y, a.z, a.w}, d[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        u[2 * k] = __uint_as_float(c[k] << 16); u[2 * k + 1] = __uint_as_float(c[k] & 0xffff0000u);
-        v[2 * k] = __uint_as_float(d[k] << 16); v[2 * k + 1] = __uint_as_float(d[k] & 0xffff0000u);
+        x[2 * k] = __uint_as_float(c[k] << 16); x[2 * k + 1] = __uint_as_float(c[k] & 0xffff0000u);
+        y[2 * k] = __uint_as_float(d[k] << 16); y[2 * k + 1] = __uint_as_float(d[k] & 0xffff0000u);
       }
     }
   }
@@ -393,7 +398,9 @@ __global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_ker
   __shared__ uint32_t s_begin[5], s_top[2][D / 8];
   constexpr int TPR = D / 16;             // threads of a row, eight pairs each
   chain_sync();
+  extern __shared__ uint4 s_ahead[];
   const int tid = threadIdx.x, q = tid % TPR, i0 = q * 8;
+  const Pairs<D, SLABS> pairs{s_ahead + tid};
   // blocks of the two kinds take turns, so that the ones that wait and the ones that stream share the SMs
   const int i_kv = (int)((long long)blockIdx.x * kv_blocks / gridDim.x);
   if ((int)((long long)(blockIdx.x + 1) * kv_blocks / gridDim.x) == i_kv) {
@@ -402,14 +409,15 @@ __global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_ker
     const int r = b / parts * 64 + tid / TPR, h0 = b % parts * per_q;
     if (r >= p.T) return;
     float c[8], s[8];
+    const int h1 = min(h0 + per_q, p.Hq);
+    for (int k = 0; k < kAheadHeads; ++k) pairs.ask(p, k, h0 + k < h1, r, h0 + k, i0);
     if (p.rope_pos) load_angles<D>(p, r, i0, c, s);
-#pragma unroll 2
-    for (int h = h0; h < min(h0 + per_q, p.Hq); ++h) {
-      Pairs<D, SLABS> pairs;
-      pairs.load(p, r, h, i0);
+    for (int h = h0; h < h1; ++h) {
+      const int slot = (h - h0) % kAheadHeads;
       float x[8], y[8];
-      pairs.get(x, y);
+      pairs.get(p, slot, r, h, i0, x, y);
       if (p.rope_pos) turn_pairs(x, y, c, s);
+      pairs.ask(p, slot, h + kAheadHeads < h1, r, h + kAheadHeads, i0);
       store_pairs<D>(p, r, h, i0, x, y);
     }
     return;
@@ -469,12 +477,11 @@ __global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_ker
     const int row = tid / TPR, r = t + row;
     const bool mine = row < n;
     const size_t at0 = ((size_t)blk * 2 + kv) * p.Hkv;
-    Pairs<D, SLABS> ahead;
     float c[8], s[8], before = p.scales[at0 + g0];
     int off = 0;
+    for (int k = 0; k < kAheadHeads; ++k) pairs.ask(p, k, mine && g0 + k < g1, r, head0 + g0 + k, i0);      // all: per_kv is at most that
     if (mine) {
       off = p.cache_pos[r] % kB8;
-      ahead.load(p, r, head0 + g0, i0);
       if (turns) load_angles<D>(p, r, i0, c, s);
     }
     __syncthreads();      // the run before has been done
@@ -484,7 +491,7 @@ __global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_ker
     for (int g = g0; g < g1; ++g) {
       float x[8], y[8], amax = 0.f;
       if (mine) {
-        ahead.get(x, y);
+        pairs.get(p, g - g0, r, head0 + g, i0, x, y);
         if (turns) turn_pairs(x, y, c, s);
 #pragma unroll
         for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fmaxf(finite_abs(x[k]), finite_abs(y[k])));
@@ -492,11 +499,9 @@ __global__ void __launch_bounds__(4 * D, SLABS ? 1 : 1024 / (4 * D)) append8_ker
       // of numbers >= 0, bits order as they do
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
       if ((tid & 31) == 0) s_top[g & 1][tid >> 5] = top;
+      pairs.ask(p, 0, false, 0, 0, 0);      // counts as a turn
       const float now = before;
-      if (g + 1 < g1) {      // the next head's, while this one's largest value is found
-        before = p.scales[at0 + g + 1];
-        if (mine) ahead.load(p, r, head0 + g + 1, i0);
-      }
+      if (g + 1 < g1) before = p.scales[at0 + g + 1];      // while this one's largest value is found
       __syncthreads();
       uint32_t all = 0;
 #pragma unroll
@@ -569,18 +574,23 @@ extern "C" int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long
     if (kv + q > 0x7fffffffll) return -4;
     return launch_chained(D == 128 ? append8_rows_kernel<128> : append8_rows_kernel<64>, (unsigned)(kv + q), 256, 0, stream, p, (int)kv);
   }
-  // several heads for what a block finds out about its rows, as long as every SM gets blocks
+  // Several heads for what a block finds out about its rows, as long as every SM gets two blocks (8992 rows, 28 / 4 heads: 38 us; four
+  // blocks: 43)
   const int ranges = (T + kB8 - 1) / kB8;
   auto blocks_of = [](long long n, int heads, int per) { return n * ((heads + per - 1) / per); };
-  int per_kv = 4, per_q = 8;
-  while (per_kv > 1 && blocks_of(2 * ranges, Hkv, per_kv) < 4 * num_sms()) per_kv /= 2;
-  while (per_q > 1 && blocks_of(ranges, Hq, per_q) < 4 * num_sms()) per_q /= 2;
+  int per_kv = kAheadHeads, per_q = 16;
+  while (per_kv > 1 && blocks_of(2 * ranges, Hkv, per_kv) < 2 * num_sms()) per_kv /= 2;
+  while (per_q > 1 && blocks_of(ranges, Hq, per_q) < 2 * num_sms()) per_q /= 2;
   const long long kv = blocks_of(2 * ranges, Hkv, per_kv);
   const long long q = rope_pos || slabs ? blocks_of(ranges, Hq, per_q) : 0;
   if (kv + q > 0x7fffffffll) return -4;
-  auto kernel = D == 128 ? (slabs ? append8_kernel<128, true> : append8_kernel<128, false>)
-                         : (slabs ? append8_kernel<64, true> : append8_kernel<64, false>);
-  return launch_chained(kernel, (unsigned)(kv + q), 4 * D, 0, stream, p, (int)kv, per_kv, per_q);
+  auto launch = [&](auto kernel, int bytes) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+    return launch_chained(kernel, (unsigned)(kv + q), 4 * D, bytes, stream, p, (int)kv, per_kv, per_q);
+  };
+  if (slabs) return D == 128 ? launch(append8_kernel<128, true>, 0) : launch(append8_kernel<64, true>, 0);
+  return D == 128 ? launch(append8_kernel<128, false>, Pairs<128, false>::kBytes) : launch(append8_kernel<64, false>, Pairs<64, false>::kBytes);
 }
 
 extern "C" int sb_kv8_copy_blocks(void* codes, float* scales, const int* src, const int* dst, int n_pairs, int num_blocks,

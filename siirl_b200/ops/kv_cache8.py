@@ -12,6 +12,7 @@ rounded to it.  A row at offset 0 of a block starts it anew: rows that the call 
 that lie in the same block have to follow one another; where one place is named twice, its last row counts."""
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import math
@@ -286,11 +287,17 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     """:func:`siirl_b200.ops.kv_cache.prefill_attention_with_prefix` on an 8-bit cache, on the GPU.  The visible keys and values
     are unpacked to bf16 once per call: ``4 * Hkv * D`` bytes for every token up to the next multiple of 128, beside the
     output."""
-    chunk_lens, prefix_lens, slots = ([int(x) for x in v] for v in (chunk_lens, prefix_lens, slots))
-    check_chunks(qkv, chunk_lens, prefix_lens, slots, cache, block_table, n_heads, n_kv_heads, head_dim)
-    rows = qkv.shape[0]
+    _check(cache, n_heads, n_kv_heads, head_dim, qkv)
+    _check_ints(qkv, block_table)
+    rows, width = qkv.shape
+    lists = [array.array("i", v) for v in (chunk_lens, prefix_lens, slots)]
+    total = len(lists[0])
+    if width != (n_heads + 2 * n_kv_heads) * head_dim or qkv.dtype is not torch.bfloat16 or block_table.dim() != 2 or \
+            total != len(lists[1]) or total != len(lists[2]):
+        check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
+    held, max_blocks = block_table.shape
     out = torch.empty(rows, n_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
-    if rows == 0:
+    if rows == 0 and not any(lists[0]):
         return out
     stride, one = qkv.stride()
     if one != 1 or stride % 8 or qkv.data_ptr() % 16:
@@ -299,19 +306,21 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     L = _lib.get_lib()
     with _device(qkv.get_device()):
         most, at = L.sb_kv8_chunk_seqs(), 0
-        for i in range(0, len(slots), most):
-            ints = ctypes.c_int * len(slots[i:i + most])
-            lists = [ints(*v[i:i + most]) for v in (chunk_lens, prefix_lens, slots)]
-            n = len(lists[0])
-            sizes = (ctypes.c_longlong * 2)()
-            _lib.check(L.sb_kv8_chunk_sizes(*lists, n, n_heads, n_kv_heads, head_dim, sizes), "sb_kv8_chunk_sizes")
+        sizes = array.array("q", (0, 0, 0))
+        for i in range(0, total, most):
+            n = min(most, total - i)
+            places = [v.buffer_info()[0] + 4 * i for v in lists]
+            rc = L.sb_kv8_chunk_sizes(*places, n, n_heads, n_kv_heads, head_dim, rows - at, held, max_blocks, sizes.buffer_info()[0])
+            if rc == -5 or i + n == total and at + sizes[2] != rows:
+                check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
+            _lib.check(rc, "sb_kv8_chunk_sizes")
             # buffers of the call's own, as for single tokens
             ws = torch.empty(2 * sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=qkv.device)
             _lib.check(L.sb_kv8_chunks(
                 qkv.data_ptr() + 2 * at * stride, stride, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.codes.shape[0],
-                block_table.data_ptr(), block_table.shape[1], *lists, n, ws.data_ptr(), ws.data_ptr() + 2 * sizes[0],
+                block_table.data_ptr(), max_blocks, *places, n, ws.data_ptr(), ws.data_ptr() + 2 * sizes[0],
                 out.data_ptr() + 2 * at * out.shape[1], n_heads, n_kv_heads, head_dim, 1.0 / math.sqrt(head_dim),
                 _lib.status_word(qkv.device).data_ptr(), _lib.stream()), "sb_kv8_chunks")
             _lib.add_launches(int(sizes[1] > 0))        # shares of the keys are joined
-            at += sum(lists[0])
+            at += sizes[2]
     return out

@@ -33,7 +33,7 @@ _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_
 # then passed as plain numbers, which saves an object for each.
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
-              "sb_kv8_chunk_sizes": "pppiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
+              "sb_kv8_chunk_sizes": "pppiiiiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
 
 
 class _CountingLib:
