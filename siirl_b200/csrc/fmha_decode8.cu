@@ -17,9 +17,10 @@
 // only the diagonal (token of the row) blocks of O^T mean something; the query terms of the other token's half are zeros.
 //
 // The tiles of all (sequence, kv head, group of at most NR query heads) form one list, and every CTA of a persistent grid of
-// one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry; a piece that is not
-// the whole entry leaves a normalised partial result and its log-sum-exp in a workspace, two slots per CTA, and a small
-// kernel merges them.  The warps:
+// one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry.  A piece that is not
+// the whole entry leaves a normalised result and its log-sum-exp in a workspace, two slots per CTA, and counts itself; whoever
+// finds that all others have joins them.  A second kernel for that would cost the host as much again as this one.
+// The warps:
 //   0..7   soft-max in two groups, each with an O^T and weights' references of its own.  D = 128: thread = row of the tile, the
 //          first four warps take the even tiles of the range, the others the odd ones, so that two tiles are under way.
 //          D = 64: the groups take the first and the second tokens of every tile's rows.  A vote of the group per tile says
@@ -117,8 +118,8 @@ struct Decode8Params {
   int num_blocks, max_blocks, B, Hq, Hkv, groups;
   __nv_bfloat16* out;       // [B, Hq * D]
   float* ws_o;              // [2 * grid][NR][D]
-  float* ws_lse;            // [2 * grid][NR]
-  int* ws_pre;              // [B + 1] tiles before each sequence, written by the first CTA
+  float* ws_lse;            // [2 * grid][4][NR]: each output warp's own
+  int* counts;              // [B * entries][4] pieces that have been left, zeros before and after
   float scale_log2;
   int* status;
 };
@@ -206,6 +207,61 @@ __device__ __noinline__ float d8_dot(const __nv_bfloat16* q, const uint8_t* k, i
 #pragma unroll 1
   for (int d = 0; d < D; ++d) s = fmaf(__bfloat162float(q[d]), from_e4m3x2(k[(((d >> 4) ^ (r & 7)) << 4) + (d & 15)]).x, s);
   return s;
+}
+
+// A warp has left its columns of one of the pieces of an entry, which CTAs c0 .. c1 have (c0 in its slot `own`).  If it is the last
+// one: mean of all, weighted by 2^(log-sum-exp), to the output.  `parts` and `lses` point at the lane's column and the warp's
+// sums of slot 0.
+template <int D, int NR>
+__device__ __noinline__ void d8_join(const float* parts, const float* lses, int* count, int c0, int c1, int own, int heads,
+                                     __nv_bfloat16* orow) {
+  __threadfence();      // what this lane has written, before the warp counts
+  __syncwarp();
+  int before = 0;
+  const bool one = (threadIdx.x & 31) == 0;
+  if (one) before = atomicAdd(count, 1);
+  if (__shfl_sync(0xffffffffu, before, 0) != c1 - c0) return;
+  __threadfence();
+  if (one) *count = 0;
+  constexpr int U = 16 / NR;      // pieces whose reads are under way together
+  float top[NR], sum[NR], acc[NR];
+#pragma unroll
+  for (int h = 0; h < NR; ++h) {
+    top[h] = -INFINITY;
+    sum[h] = acc[h] = 0.f;
+  }
+#pragma unroll 1
+  for (int c = c0; c <= c1; c += U) {
+    float o[U][NR], lse[U][NR];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t slot = 2 * min(c + u, c1) + (c + u == c0 ? own : 0);
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        o[u][h] = h < heads ? __ldcg(parts + (slot * NR + h) * D) : 0.f;
+        lse[u][h] = c + u <= c1 ? __ldcg(lses + slot * 4 * NR + h) : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < NR; ++h) {
+      float now = top[h];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now = fmaxf(now, lse[u][h]);
+      const float f = top[h] == -INFINITY ? 0.f : fast_exp2(top[h] - now);
+      sum[h] *= f;
+      acc[h] *= f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = lse[u][h] == -INFINITY ? 0.f : fast_exp2(lse[u][h] - now);
+        sum[h] += e;
+        acc[h] += e == 0.f ? 0.f : e * o[u][h];
+      }
+      top[h] = now;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < NR; ++h)
+    if (h < heads) orow[h * D] = __float2bfloat16(sum[h] == 0.f ? 0.f : acc[h] / sum[h]);
 }
 
 constexpr int kQ8Threads = 16 * 32;
@@ -312,8 +368,6 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   }
   const int total = s_pre[p.B] * entries, ranges = d8_ranges(total, gridDim.x);
   const int begin = d8_begin(total, blockIdx.x, ranges), end = d8_begin(total, blockIdx.x + 1, ranges);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= p.B; i += kQ8Threads) p.ws_pre[i] = s_pre[i];
 
   if (warp == 12) {
     // ------------------------------ producer ------------------------------
@@ -861,7 +915,14 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
             if (whole) orow[h * D] = __float2bfloat16(o[h]);
             else wrow[h * D] = o[h];
           }
-        if (!whole && quarter == 0 && lane < NR) p.ws_lse[(size_t)slot * NR + lane] = lse;
+        if (!whole) {
+          if (lane < NR) p.ws_lse[((size_t)slot * 4 + quarter) * NR + lane] = lse;
+          // the range that holds position x is the last one that begins at or before it
+          const int first = s_pre[q.row] * entries + q.entry * q.tiles;
+          const int c0 = (int)(((long long)(first + 1) * ranges - 1) / total), c1 = (int)(((long long)(first + q.tiles) * ranges - 1) / total);
+          d8_join<D, NR>(p.ws_o + d, p.ws_lse + quarter * NR, p.counts + ((size_t)q.row * entries + q.entry) * 4 + quarter, c0, c1,
+                         d8_begin(total, c0, ranges) >= first ? 0 : 1, left, orow);
+        }
       }
       cur += q.n;
     }
@@ -871,39 +932,6 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   if (warp == 13) {
     tc_fence_after();
     tmem_dealloc(tmem_base, L::kTmemCols);
-  }
-}
-
-// entries whose tiles are spread over several ranges: mean of the partial results, weighted by 2^(log-sum-exp)
-template <int D, int NR>
-__global__ void __launch_bounds__(128) fmha_decode8_merge_kernel(Decode8Params p, int grid) {
-  chain_sync();
-  const int entries = p.Hkv * p.groups, b = blockIdx.x, entry = blockIdx.y;
-  const int total = p.ws_pre[p.B] * entries, before = p.ws_pre[b], tiles = p.ws_pre[b + 1] - before;
-  if (tiles == 0) return;
-  const int ranges = d8_ranges(total, grid);
-  const int first = before * entries + entry * tiles;
-  // the range that holds position x is the last one that begins at or before it
-  const int c0 = (int)(((long long)(first + 1) * ranges - 1) / total), c1 = (int)(((long long)(first + tiles) * ranges - 1) / total);
-  if (c0 == c1) return;
-  const int rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups, group = entry % p.groups;
-  const int left = min(per_group, rep - group * per_group), head0 = entry / p.groups * rep + group * per_group;
-  for (int i = threadIdx.x * 4; i < left * D; i += 128 * 4) {
-    const int h = i / D;
-    float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = c0; c <= c1; ++c) {
-      const int slot = 2 * c + (d8_begin(total, c, ranges) >= first ? 0 : 1);
-      const float lse = p.ws_lse[(size_t)slot * NR + h];
-      const float4 o = *reinterpret_cast<const float4*>(p.ws_o + (size_t)slot * NR * D + i);
-      const float now = fmaxf(top, lse);
-      const float f = now == -INFINITY ? 0.f : exp2f(top - now), w = lse == -INFINITY ? 0.f : exp2f(lse - now);
-      sum = sum * f + w;
-      acc[0] = acc[0] * f + w * o.x; acc[1] = acc[1] * f + w * o.y; acc[2] = acc[2] * f + w * o.z; acc[3] = acc[3] * f + w * o.w;
-      top = now;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.Hq + head0) * D + i) =
-        make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   }
 }
 
@@ -920,9 +948,7 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
     if (e != cudaSuccess) return (int)e;
     configured = dev;
   }
-  const int rc = launch_chained(kernel, (unsigned)grid, kQ8Threads, L::kTotal, stream, mc, p);
-  if (rc || p.max_blocks <= L::BPT) return rc;      // one tile per entry: nothing is split
-  return launch_chained(fmha_decode8_merge_kernel<D, NR>, dim3(p.B, p.Hkv * p.groups), 128, 0, stream, p, grid);
+  return launch_chained(kernel, (unsigned)grid, kQ8Threads, L::kTotal, stream, mc, p);
 }
 
 }  // namespace sb
@@ -930,14 +956,23 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
 using namespace sb;
 
 // Workspaces: with rows = 8 where at most 8 query heads share a kv head or D = 64, else 16, ws_o has 2 * grid * rows * D floats,
-// ws_lse 2 * grid * rows, ws_pre B + 1 ints.
+// ws_lse 8 * grid * rows; counts B * Hkv * ceil(Hq / Hkv / rows) * 4 ints, which are zeros and stay zeros after every call, but one
+// whose waits ran out.
+// Number of the capture that `stream` takes part in, 0 outside of one
+extern "C" unsigned long long sb_capture_id(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) cudaGetLastError();
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" int sb_kv8_decode_grid() { return num_sms(); }
 
 // One query row per sequence (at most 1024) against its cached context of seq_lens[b] tokens, the current one included; 0: idle
 // slot, its output row is zero.  Rows start on 4-byte boundaries.
 extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const float* scales, int num_blocks,
                              const int* seq_lens, const int* block_table, int max_blocks, void* out, float* ws_o,
-                             float* ws_lse, int* ws_pre, int B, int Hq, int Hkv, int D, float scale, int* status,
+                             float* ws_lse, int* counts, int B, int Hq, int Hkv, int D, float scale, int* status,
                              cudaStream_t stream) {
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
@@ -958,7 +993,7 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   p.block_table = block_table; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
   const int most = Hq / Hkv <= 8 || D == 64 ? 8 : 16;
   p.groups = (Hq / Hkv + most - 1) / most;
-  p.out = (__nv_bfloat16*)out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.ws_pre = ws_pre;
+  p.out = (__nv_bfloat16*)out; p.ws_o = ws_o; p.ws_lse = ws_lse; p.counts = counts;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   const int grid = num_sms();
   if (D == 64) return launch_decode8<64, 8>(mc, p, grid, stream);

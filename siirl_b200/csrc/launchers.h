@@ -151,10 +151,11 @@ int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long long slab_
 int sb_kv8_copy_blocks(void* codes, float* scales, const int* src, const int* dst, int n_pairs, int num_blocks,
                        int per_block, long long bytes, cudaStream_t stream);
 // ---- fmha_decode8.cu ----
+unsigned long long sb_capture_id(cudaStream_t stream);
 int sb_kv8_decode_grid();
 int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const float* scales, int num_blocks,
                   const int* seq_lens, const int* block_table, int max_blocks, void* out, float* ws_o, float* ws_lse,
-                  int* ws_pre, int B, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream);
+                  int* counts, int B, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream);
 // ---- fmha_chunk8.cu ----
 int sb_kv8_chunk_seqs();
 int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D, int rows, int slots,

@@ -241,24 +241,47 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
         _refuse("query rows are bf16")
     if q_rows.stride(0) % 2 or q_rows.data_ptr() % 4:
         q_rows = q_rows[:, :width].contiguous()
+    dev = q_rows.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return decode_attention(q_rows, cache, seq_lens, block_table, n_heads, n_kv_heads, head_dim, scale, out)
     L = _lib.get_lib()
     codes, scales = cache
     stride, max_blocks = q_rows.stride(0), block_table.shape[1]
-    with _device(q_rows.get_device()):
-        part = 2 * L.sb_kv8_decode_grid() * (8 if n_heads <= 8 * n_kv_heads or head_dim == 64 else 16)
-        for at in range(0, B, ROWS):
-            n = min(ROWS, B - at)
-            # two partial results per block of the grid, and the sequences' places in the list of tiles.  A buffer of the
-            # call's own: calls on other streams and graphs that hold one write to theirs
-            ws = torch.empty(part * (head_dim + 1) + n + 1, dtype=torch.float32, device=q_rows.device)
-            o = ws.data_ptr()
-            _lib.check(L.sb_kv8_decode(
-                q_rows.data_ptr() + 2 * at * stride, stride, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
-                seq_lens.data_ptr() + 4 * at, block_table.data_ptr() + 4 * at * max_blocks, max_blocks,
-                out.data_ptr() + 2 * at * width, o, o + 4 * part * head_dim, o + 4 * part * (head_dim + 1), n, n_heads,
-                n_kv_heads, head_dim, scale, _lib.status_word(q_rows.device).data_ptr(), _lib.stream()), "sb_kv8_decode")
-            _lib.add_launches(int(max_blocks > 2 * 128 // head_dim))      # ranges' shares are merged
+    rows = 8 if n_heads <= 8 * n_kv_heads or head_dim == 64 else 16
+    part = 2 * L.sb_kv8_decode_grid() * rows        # rows of partial results: two for each block of the grid
+    entries = n_kv_heads * -(-(n_heads // n_kv_heads) // rows)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    floats, counts = _decode_workspace(dev, stream, part * (head_dim + 4), 4 * min(B, ROWS) * entries)
+    for at in range(0, B, ROWS):
+        n = min(ROWS, B - at)
+        _lib.check(L.sb_kv8_decode(
+            q_rows.data_ptr() + 2 * at * stride, stride, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+            seq_lens.data_ptr() + 4 * at, block_table.data_ptr() + 4 * at * max_blocks, max_blocks,
+            out.data_ptr() + 2 * at * width, floats.data_ptr(), floats.data_ptr() + 4 * part * head_dim, counts.data_ptr(), n,
+            n_heads, n_kv_heads, head_dim, scale, _lib.status_word(q_rows.device).data_ptr(), stream), "sb_kv8_decode")
     return out
+
+
+# Partial results, and counters of pieces, which every call leaves as zeros: of each stream, whose calls come one after the other,
+# and of each stream of a capture, since a graph may be replayed beside anything.  A capture's are kept until the stream's next one,
+# so that nothing else in the graph gets their memory, and its first call clears the counters in every replay.
+_decode_buffers: dict = {}
+
+
+def _decode_workspace(dev: int, stream: int, floats: int, counts: int):
+    capture = _lib.get_lib().sb_capture_id(stream)
+    held = _decode_buffers.get((dev, stream, capture != 0))
+    if held is None or held[2] != capture or held[0].numel() < floats or held[1].numel() < counts:
+        more = (0, 0) if held is None or held[2] != capture else (held[0].numel(), held[1].numel())
+        held = (torch.empty(max(floats, more[0]), dtype=torch.float32, device=f"cuda:{dev}"),
+                torch.zeros(max(counts, more[1]), dtype=torch.int32, device=f"cuda:{dev}"), capture)
+        _decode_buffers[dev, stream, capture != 0] = held
+    return held[:2]
+
+
+# a kernel that gave up a wait may have left counters behind
+_lib.on_status_error(_decode_buffers.clear)
 
 
 # ---- chunks of prompts --------------------------------------------------------------------------

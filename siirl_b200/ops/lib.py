@@ -24,7 +24,7 @@ _status_words: dict[int, torch.Tensor] = {}
 _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_rows": 0, "sb_ppo_token_loss": 2,
                      "sb_fmha_bwd": 3, "sb_kk_partition": 0, "sb_rmsnorm_bwd_blocks": 0, "sb_colsum_blocks": 0,
                      "sb_colsum_bf16": 2, "sb_gemm_set_pair_kernel": 0, "sb_fmha_decode_chunk_tiles": 0,
-                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_kv8_chunk_seqs": 0, "sb_kv8_chunk_sizes": 0,
+                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_capture_id": 0, "sb_kv8_chunk_seqs": 0, "sb_kv8_chunk_sizes": 0,
                      "sb_kv8_chunks": 2, "sb_recurrence_prefill": 2, "sb_attn_window_decode": 2, "sb_latent_decode": 2,
                      "sb_delta_prefill": 3}
 
@@ -33,7 +33,7 @@ _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_
 # then passed as plain numbers, which saves an object for each.
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
-              "sb_kv8_chunk_sizes": "pppiiiiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
+              "sb_capture_id": "p", "sb_kv8_chunk_sizes": "pppiiiiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
 
 
 class _CountingLib:
@@ -48,6 +48,8 @@ class _CountingLib:
         fn = self._cache.get(name)
         if fn is None:
             raw = getattr(self._cdll, name)
+            if name == "sb_capture_id":
+                raw.restype = ctypes.c_ulonglong
             if name in _ARGUMENTS:
                 raw.argtypes = [_LETTERS[x] for x in _ARGUMENTS[name]]
             k = _KERNELS_PER_CALL.get(name, 1)
@@ -172,12 +174,22 @@ def status_word(device: Optional[torch.device] = None) -> torch.Tensor:
     return w
 
 
+_after_status_errors: list = []
+
+
+def on_status_error(call) -> None:
+    """``call`` runs when :func:`check_status` finds that a kernel gave up: for workspaces that expect kernels to end."""
+    _after_status_errors.append(call)
+
+
 def check_status(device: Optional[torch.device] = None) -> None:
     """Synchronising read of the status word; raises KernelStatusError when a kernel gave up a wait."""
     w = status_word(device)
     code = int(w.item())
     if code != 0:
         w.zero_()
+        for call in _after_status_errors:
+            call()
         raise KernelStatusError(code)
 
 

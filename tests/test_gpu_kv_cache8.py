@@ -306,6 +306,37 @@ def test_decode_attention_of_strided_rows_on_another_stream_and_in_a_graph():
     lib.check_status()
 
 
+def test_decode_attention_in_graphs_that_take_turns():
+    """Two graphs of two calls each and calls outside of them, replayed in any order; a larger call behind a smaller one."""
+    hq, hkv, d = 28, 4, 128
+    cache, table, q, n = _decode([2000, 65, 900, 1500], hq, hkv, d, 40)
+    g, q, n, table = _gpu(cache), q.to(DEV), n.to(DEV), table.to(DEV)
+
+    def call(k):
+        return kvc.decode_attention(q[:k], g, n[:k], table[:k], hq, hkv, d)
+    want = {k: call(k).clone() for k in (1, 2, 4)}
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = [call(1), call(4)]
+        graphs.append((graph, held))
+    for i in (0, 1, 1, 0):
+        for t in graphs[i][1]:
+            t.zero_()
+        graphs[i][0].replay()
+        assert torch.equal(call(2), want[2])
+        assert torch.equal(graphs[i][1][0], want[1]) and torch.equal(graphs[i][1][1], want[4])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        others = [call(4) for _ in range(5)]
+    here = [call(4) for _ in range(5)]
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, want[4]) for x in others + here)
+    lib.check_status()
+
+
 def _check_prefix(new, old, hq, hkv, d, spread=1.0, q_scale=1.0):
     """Bounds: weights and output are rounded to 16 bits; see _check_decode for the rest."""
     total = [a + b for a, b in zip(new, old)]
