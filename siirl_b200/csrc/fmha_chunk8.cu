@@ -4,7 +4,9 @@
 // unpack8_kernel writes the visible tokens' keys and values once as bf16 rows [2, Hkv, rows, D] (code times scale, exact where
 // the scale is a power of two), every sequence from a multiple of 128 rows on, zeros behind its last token.  It moves 5 bytes per
 // cached number, against 4 * Hq / Hkv * chunk flops per number that the products take; converting in every block of the product
-// kernel instead would cost it shared memory bandwidth, of which its operands take three quarters.
+// kernel instead would cost it shared memory bandwidth, of which its operands take three quarters.  A code that is NaN is written
+// as zero and its block of 64 rows marked: in a tile that some rows see in part, zero times a value that is NaN would reach rows
+// before it.  The rows that do see it get their NaN at the end, from the codes.
 //
 // fmha_chunk_kernel: one block takes one or two tiles of 128 rows of one kv head, a row being (position, query head of the kv
 // head): heads that share keys share a tile, so that short chunks fill it, too, and keys are fetched once for all of them.
@@ -53,11 +55,14 @@ __device__ __forceinline__ uint2 bf16_of(uint32_t codes, float scale) {
   return make_uint2(pack_bf16x2(a.x * scale, a.y * scale), pack_bf16x2(b.x * scale, b.y * scale));
 }
 
-// block x: 64 rows; block y: k and v heads
+// bytes of four codes: 0xff where one is NaN
+__device__ __forceinline__ uint32_t nan_codes(uint32_t c) { return __vcmpeq4(c & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+// block x: 64 rows; block y: k and v heads; marks: [2 * Hkv, rows / 64]
 template <int D>
 __global__ void __launch_bounds__(256) unpack8_kernel(const __grid_constant__ ChunkSeqs q, const uint8_t* codes, const float* scales,
                                                       int num_blocks, const int* block_table, int max_blocks, int Hkv,
-                                                      __nv_bfloat16* out) {
+                                                      __nv_bfloat16* out, int* marks) {
   chain_sync();
   const int row = blockIdx.x * 64, i = find_seq(q.kv_row, q.n, row), t0 = row - q.kv_row[i], left = q.total[i] - t0;
   const int hd = blockIdx.y, kv = hd >= Hkv;
@@ -67,12 +72,16 @@ __global__ void __launch_bounds__(256) unpack8_kernel(const __grid_constant__ Ch
   const float scale = blk < 0 ? 0.f : scales[at];
   const uint4* src = reinterpret_cast<const uint4*>(codes + at * 64 * D);
   uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)hd * q.rows + row) * D);
+  uint32_t nan = 0;
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) {
     const int u = k * 256 + threadIdx.x;      // 16 numbers
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
     if (blk >= 0 && u * 16 / D < left) {
-      const uint4 c = src[u];
+      uint4 c = src[u];
+      const uint4 m = make_uint4(nan_codes(c.x), nan_codes(c.y), nan_codes(c.z), nan_codes(c.w));
+      c = make_uint4(c.x & ~m.x, c.y & ~m.y, c.z & ~m.z, c.w & ~m.w);
+      nan |= m.x | m.y | m.z | m.w;
       const uint2 p0 = bf16_of(c.x, scale), p1 = bf16_of(c.y, scale), p2 = bf16_of(c.z, scale), p3 = bf16_of(c.w, scale);
       a = make_uint4(p0.x, p0.y, p1.x, p1.y);
       b = make_uint4(p2.x, p2.y, p3.x, p3.y);
@@ -80,12 +89,41 @@ __global__ void __launch_bounds__(256) unpack8_kernel(const __grid_constant__ Ch
     dst[2 * u] = a;
     dst[2 * u + 1] = b;
   }
+  const int any = __syncthreads_or(nan != 0);
+  if (threadIdx.x == 0) marks[hd * (q.rows / 64) + blockIdx.x] = any;
+}
+
+// NaN for a row of the output where it sees one, in a key for all columns: tokens t0 (a block's first) .. t1 - 1.  `codes`: of the key
+// head in block 0, those of its values `values` further on; `marks`: of its block of t0 and those behind it, likewise
+template <int D, typename T>
+__device__ __noinline__ void mark_nan(const int* marks, int value_marks, const uint8_t* codes, size_t values, size_t block_bytes,
+                                      const int* blocks, int t0, int t1, T* row) {
+  for (int t = t0; t < t1; ++t) {
+    const int key = marks[(t - t0) / 64], value = marks[value_marks + (t - t0) / 64];
+    if (!key && !value) {
+      t |= 63;
+      continue;
+    }
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(codes + blocks[t / 64] * block_bytes + t % 64 * D);
+    uint32_t any = 0;
+    for (int k = 0; key && k < D / 4; ++k) any |= nan_codes(c[k]);
+    for (int k = 0; k < D / 4; ++k) {
+      const uint32_t m = any ? 0xffffffffu : value ? nan_codes(c[values / 4 + k]) : 0u;
+      for (int i = 0; m && i < 4; ++i)
+        if (m >> (8 * i) & 1) row[4 * k + i] = T(__int_as_float(0x7fc00000));
+    }
+    if (any) return;
+  }
 }
 
 struct ChunkParams {
   __nv_bfloat16* out;      // [chunk rows, Hq * D]
   float* ws_o;             // [tile, kv head, split, query tile, 128, D], where splits > 1
   float* ws_lse;           // [.., 128]
+  const int* marks;        // unpack8_kernel's
+  const uint8_t* codes;
+  const int* block_table;
+  int max_blocks;
   int Hq, Hkv, rep, span, splits;      // span: positions of 128 rows
   float scale_log2;
   int* status;
@@ -160,6 +198,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* full = bar_q + 10;                                       // [kStages] ring of K and V tiles
   uint64_t* empty = full + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + kStages);
+  int* s_nan = reinterpret_cast<int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -193,6 +232,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int j0 = (int)((long long)all * split / p.splits), j1 = (int)((long long)all * (split + 1) / p.splits);
   const int n0 = max(0, min(key_tiles(0), j1) - j0), n1 = QT == 2 ? max(0, min(key_tiles(1), j1) - j0) : 0;
   const int n_max = max(n0, n1);
+  const int* marks = p.marks + g * (seqs.rows / 64) + (seqs.kv_row[seq] + j0 * KV) / 64;
 
   if (warp == kTmaWarp) {
     // ------------------------------ TMA producer ------------------------------
@@ -223,6 +263,12 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int k = max(0, i - kStages); k < i; ++k) mbar_wait(&full[k % kStages], (k / kStages) & 1, nullptr, 0);
       }
     }
+    // while the last tiles are worked on: whether one of the keys and values is NaN
+    __syncwarp();
+    int any = 0;
+    for (int i = lane; i < n_max * (KV / 64); i += 32) any |= marks[i] | marks[p.Hkv * (seqs.rows / 64) + i];
+    any = __any_sync(0xffffffffu, any);
+    if (lane == 0) *s_nan = any;
   } else if (warp == kMmaWarp) {
     // ------------------------------ MMA issuer: one thread ------------------------------
     // The soft-max warps leave it few issue slots: descriptors differ in their low words only, which are kept and stepped
@@ -416,6 +462,21 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
   }
+  if (*s_nan && warp < kTmaWarp) {      // over what the thread has written
+    const int w = warp >> 2, row = tid & 127, at = row / p.rep, qpos = prefix + c0 + w * p.span + at;
+    const int t0 = j0 * KV, t1 = min(qpos + 1, t0 + (w ? n1 : n0) * KV);
+    if (at < p.span && qpos < total) {
+      const size_t values = (size_t)p.Hkv * 64 * D, part = ((((size_t)tile * p.Hkv + g) * p.splits + split) * QT + w) * 128 + row;
+      const uint8_t* codes = p.codes + (size_t)g * 64 * D;
+      const int* blocks = p.block_table + (size_t)seqs.slot[seq] * p.max_blocks;
+      const int more = p.Hkv * (seqs.rows / 64);
+      if (p.splits > 1)
+        mark_nan<D>(marks, more, codes, values, 2 * values, blocks, t0, t1, p.ws_o + part * D);
+      else
+        mark_nan<D>(marks, more, codes, values, 2 * values, blocks, t0, t1,
+                    p.out + ((size_t)seqs.q_row[seq] + qpos - prefix) * (p.Hq * D) + (size_t)(g * p.rep + row - at * p.rep) * D);
+    }
+  }
 }
 
 // Mean of the shares' results, weighted by 2^(log-sum-exp).  A block takes 16 rows, half a warp each: first the largest weight,
@@ -459,6 +520,9 @@ struct ChunkPlan {
   ChunkSeqs s;
   int qt, kv, ctas, span, splits;
 };
+// 16-bit numbers of the unpacked keys and values, and of the marks behind them
+static long long unpacked(const ChunkPlan& c, int Hkv, int D) { return 2ll * Hkv * c.s.rows * D; }
+static long long marks_of(const ChunkPlan& c, int Hkv) { return ((long long)Hkv * (c.s.rows / 32) + 3) / 4 * 8; }
 static int make_chunk_plan(ChunkPlan& c, const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D) {
   const int rep = Hq / Hkv;
   c.span = 128 / rep;
@@ -525,7 +589,7 @@ using namespace sb;
 
 extern "C" int sb_kv8_chunk_seqs() { return kChunkSeqs; }
 
-// Sizes of a call's workspaces: sizes[0] bf16 numbers of unpacked keys and values, sizes[1] floats (0: the result is written at
+// Sizes of a call's workspaces: sizes[0] 16-bit numbers for unpacked keys and values (`kv`), sizes[1] floats (0: the result is written at
 // once); sizes[2]: rows of the chunks.  The lists are the host's, of at most kChunkSeqs sequences.  -5: chunks that `rows` rows, or
 // a table of `slots` rows of `max_blocks` blocks, cannot hold.
 extern "C" int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D, int rows, int slots,
@@ -539,7 +603,7 @@ extern "C" int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int
   if (sum > rows) return -5;
   ChunkPlan c;
   const int rc = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
-  sizes[0] = 2ll * Hkv * c.s.rows * D;
+  sizes[0] = unpacked(c, Hkv, D) + marks_of(c, Hkv);
   sizes[1] = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * (D + 1) : 0;
   sizes[2] = sum;
   return rc;
@@ -566,12 +630,14 @@ extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, const void* 
   if (r) return r;
   r = make_tensor_map_bf16_2d(&mkv, kv, D, 2ll * Hkv * c.s.rows, D, 64, c.kv);
   if (r) return r;
+  int* marks = reinterpret_cast<int*>((__nv_bfloat16*)kv + unpacked(c, Hkv, D));
   r = launch_chained(D == 128 ? unpack8_kernel<128> : unpack8_kernel<64>, dim3(c.s.rows / 64, 2 * Hkv), 256, 0, stream, c.s,
-                     (const uint8_t*)codes, scales, num_blocks, block_table, max_blocks, Hkv, (__nv_bfloat16*)kv);
+                     (const uint8_t*)codes, scales, num_blocks, block_table, max_blocks, Hkv, (__nv_bfloat16*)kv, marks);
   if (r) return r;
   ChunkParams p;
   p.out = (__nv_bfloat16*)out; p.ws_o = ws;
   p.ws_lse = ws + (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * D;
+  p.marks = marks; p.codes = (const uint8_t*)codes; p.block_table = block_table; p.max_blocks = max_blocks;
   p.Hq = Hq; p.Hkv = Hkv; p.rep = Hq / Hkv; p.span = c.span; p.splits = c.splits;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   if (c.qt == 1) return D == 128 ? launch_chunk<128, 64, 1, 2>(mq, mkv, c, p, stream) : launch_chunk<64, 64, 1, 3>(mq, mkv, c, p, stream);

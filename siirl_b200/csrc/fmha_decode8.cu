@@ -75,11 +75,6 @@ __device__ __forceinline__ float redux_max(float x) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
 // whether `any` is set in one of the 128 threads of four soft-max warps
 __device__ __forceinline__ bool vote_128(int group, bool any) {
   uint32_t r;
@@ -955,9 +950,6 @@ static int launch_decode8(const CUtensorMap& mc, const Decode8Params& p, int gri
 
 using namespace sb;
 
-// Workspaces: with rows = 8 where at most 8 query heads share a kv head or D = 64, else 16, ws_o has 2 * grid * rows * D floats,
-// ws_lse 8 * grid * rows; counts B * Hkv * ceil(Hq / Hkv / rows) * 4 ints, which are zeros and stay zeros after every call, but one
-// whose waits ran out.
 // Number of the capture that `stream` takes part in, 0 outside of one
 extern "C" unsigned long long sb_capture_id(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -968,6 +960,10 @@ extern "C" unsigned long long sb_capture_id(cudaStream_t stream) {
 
 extern "C" int sb_kv8_decode_grid() { return num_sms(); }
 
+// Workspaces: with rows = 8 where at most 8 query heads share a kv head or D = 64, else 16, ws_o has 2 * grid * rows * D floats,
+// ws_lse 8 * grid * rows; counts B * Hkv * ceil(Hq / Hkv / rows) * 4 ints, which are zeros and stay zeros after every call, but one
+// whose waits ran out.
+//
 // One query row per sequence (at most 1024) against its cached context of seq_lens[b] tokens, the current one included; 0: idle
 // slot, its output row is zero.  Rows start on 4-byte boundaries.
 extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const float* scales, int num_blocks,
@@ -976,7 +972,7 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
                              cudaStream_t stream) {
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
-  if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || max_blocks < 1 || num_blocks < 1) return -3;
+  if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || reinterpret_cast<uintptr_t>(q) % 4 || reinterpret_cast<uintptr_t>(out) % 16 || max_blocks < 1 || num_blocks < 1) return -3;
   const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (long long)(max_blocks + 1) / 2 * B * Hkv * 4;
   if (rows > 0x7fffffffll || tiles > 0x7fffffffll) return -4;
   static thread_local bool tl_context_bound = false;

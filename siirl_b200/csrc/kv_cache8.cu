@@ -556,7 +556,7 @@ extern "C" int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long
                              int num_blocks, int T, int Hq, int Hkv, int D, cudaStream_t stream) {
   if (T == 0) return 0;
   if (D != 64 && D != 128) return -2;
-  if (row_stride % 2 || (slabs && (splits < 1 || slab_stride % 2)) || (rope_pos && table_rows < 1)) return -3;
+  if (row_stride % 2 || reinterpret_cast<uintptr_t>(qkv) % 4 || reinterpret_cast<uintptr_t>(slabs) % 8 || (slabs && (splits < 1 || slab_stride % 2)) || (rope_pos && table_rows < 1)) return -3;
   Append8Params p;
   p.qkv = (__nv_bfloat16*)qkv; p.row_stride = row_stride; p.slabs = slabs; p.slab_stride = slab_stride; p.splits = splits;
   p.bias = (const __nv_bfloat16*)bias; p.rope_pos = rope_pos; p.pos_rows = pos_rows; p.sec0 = sec0; p.sec1 = sec1;

@@ -135,8 +135,8 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
     if slabs is None:
         if bias is not None:
             _refuse("a bias is added to partial sums only")
-    elif slabs.dtype is not torch.float32 or not slabs.is_contiguous() or slabs.shape[0] == 0:
-        _refuse("partial sums are contiguous float32")
+    elif slabs.dtype is not torch.float32 or not slabs.is_contiguous() or slabs.shape[0] == 0 or slabs.data_ptr() % 8:
+        _refuse("partial sums are contiguous float32 from an 8-byte boundary on")
     elif bias is not None and (bias.shape != (width,) or not bias.is_contiguous() or bias.get_device() != dev or
                                bias.dtype is not torch.bfloat16):
         _refuse(f"the bias is {width} bf16 numbers")
@@ -229,18 +229,18 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
         rep = n_heads // n_kv_heads
         out.zero_()
         for b in range(B):
-            n = int(seq_lens[b])
-            if n == 0:
+            n = min(int(seq_lens[b]), BLOCK * block_table.shape[1])
+            if n <= 0:
                 continue
             x = cache.dequantize(block_table[b, :(n + BLOCK - 1) // BLOCK].long())
             k, v = (x[:, i].permute(1, 0, 2, 3).reshape(n_kv_heads, -1, head_dim)[:, :n].repeat_interleave(rep, 0) for i in (0, 1))
             s = torch.einsum("hd,hnd->hn", q_rows[b, :width].reshape(n_heads, head_dim).float(), k) * scale
             out[b] = torch.einsum("hn,hnd->hd", torch.softmax(s, -1), v).reshape(-1).to(out.dtype)
         return out
-    if q_rows.dtype is not torch.bfloat16:
-        _refuse("query rows are bf16")
+    if q_rows.dtype is not torch.bfloat16 or out.data_ptr() % 16:
+        _refuse("query rows are bf16, and the output starts on a 16-byte boundary")
     if q_rows.stride(0) % 2 or q_rows.data_ptr() % 4:
-        q_rows = q_rows[:, :width].contiguous()
+        q_rows = q_rows[:, :width].clone(memory_format=torch.contiguous_format)      # contiguous rows may be the odd ones
     dev = q_rows.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
@@ -323,8 +323,8 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     if rows == 0 and not any(lists[0]):
         return out
     stride, one = qkv.stride()
-    if one != 1 or stride % 8 or qkv.data_ptr() % 16:
-        qkv = qkv.contiguous()
+    if one != 1 or stride % 8 or stride < width or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)      # contiguous rows may be the odd ones
         stride = qkv.shape[1]
     L = _lib.get_lib()
     with _device(qkv.get_device()):
@@ -337,7 +337,7 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
             if rc == -5 or i + n == total and at + sizes[2] != rows:
                 check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
             _lib.check(rc, "sb_kv8_chunk_sizes")
-            # buffers of the call's own, as for single tokens
+            # buffers of the call's own
             ws = torch.empty(2 * sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=qkv.device)
             _lib.check(L.sb_kv8_chunks(
                 qkv.data_ptr() + 2 * at * stride, stride, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.codes.shape[0],

@@ -67,7 +67,7 @@ def attention(q, codes, scales, blocks, seen, hq, hkv, d, scale):
     """``q [rows, hq * d]``; row i sees the first ``seen[i]`` tokens of the blocks.  Returns (output, sum of weight * |value|)."""
     out, size = (torch.zeros(q.shape[0], hq, d, dtype=torch.float64) for _ in range(2))
     if not len(blocks):
-        return out.view(len(q), -1), size.view(len(q), -1)
+        return out.view(len(q), hq * d), size.view(len(q), hq * d)
     x = codes[blocks].double() * scales[blocks].double()[..., None, None]
     for h in range(hq):
         g = h // (hq // hkv)
@@ -76,4 +76,4 @@ def attention(q, codes, scales, blocks, seen, hq, hkv, d, scale):
             if n:
                 w = torch.softmax(k[:n] @ q[i, h * d:(h + 1) * d].double() * scale, 0)
                 out[i, h], size[i, h] = w @ v[:n], w @ v[:n].abs()
-    return out.view(len(q), -1), size.view(len(q), -1)
+    return out.view(len(q), hq * d), size.view(len(q), hq * d)

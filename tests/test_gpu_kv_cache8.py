@@ -428,3 +428,116 @@ def test_engine_on_the_8_bit_cache():
     assert eager.stats["prefix_cache_hit_tokens"] >= 64 + 128
     lib.check_status()
     assert eager.alloc.num_free == eager.alloc.num_blocks
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (4, 1, 64)])
+@pytest.mark.parametrize("new,old", [((5,), (3000,)), ((300, 40), (70, 0)), ((2300,), (1,))])
+def test_prefix_attention_keeps_nan_from_rows_that_do_not_see_it(hq, hkv, d, new, old):
+    """A key, and values of some columns, of tokens of the chunks and of a prefix: NaN in the rows that see them, and nowhere else."""
+    total = [a + b for a, b in zip(new, old)]
+    need = [(n + 63) // 64 for n in total]
+    cache = _random_cache(sum(need), hkv, d)
+    nan = cache.codes.view(torch.uint8)
+    table, first = torch.full((len(new), max(need)), -1, dtype=torch.int32), 0
+    for i, k in enumerate(need):
+        table[i, :k] = torch.arange(first, first + k)
+        t = total[i] - 3
+        nan[first + t // 64, 1, 0, t % 64, [3, d - 1]] = 0x7f
+        t = total[i] - 2
+        nan[first + t // 64, 1, hkv - 1, t % 64, 17] = 0xff
+        t = total[i] - 1
+        nan[first + t // 64, 0, 0, t % 64, 5] = 0x7f
+        first += k
+    nan[0, 1, hkv - 1, 0, 40] = 0x7f        # all rows of the first sequence
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d).bfloat16()
+    out = kvc.prefill_attention_with_prefix(rows.to(DEV), new, old, list(range(len(new))), _gpu(cache), table.to(DEV), hq, hkv, d)
+    out = out.cpu().double()
+    lib.check_status()
+    at = 0
+    for i, (a, o, k) in enumerate(zip(new, old, need)):
+        pick = sorted(set(range(0, a, 97)) | set(range(max(0, a - 5), a)))
+        want, size = oracle.attention(rows[[at + j for j in pick], :hq * d], *cache, table[i, :k].long(), [o + j + 1 for j in pick],
+                                      hq, hkv, d, d ** -0.5)
+        got = out[[at + j for j in pick]]
+        assert torch.equal(got.isnan(), want.isnan())
+        err = (got - want).abs()
+        assert bool((err <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size)[~want.isnan()].all())
+        at += a
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (16, 1, 128)])
+def test_attention_of_more_sequences_than_a_launch_takes(hq, hkv, d):
+    """Single tokens of 1300 sequences, some idle; chunks of 110, some empty."""
+    n, most = 1300, 3
+    cache = _random_cache(n, hkv, d)
+    table = torch.randint(0, n, (n, most), dtype=torch.int32)
+    lens = torch.randint(0, 64 * most + 1, (n,), dtype=torch.int32)
+    lens[::7] = 0
+    q = torch.randn(n, hq * d).bfloat16()
+    out = kvc.decode_attention(q.to(DEV), _gpu(cache), lens.to(DEV), table.to(DEV), hq, hkv, d).cpu().double()
+    for i in (0, 1, 500, 1022, 1023, 1024, 1025, 1298, 1299):
+        want, size = oracle.attention(q[i:i + 1], *cache, table[i].long(), [int(lens[i])], hq, hkv, d, d ** -0.5)
+        assert bool(((out[i:i + 1] - want).abs() <= BF16 * want.abs() + 2.0 ** -10 * size).all()), i
+    assert not out[lens == 0].any()
+    _check_prefix([(5 * i) % 23 if i % 9 else 0 for i in range(110)], [(31 * i) % 130 for i in range(110)], hq, hkv, d)
+
+
+def test_calls_of_nothing():
+    hq, hkv, d = 4, 2, 64
+    cache = _gpu(_random_cache(4, hkv, d))
+    before = cache.codes.view(torch.uint8).clone()
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    table, width = torch.zeros(2, 2, dtype=torch.int32, device=DEV), (hq + 2 * hkv) * d
+    none = torch.empty(0, width, device=DEV, dtype=torch.bfloat16)
+    cos, sin = (x.to(DEV) for x in ref.rope_tables(d, 64, 1e4))
+    assert kvc.decode_attention(none, cache, i(), table[:0], hq, hkv, d).shape == (0, hq * d)
+    assert not kvc.decode_attention(torch.ones(2, hq * d, device=DEV).bfloat16(), cache, i(0, 0), table, hq, hkv, d).any()
+    kvc.kv_append(none, i(), i(), table, cache, hq, hkv, d)
+    assert kvc.rope_kv_append(none, i(), cos, sin, None, i(), i(), table, cache, hq, hkv, d).shape == (0, width)
+    kvc.kv_copy_blocks(cache, i(), i())
+    assert kvc.prefill_attention_with_prefix(none, [], [], [], cache, table, hq, hkv, d).shape == (0, hq * d)
+    assert kvc.prefill_attention_with_prefix(none, [0, 0], [0, 70], [0, 1], cache, table, hq, hkv, d).shape == (0, hq * d)
+    row = torch.randn(1, width, device=DEV).bfloat16()
+    kept = row.clone()
+    kvc.kv_append(row, i(-1), i(3), table, cache, hq, hkv, d)       # a row of no sequence
+    kvc.kv_append(row, i(0), i(128), table, cache, hq, hkv, d)      # and one behind the table
+    torch.cuda.synchronize()
+    assert torch.equal(cache.codes.view(torch.uint8), before) and torch.equal(row, kept)
+
+
+def test_lengths_beyond_the_table_end_with_it():
+    hq, hkv, d = 4, 2, 128
+    cache = _gpu(_random_cache(5, hkv, d))
+    table = torch.tensor([[4, 1], [0, 3]], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, hq * d, device=DEV).bfloat16()
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    want = kvc.decode_attention(q, cache, i(128, 0), table, hq, hkv, d)
+    assert torch.equal(kvc.decode_attention(q, cache, i(2 ** 31 - 1, -5), table, hq, hkv, d), want)
+    here = kvc.decode_attention(q.cpu(), Cache8(*(x.cpu() for x in cache)), i(2 ** 31 - 1, -5).cpu(), table.cpu(), hq, hkv, d)
+    # two roundings to bf16, and the kernel's own error
+    assert float((here.float() - want.cpu().float()).abs().max()) <= 2.0 ** -6 * float(want.abs().max())
+
+
+def test_refusals_of_what_starts_at_odd_places():
+    hq, hkv, d = 4, 2, 64
+    cache, width = _gpu(_random_cache(4, hkv, d)), (4 + 2 * 2) * 64
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    cos, sin = (x.to(DEV) for x in ref.rope_tables(d, 64, 1e4))
+    q = torch.randn(2, width, device=DEV).bfloat16()
+    out = torch.empty(2 * hq * d + 8, dtype=torch.bfloat16, device=DEV)[3:3 + 2 * hq * d].view(2, hq * d)
+    sums = torch.zeros(2 * width + 1, device=DEV)[1:].view(1, 2, width)
+    odd = torch.zeros(2 * width + 1, dtype=torch.bfloat16, device=DEV)[1:].view(2, width)
+    for call in (lambda: kvc.decode_attention(q, cache, lens, table, hq, hkv, d, out=out),
+                 lambda: kvc.rope_kv_append(sums, lens, cos, sin, None, lens, lens, table, cache, hq, hkv, d),
+                 lambda: kvc.rope_kv_append(odd, lens, cos, sin, None, lens, lens, table, cache, hq, hkv, d)):
+        with pytest.raises(ValueError, match="8-bit cache"):
+            call()
+    want = kvc.decode_attention(q, cache, lens, table, hq, hkv, d)      # query rows may start anywhere
+    odd.copy_(q)
+    assert torch.equal(kvc.decode_attention(odd, cache, lens, table, hq, hkv, d), want)
+    odd_q = torch.zeros(2 * hq * d + 1, dtype=torch.bfloat16, device=DEV)[1:].view(2, hq * d)
+    odd_q.copy_(q[:, :hq * d])
+    assert torch.equal(kvc.decode_attention(odd_q, cache, lens, table, hq, hkv, d), want)
+    n, p, s = [2], [3], [0]
+    assert torch.equal(kvc.prefill_attention_with_prefix(odd, n, p, s, cache, table, hq, hkv, d),
+                       kvc.prefill_attention_with_prefix(q, n, p, s, cache, table, hq, hkv, d))
