@@ -8,18 +8,24 @@
 // as zero and its block of 64 rows marked: in a tile that some rows see in part, zero times a value that is NaN would reach rows
 // before it.  The rows that do see it get their NaN at the end, from the codes.
 //
-// fmha_chunk_kernel: one block takes one or two tiles of 128 rows of one kv head, a row being (position, query head of the kv
-// head): heads that share keys share a tile, so that short chunks fill it, too, and keys are fetched once for all of them.
-//   S = Q K_j^T      tcgen05.mma 128 x KV x D -> TMEM
-//   soft-max         one warpgroup per tile, thread = row; weights (bf16) replace the scores in TMEM, in two halves, each
-//                    handed to the products at once
-//   O += P V_j       tcgen05.mma 128 x D x KV, P from TMEM, V through an MN-major descriptor
-// The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.  At D = 64
-// the exponentials (16 a cycle and SM) take twice as long as the products, and every fourth pair is computed on the
-// fused-multiply-add units (4 sequences of up to 2000 rows, 14 / 2 heads: 262 us, 283 without; at D = 128 it costs what it
-// saves): 2^x = 2^n 2^f with n the nearest integer and a cubic in f, |f| <= 1/2, fitted for the smallest largest relative error
-// (7.5e-5, a fiftieth of a bf16 step) by iteratively reweighted least squares.
-// Where there are fewer blocks than fit the SMs, the key tiles are split over several, whose results chunk_merge_kernel joins.
+// fmha_chunk_kernel: a block takes 128 rows of one kv head, a row being (position, query head of the kv head): heads that share
+// keys share a block, so that short chunks fill it, too, and keys are fetched once for all of them.  For every 64 keys:
+//   S = Q K_j^T      tcgen05.mma 128 x 64 x D -> TMEM, one of two places: the next scores are computed meanwhile
+//   soft-max         one warpgroup, thread = row; weights (bf16) replace the scores in TMEM, in two halves, each handed to the
+//                    products at once
+//   O += P V_j       tcgen05.mma 128 x D x 64, P from TMEM, V through an MN-major descriptor
+// Two blocks of an SM share its tensor cores: one computes weights while the other's products run.  (One block with two tiles of
+// 128 keys each, which read a third less from shared memory: 2 sequences of up to 2148 rows, 32 / 8 heads, 740 us against 706, and
+// more blocks that are not full.)
+// The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.
+// The exponentials (16 a cycle and SM) take as long as the products, at D = 64 twice as long: every fourth pair, at D = 64 every
+// second one, is computed on the fused-multiply-add units (2048 rows of one prompt, 28 / 4 heads: 157 us, 165 without; 4 sequences
+// of up to 2000 rows, 14 / 2 heads, D = 64: 249, 265 without): 2^x = 2^n 2^f with n the nearest integer and a cubic in f,
+// |f| <= 1/2, fitted for the smallest largest relative error (7.5e-5, a fiftieth of a bf16 step) by iteratively reweighted
+// least squares.
+// Bound by the tensor cores at the clock that the power limit leaves: 2 sequences of up to 2148 rows behind up to 14,000 tokens: 706 us,
+// 1.22 PFLOP/s, 88 % of what a long run of a library product reaches.
+// Where there are few blocks, the key tiles are split over several, whose results chunk_merge_kernel joins.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -29,6 +35,8 @@
 
 namespace sb {
 
+constexpr int kChunkKeys = 64;       // keys of a tile
+constexpr int kChunkCtas = 2;        // blocks of an SM
 constexpr int kChunkSeqs = 48;       // sequences of one launch: what goes with it costs the host time
 
 struct ChunkSeqs {
@@ -129,13 +137,12 @@ struct ChunkParams {
   int* status;
 };
 
-template <int D, int KV, int QT>
+template <int D>
 struct ChunkSmem {
-  static constexpr int kQBytes = 128 * D * 2, kKvBytes = KV * D * 2;
-  static constexpr int kStages = QT == 1 ? 4 : D == 128 ? 5 : 6;
-  static constexpr int kRingOff = QT * kQBytes;
-  static constexpr int kBarOff = kRingOff + kStages * kKvBytes;  // q[2], s_full[2], p_full[2][2], o_full[2], full[], empty[]
-  static constexpr int kTotal = kBarOff + (10 + 2 * kStages) * 8 + 16;
+  static constexpr int kQBytes = 128 * D * 2, kKvBytes = kChunkKeys * D * 2;
+  static constexpr int kStages = 4;
+  static constexpr int kBarOff = kQBytes + kStages * kKvBytes;  // q, s_full[2], p_full[2][2], o_full, o_step, full[], empty[]
+  static constexpr int kTotal = kBarOff + (9 + 2 * kStages) * 8 + 16;
 };
 
 // two of 2^x, x >= -126: see above
@@ -174,15 +181,14 @@ __device__ __forceinline__ void umma_bf16_ts_lo(uint32_t tmem_d, uint32_t tmem_a
       : "memory");
 }
 
-// KV: keys of a tile; QT: query tiles; CTAS: blocks of an SM.
-// Four warps for the soft-max of each query tile (thread = row), then one for TMA and the MMA issuer.
-template <int D, int KV, int QT, int CTAS>
-__global__ void __launch_bounds__(QT * 128 + 64, CTAS)
+// Four warps for the soft-max (thread = row), then one for TMA and the MMA issuer.
+template <int D>
+__global__ void __launch_bounds__(192, kChunkCtas)
 fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                   const __grid_constant__ ChunkSeqs seqs, ChunkParams p) {
-  using L = ChunkSmem<D, KV, QT>;
-  constexpr int kDChunks = D / 64, kStages = L::kStages, kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1;
-  constexpr uint32_t kTmemCols = QT * (KV + D) <= 128 ? 128 : QT * (KV + D) <= 256 ? 256 : 512;
+  using L = ChunkSmem<D>;
+  constexpr int KV = kChunkKeys, kDChunks = D / 64, kStages = L::kStages, kTmaWarp = 4, kMmaWarp = 5;
+  constexpr uint32_t kTmemCols = 256;      // two places of scores, then the output
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   if (smem_u32(smem) & 1023u) {
@@ -190,12 +196,13 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     return;
   }
   uint8_t* sQ = smem;
-  uint8_t* ring = smem + L::kRingOff;
-  uint64_t* bar_q = reinterpret_cast<uint64_t*>(smem + L::kBarOff);  // [2]
-  uint64_t* s_full = bar_q + 2;                                      // [2] scores are in TMEM
-  uint64_t* p_full = bar_q + 4;                                      // [2][2] halves of the weights have replaced the scores
-  uint64_t* o_full = bar_q + 8;                                      // [2] the output is complete
-  uint64_t* full = bar_q + 10;                                       // [kStages] ring of K and V tiles
+  uint8_t* ring = smem + L::kQBytes;
+  uint64_t* bar_q = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* s_full = bar_q + 1;                                      // [place] scores are in TMEM
+  uint64_t* p_full = bar_q + 3;                                      // [place][2] halves of the weights have replaced the scores
+  uint64_t* o_full = bar_q + 7;                                      // the output is complete
+  uint64_t* o_step = bar_q + 8;                                      // it has the products of one more tile
+  uint64_t* full = bar_q + 9;                                        // [kStages] ring of K and V tiles
   uint64_t* empty = full + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + kStages);
   int* s_nan = reinterpret_cast<int*>(tmem_slot + 1);
@@ -204,7 +211,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (tid == 0) {
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_kv);
-    for (int i = 0; i < 10; ++i) mbar_init(&bar_q[i], i >= 4 && i < 8 ? 4 : 1);
+    for (int i = 0; i < 9; ++i) mbar_init(&bar_q[i], i >= 3 && i < 7 ? 4 : 1);
     for (int i = 0; i < 2 * kStages; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
   }
@@ -222,32 +229,20 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int tile = (int)(blockIdx.x / p.splits / p.Hkv), seq = find_seq(seqs.tile, seqs.n, tile);
   const int prefix = seqs.prefix[seq], total = seqs.total[seq];
   const int tile_end = seq + 1 < seqs.n ? seqs.tile[seq + 1] : seqs.tiles;
-  const int c0 = (tile_end - 1 - tile) * QT * p.span;      // first position, in the chunk
-  // key tiles that query tile w walks over: first .. key_tiles(w) - 1
-  auto key_tiles = [&](int w) {
-    const int from = prefix + c0 + w * p.span;
-    return from >= total ? 0 : (min(from + p.span, total) + KV - 1) / KV;
-  };
-  const int all = max(key_tiles(0), QT == 2 ? key_tiles(1) : 0);
-  const int j0 = (int)((long long)all * split / p.splits), j1 = (int)((long long)all * (split + 1) / p.splits);
-  const int n0 = max(0, min(key_tiles(0), j1) - j0), n1 = QT == 2 ? max(0, min(key_tiles(1), j1) - j0) : 0;
-  const int n_max = max(n0, n1);
+  const int c0 = (tile_end - 1 - tile) * p.span, first = prefix + c0;      // first position, in the chunk and in the sequence
+  const int all = (min(first + p.span, total) + KV - 1) / KV;
+  const int j0 = (int)((long long)all * split / p.splits), n = (int)((long long)all * (split + 1) / p.splits) - j0;      // key tiles
   const int* marks = p.marks + g * (seqs.rows / 64) + (seqs.kv_row[seq] + j0 * KV) / 64;
 
   if (warp == kTmaWarp) {
     // ------------------------------ TMA producer ------------------------------
-    if (lane == 0 && n_max > 0) {
-      const int q_row = seqs.q_row[seq] + c0;
+    if (lane == 0 && n > 0) {
       const int k_row = g * seqs.rows + seqs.kv_row[seq] + j0 * KV, v_row = k_row + p.Hkv * seqs.rows;
-      auto load_q = [&](int w) {
-        mbar_arrive_expect_tx(&bar_q[w], (uint32_t)(kDChunks * p.rep * p.span * 128));
+      mbar_arrive_expect_tx(bar_q, (uint32_t)(kDChunks * p.rep * p.span * 128));
 #pragma unroll
-        for (int c = 0; c < kDChunks; ++c)
-          tma_load_3d(sQ + w * L::kQBytes + c * 16384, &map_q, &bar_q[w], c * 64, g * p.rep, q_row + w * p.span);
-      };
-      load_q(0);
+      for (int c = 0; c < kDChunks; ++c) tma_load_3d(sQ + c * 16384, &map_q, bar_q, c * 64, g * p.rep, seqs.q_row[seq] + c0);
       int i = 0;
-      for (; i < 2 * n_max; ++i) {  // K0 V0 K1 V1 ...
+      for (; i < 2 * n; ++i) {  // K0 V0 K1 V1 ...
         const int st = i % kStages;
         if (!mbar_wait(&empty[st], ((i / kStages) & 1) ^ 1, p.status, kStatusTimeoutProducer)) break;
         uint8_t* dst = ring + st * L::kKvBytes;
@@ -255,18 +250,16 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         mbar_arrive_expect_tx(&full[st], L::kKvBytes);
 #pragma unroll
         for (int c = 0; c < kDChunks; ++c) tma_load_2d(dst + c * (KV * 128), &map_kv, &full[st], c * 64, row);
-        if (i == 0 && n1 > 0) load_q(1);
       }
-      if (i < 2 * n_max) {  // gave up: no copy may land in shared memory that has been handed on
-        mbar_wait(&bar_q[0], 0, nullptr, 0);
-        if (n1 > 0 && i > 0) mbar_wait(&bar_q[1], 0, nullptr, 0);
+      if (i < 2 * n) {  // gave up: no copy may land in shared memory that has been handed on
+        mbar_wait(bar_q, 0, nullptr, 0);
         for (int k = max(0, i - kStages); k < i; ++k) mbar_wait(&full[k % kStages], (k / kStages) & 1, nullptr, 0);
       }
     }
     // while the last tiles are worked on: whether one of the keys and values is NaN
     __syncwarp();
     int any = 0;
-    for (int i = lane; i < n_max * (KV / 64); i += 32) any |= marks[i] | marks[p.Hkv * (seqs.rows / 64) + i];
+    for (int i = lane; i < n * (KV / 64); i += 32) any |= marks[i] | marks[p.Hkv * (seqs.rows / 64) + i];
     any = __any_sync(0xffffffffu, any);
     if (lane == 0) *s_nan = any;
   } else if (warp == kMmaWarp) {
@@ -279,12 +272,28 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint32_t q_lo = (uint32_t)umma_smem_desc(smem_u32(sQ), 16, 1024), k_lo = (uint32_t)umma_smem_desc(smem_u32(ring), 16, 1024);
       const uint32_t v_lo = (uint32_t)umma_smem_desc(smem_u32(ring), KV * 128, 1024);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, p.status, kStatusTimeoutMma); };
-      auto scores = [&](int w, int stage) {
-        const uint32_t a = q_lo + w * (L::kQBytes >> 4), b = k_lo + stage * kStep;
+      auto scores = [&](int place, int stage) {
+        const uint32_t b = k_lo + stage * kStep;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16_ss_lo(tmem_base + w * KV, a + (kk / 4) * 1024 + (kk % 4) * 2, b + (kk / 4) * (KV * 8) + (kk % 4) * 2, idesc_s, kk > 0);
-        umma_commit(&s_full[w]);
+          umma_bf16_ss_lo(tmem_base + place * KV, q_lo + (kk / 4) * 1024 + (kk % 4) * 2, b + (kk / 4) * (KV * 8) + (kk % 4) * 2, idesc_s, kk > 0);
+        umma_commit(&s_full[place]);
+        umma_commit(&empty[stage]);
+      };
+      auto products = [&](int place, int stage, int parity, bool first) {
+        const uint32_t v = v_lo + stage * kStep;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!wait(&p_full[2 * place + part], parity)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < KV / 32; ++k) {
+            const int kk = part * (KV / 32) + k;
+            umma_bf16_ts_lo(tmem_base + 2 * KV, tmem_base + place * KV + kk * 8, v + kk * 128, idesc_o, kk > 0 || !first);
+          }
+        }
+        umma_commit(&empty[stage]);
+        return true;
       };
       int ks = 0, vs = 1;                  // ring places of K_j and V_j
       uint32_t k_phase = 0, v_phase = 0;
@@ -295,62 +304,34 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           phase ^= 1;
         }
       };
-      bool ok = n_max > 0 && wait(&bar_q[0], 0) && wait(&full[0], 0);
+      bool ok = n > 0 && wait(bar_q, 0) && wait(&full[0], 0);
       tc_fence_after();
-      if (ok) {
-        if (n0 > 0) scores(0, 0);
-        if (n1 > 0) {
-          ok = wait(&bar_q[1], 0);
-          if (ok) scores(1, 0);
-        }
-        umma_commit(&empty[0]);
-      }
-      for (int j = 0; j < n_max && ok; ++j) {
+      if (ok) scores(0, 0);
+      for (int j = 0; j < n && ok; ++j) {
         step(ks, k_phase);
-        ok = wait(&full[vs], v_phase) && (j + 1 >= n_max || wait(&full[ks], k_phase));
-#pragma unroll
-        for (int w = 0; w < QT; ++w) {
-          const int n = w ? n1 : n0;
-          if (j < n) {
-            const uint32_t v = v_lo + vs * kStep;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              ok = ok && wait(&p_full[2 * w + part], j & 1);
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll
-              for (int k = 0; k < KV / 32; ++k) {
-                const int kk = part * (KV / 32) + k;
-                umma_bf16_ts_lo(tmem_base + QT * KV + w * D, tmem_base + w * KV + kk * 8, v + kk * 128, idesc_o, kk > 0 || j > 0);
-              }
-            }
-            if (ok && j + 1 < n) scores(w, ks);
-            else if (ok) umma_commit(&o_full[w]);
-          }
-          if (w == QT - 1) {
-            umma_commit(&empty[vs]);
-            if (j + 1 < n_max) umma_commit(&empty[ks]);
-          }
-        }
+        const bool more = j + 1 < n;
+        if (more) ok = wait(&full[ks], k_phase);
+        if (more && ok) scores(j + 1 & 1, ks);
+        ok = ok && wait(&full[vs], v_phase) && products(j & 1, vs, j >> 1 & 1, j == 0);
+        if (!ok) break;
+        umma_commit(more ? o_step : o_full);
         step(vs, v_phase);
       }
     }
     __syncwarp();
   } else {
     // ------------------------------ softmax and output: thread = row ------------------------------
-    const int w = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tmem_s = tmem_base + lane_off + w * KV;
-    const uint32_t tmem_o = tmem_base + lane_off + QT * KV + w * D;
-    const int first = prefix + c0 + w * p.span, at = row / p.rep, head = row - at * p.rep;
+    const int row = tid, at = row / p.rep, head = row - at * p.rep;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16, tmem_o = tmem_base + lane_off + 2 * KV;
     const int qpos = first + at;      // position within the sequence
-    const int n = w ? n1 : n0;
     const float sc = p.scale_log2;
     float m_ref = -INFINITY;          // reference of the weights, scaled
     float2 l_run[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[w], j & 1, p.status, kStatusTimeoutEpilogue));
+      const int place = j & 1;
+      const uint32_t tmem_s = tmem_base + lane_off + place * KV;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[place], j >> 1 & 1, p.status, kStatusTimeoutEpilogue));
       if (!ok) break;
       tc_fence_after();
       uint32_t s[KV / 32][32];
@@ -369,7 +350,13 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       for (int i = 0; i < KV; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i / 32][i % 32]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
       if (__any_sync(0xffffffffu, top > m_ref + 8.f)) {
-        // The barrier of the scores also said that P V of the previous tile is done
+        // The barrier of the scores also said that the products of the tile before the last one are done: o_step is at most one
+        // phase behind
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(o_step, j - 1 & 1, p.status, kStatusTimeoutEpilogue));
+          if (!ok) break;
+          tc_fence_after();
+        }
         const float m_new = fmaxf(m_ref, top), alpha = fast_exp2(m_ref - (m_new == -INFINITY ? 0.f : m_new));
         m_ref = m_new;
 #pragma unroll
@@ -400,7 +387,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           for (int i = i0; i < i0 + 32; i += 2) {
             float2 x = make_float2(__uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
             x = fma_f32x2(x, sc2, neg);
-            if (D == 64 && i % 8 == 6) {
+            if (i % 8 == 6 || D == 64 && i % 8 == 2) {
               x = poly_exp2(x);
             } else {
               x.x = fast_exp2(x.x);
@@ -414,17 +401,17 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * w + part]);
+        if (lane == 0) mbar_arrive(&p_full[2 * place + part]);
       }
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[w], 0, p.status, kStatusTimeoutEpilogue));
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full, 0, p.status, kStatusTimeoutEpilogue));
     // ---- O / l -> bf16, or the share's normalised result (TMEM loads are warp-collective; only the stores are predicated) ----
     if (ok) {
       tc_fence_after();
       const bool row_valid = at < p.span && qpos < total;
       const float l = m_ref == -INFINITY ? 0.f : (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
       const float inv_l = l != 0.f ? 1.f / l : 0.f;
-      const size_t part = ((((size_t)tile * p.Hkv + g) * p.splits + split) * QT + w) * 128 + row;
+      const size_t part = (((size_t)tile * p.Hkv + g) * p.splits + split) * 128 + row;
       const size_t out_row = (size_t)seqs.q_row[seq] + (row_valid ? qpos - prefix : 0);
       __nv_bfloat16* orow = p.out + out_row * (size_t)(p.Hq * D) + (size_t)(g * p.rep + head) * D;
       if (n > 0) {
@@ -463,10 +450,9 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tmem_dealloc(tmem_base, kTmemCols);
   }
   if (*s_nan && warp < kTmaWarp) {      // over what the thread has written
-    const int w = warp >> 2, row = tid & 127, at = row / p.rep, qpos = prefix + c0 + w * p.span + at;
-    const int t0 = j0 * KV, t1 = min(qpos + 1, t0 + (w ? n1 : n0) * KV);
+    const int row = tid, at = row / p.rep, qpos = first + at, t0 = j0 * KV, t1 = min(qpos + 1, t0 + n * KV);
     if (at < p.span && qpos < total) {
-      const size_t values = (size_t)p.Hkv * 64 * D, part = ((((size_t)tile * p.Hkv + g) * p.splits + split) * QT + w) * 128 + row;
+      const size_t values = (size_t)p.Hkv * 64 * D, part = (((size_t)tile * p.Hkv + g) * p.splits + split) * 128 + row;
       const uint8_t* codes = p.codes + (size_t)g * 64 * D;
       const int* blocks = p.block_table + (size_t)seqs.slot[seq] * p.max_blocks;
       const int more = p.Hkv * (seqs.rows / 64);
@@ -482,15 +468,15 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 // Mean of the shares' results, weighted by 2^(log-sum-exp).  A block takes 16 rows, half a warp each: first the largest weight,
 // then all shares at once, so that their reads are under way together (32 shares of 30 rows: 9 us less than one after the other).
 template <int D>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkSeqs seqs, ChunkParams p, int qt) {
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkSeqs seqs, ChunkParams p) {
   chain_sync();
   const int unit = blockIdx.x / 8, row = blockIdx.x % 8 * 16 + (threadIdx.x >> 4), l = threadIdx.x & 15;
-  const int w = unit % qt, g = unit / qt % p.Hkv, tile = unit / qt / p.Hkv, seq = find_seq(seqs.tile, seqs.n, tile);
+  const int g = unit % p.Hkv, tile = unit / p.Hkv, seq = find_seq(seqs.tile, seqs.n, tile);
   const int tile_end = seq + 1 < seqs.n ? seqs.tile[seq + 1] : seqs.tiles;
-  const int at = row / p.rep, pos = ((tile_end - 1 - tile) * qt + w) * p.span + at;
+  const int at = row / p.rep, pos = (tile_end - 1 - tile) * p.span + at;
   if (at >= p.span || pos >= seqs.total[seq] - seqs.prefix[seq]) return;
   constexpr int N = D / 64;      // groups of four columns of a lane
-  const size_t first = (((size_t)tile * p.Hkv + g) * p.splits * qt + w) * 128 + row, step = (size_t)qt * 128;
+  const size_t first = (size_t)unit * p.splits * 128 + row, step = 128;
   float top = -INFINITY, sum = 0.f;
   for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.ws_lse[first + s * step]);
   float4 acc[N] = {};
@@ -518,7 +504,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant_
 // What a call does, from the host's lists alone
 struct ChunkPlan {
   ChunkSeqs s;
-  int qt, kv, ctas, span, splits;
+  int span, splits;
 };
 // 16-bit numbers of the unpacked keys and values, and of the marks behind them
 static long long unpacked(const ChunkPlan& c, int Hkv, int D) { return 2ll * Hkv * c.s.rows * D; }
@@ -536,39 +522,43 @@ static int make_chunk_plan(ChunkPlan& c, const int* chunk, const int* prefix, co
   }
   // those that see most first
   std::sort(order, order + live, [&](int a, int b) { return prefix[a] + chunk[a] > prefix[b] + chunk[b]; });
-  auto tiles_of = [&](int span) {
-    long long t = 0;
-    for (int k = 0; k < live; ++k) t += (chunk[order[k]] + span - 1) / span;
-    return t;
-  };
-  const long long ones = tiles_of(c.span), twos = tiles_of(2 * c.span);
-  // two tiles share their keys; one alone leaves room for a second block on the SM
-  c.qt = ones * Hkv <= 2 * num_sms() || twos * 2 * 100 > ones * 110 ? 1 : 2;
-  c.kv = c.qt == 2 && D == 128 ? 128 : 64;
-  c.ctas = c.qt == 2 ? (D == 128 ? 1 : 2) : (D == 128 ? 2 : 3);
   c.s.n = live;
   int tiles = 0, longest = 0;
+  long long all = 0;      // tiles of keys that the tiles of positions walk over
   for (int k = 0; k < live; ++k) {
     const int i = order[k], total = prefix[i] + chunk[i];
     c.s.slot[k] = slot[i]; c.s.total[k] = total; c.s.prefix[k] = prefix[i]; c.s.q_row[k] = first[i];
     c.s.kv_row[k] = (int)rows; c.s.tile[k] = tiles;
     rows += (total + 127) / 128 * 128;
-    tiles += (chunk[i] + c.qt * c.span - 1) / (c.qt * c.span);
-    longest = std::max(longest, (total + c.kv - 1) / c.kv);
+    const int rows_of = (chunk[i] + c.span - 1) / c.span;
+    tiles += rows_of;
+    all += rows_of * ((prefix[i] + chunk[i] / 2) / (long long)kChunkKeys + 1);
+    longest = std::max(longest, (total + kChunkKeys - 1) / kChunkKeys);
     if (rows * 2 * Hkv > 0x7fffffffll) return -4;
   }
   c.s.rows = (int)rows;
   c.s.tiles = tiles;
-  const long long blocks = (long long)tiles * Hkv, room = (long long)num_sms() * c.ctas;
-  c.splits = blocks ? (int)std::max(1ll, std::min({room / blocks, (long long)longest / 8, 16ll})) : 1;
+  // Shares of the keys: each costs its blocks about what twelve tiles of keys do (results in 32 bits, written and read), and spares
+  // the last blocks to run alone.  In tiles:
+  const long long blocks = (long long)tiles * Hkv, room = (long long)num_sms() * kChunkCtas;
+  c.splits = 1;
+  float best = 3.0e38f;
+  for (int s = 1; s <= 16 && s <= std::max(1, longest / 8); ++s) {
+    const float waves = (float)(blocks * s) / room, share = (float)longest / s;
+    const float time = (waves <= 1.f ? share : (float)all * Hkv / room + 0.5f * share) + (s > 1 ? 12.f * std::max(1.f, waves) + 6.f : 0.f);
+    if (time < best) {
+      best = time;
+      c.splits = s;
+    }
+  }
   if (blocks * c.splits > 0x7fffffffll / 32) return -4;
   return 0;
 }
 
-template <int D, int KV, int QT, int CTAS>
+template <int D>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mkv, const ChunkPlan& c, const ChunkParams& p, cudaStream_t stream) {
-  using L = ChunkSmem<D, KV, QT>;
-  auto kernel = fmha_chunk_kernel<D, KV, QT, CTAS>;
+  using L = ChunkSmem<D>;
+  auto kernel = fmha_chunk_kernel<D>;
   static int configured = -1;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -578,9 +568,9 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mkv, const Chu
     configured = dev;
   }
   const unsigned blocks = (unsigned)(c.s.tiles * p.Hkv * c.splits);
-  const int rc = launch_chained(kernel, blocks, QT * 128 + 64, L::kTotal, stream, mq, mkv, c.s, p);
+  const int rc = launch_chained(kernel, blocks, 192, L::kTotal, stream, mq, mkv, c.s, p);
   if (rc || c.splits == 1) return rc;
-  return launch_chained(chunk_merge_kernel<D>, (unsigned)(c.s.tiles * p.Hkv * QT * 8), 256, 0, stream, c.s, p, QT);
+  return launch_chained(chunk_merge_kernel<D>, (unsigned)(c.s.tiles * p.Hkv * 8), 256, 0, stream, c.s, p);
 }
 
 }  // namespace sb
@@ -604,7 +594,7 @@ extern "C" int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int
   ChunkPlan c;
   const int rc = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
   sizes[0] = unpacked(c, Hkv, D) + marks_of(c, Hkv);
-  sizes[1] = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * (D + 1) : 0;
+  sizes[1] = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * 128 * (D + 1) : 0;
   sizes[2] = sum;
   return rc;
 }
@@ -628,7 +618,7 @@ extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, const void* 
   CUtensorMap mq, mkv;
   r = make_tensor_map_bf16_3d(&mq, qkv, D, Hq, rows, D, row_stride, 64, Hq / Hkv, c.span);
   if (r) return r;
-  r = make_tensor_map_bf16_2d(&mkv, kv, D, 2ll * Hkv * c.s.rows, D, 64, c.kv);
+  r = make_tensor_map_bf16_2d(&mkv, kv, D, 2ll * Hkv * c.s.rows, D, 64, kChunkKeys);
   if (r) return r;
   int* marks = reinterpret_cast<int*>((__nv_bfloat16*)kv + unpacked(c, Hkv, D));
   r = launch_chained(D == 128 ? unpack8_kernel<128> : unpack8_kernel<64>, dim3(c.s.rows / 64, 2 * Hkv), 256, 0, stream, c.s,
@@ -636,10 +626,9 @@ extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, const void* 
   if (r) return r;
   ChunkParams p;
   p.out = (__nv_bfloat16*)out; p.ws_o = ws;
-  p.ws_lse = ws + (long long)c.s.tiles * Hkv * c.splits * c.qt * 128 * D;
+  p.ws_lse = ws + (long long)c.s.tiles * Hkv * c.splits * 128 * D;
   p.marks = marks; p.codes = (const uint8_t*)codes; p.block_table = block_table; p.max_blocks = max_blocks;
   p.Hq = Hq; p.Hkv = Hkv; p.rep = Hq / Hkv; p.span = c.span; p.splits = c.splits;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
-  if (c.qt == 1) return D == 128 ? launch_chunk<128, 64, 1, 2>(mq, mkv, c, p, stream) : launch_chunk<64, 64, 1, 3>(mq, mkv, c, p, stream);
-  return D == 128 ? launch_chunk<128, 128, 2, 1>(mq, mkv, c, p, stream) : launch_chunk<64, 64, 2, 2>(mq, mkv, c, p, stream);
+  return D == 128 ? launch_chunk<128>(mq, mkv, c, p, stream) : launch_chunk<64>(mq, mkv, c, p, stream);
 }
