@@ -213,13 +213,14 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
                      n_kv_heads: int, head_dim: int, scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`siirl_b200.ops.kv_cache.decode_attention` on an 8-bit cache."""
-    B, width = q_rows.shape[0], n_heads * head_dim
+    shape, width = q_rows.shape, n_heads * head_dim
     scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
     _check(cache, n_heads, n_kv_heads, head_dim, q_rows)
     _check_ints(q_rows, seq_lens, block_table)
-    if q_rows.dim() != 2 or q_rows.shape[1] < width or q_rows.stride(1) != 1:
+    if len(shape) != 2 or shape[1] < width or q_rows.stride(1) != 1:
         _refuse(f"query rows are at least {width} wide")
-    if seq_lens.shape != (B,) or block_table.dim() != 2 or block_table.shape[0] < B:
+    B, table = shape[0], block_table.shape
+    if seq_lens.shape != (B,) or len(table) != 2 or table[0] < B:
         _refuse(f"a length and a row of the table for each of {B} rows")
     if out is None:
         out = torch.empty(B, width, dtype=q_rows.dtype, device=q_rows.device)
@@ -239,15 +240,17 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
         return out
     if q_rows.dtype is not torch.bfloat16 or out.data_ptr() % 16:
         _refuse("query rows are bf16, and the output starts on a 16-byte boundary")
-    if q_rows.stride(0) % 2 or q_rows.data_ptr() % 4:
-        q_rows = q_rows[:, :width].clone(memory_format=torch.contiguous_format)      # contiguous rows may be the odd ones
     dev = q_rows.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return decode_attention(q_rows, cache, seq_lens, block_table, n_heads, n_kv_heads, head_dim, scale, out)
+    stride, q = q_rows.stride(0), q_rows.data_ptr()
+    if stride % 2 or q % 4:      # contiguous rows may be the odd ones
+        q_rows = q_rows[:, :width].clone(memory_format=torch.contiguous_format)
+        stride, q = width, q_rows.data_ptr()
     L = _lib.get_lib()
     codes, scales = cache
-    stride, max_blocks = q_rows.stride(0), block_table.shape[1]
+    max_blocks = table[1]
     rows = 8 if n_heads <= 8 * n_kv_heads or head_dim == 64 else 16
     part = 2 * L.sb_kv8_decode_grid() * rows        # rows of partial results: two for each block of the grid
     entries = n_kv_heads * -(-(n_heads // n_kv_heads) // rows)
@@ -256,7 +259,7 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
     for at in range(0, B, ROWS):
         n = min(ROWS, B - at)
         _lib.check(L.sb_kv8_decode(
-            q_rows.data_ptr() + 2 * at * stride, stride, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+            q + 2 * at * stride, stride, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
             seq_lens.data_ptr() + 4 * at, block_table.data_ptr() + 4 * at * max_blocks, max_blocks,
             out.data_ptr() + 2 * at * width, floats.data_ptr(), floats.data_ptr() + 4 * part * head_dim, counts.data_ptr(), n,
             n_heads, n_kv_heads, head_dim, scale, _lib.status_word(q_rows.device).data_ptr(), stream), "sb_kv8_decode")
@@ -270,7 +273,7 @@ _decode_buffers: dict = {}
 
 
 def _decode_workspace(dev: int, stream: int, floats: int, counts: int):
-    capture = _lib.get_lib().sb_capture_id(stream)
+    capture = _lib.get_lib().sb_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
     held = _decode_buffers.get((dev, stream, capture != 0))
     if held is None or held[2] != capture or held[0].numel() < floats or held[1].numel() < counts:
         more = (0, 0) if held is None or held[2] != capture else (held[0].numel(), held[1].numel())
