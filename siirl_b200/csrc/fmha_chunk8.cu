@@ -15,15 +15,15 @@
 //                    products at once
 //   O += P V_j       tcgen05.mma 128 x D x 64, P from TMEM, V through an MN-major descriptor
 // Two blocks of an SM share its tensor cores: one computes weights while the other's products run.  (One block with two tiles of
-// 128 keys each, which read a third less from shared memory: 2 sequences of up to 2148 rows, 32 / 8 heads, 740 us against 706, and
+// 128 keys each, which read a third less from shared memory: 2 sequences of up to 2148 rows, 32 / 8 heads, 740 us against 704, and
 // more blocks that are not full.)
 // The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.
 // The exponentials (16 a cycle and SM) take as long as the products, at D = 64 twice as long: every fourth pair, at D = 64 every
-// second one, is computed on the fused-multiply-add units (2048 rows of one prompt, 28 / 4 heads: 157 us, 165 without; 4 sequences
-// of up to 2000 rows, 14 / 2 heads, D = 64: 249, 265 without): 2^x = 2^n 2^f with n the nearest integer and a cubic in f,
+// second one, is computed on the fused-multiply-add units (2048 rows of one prompt, 28 / 4 heads: 155 us, 162 without; 4 sequences
+// of up to 2000 rows, 14 / 2 heads, D = 64: 253, 266 without): 2^x = 2^n 2^f with n the nearest integer and a cubic in f,
 // |f| <= 1/2, fitted for the smallest largest relative error (7.5e-5, a fiftieth of a bf16 step) by iteratively reweighted
 // least squares.
-// Bound by the tensor cores at the clock that the power limit leaves: 2 sequences of up to 2148 rows behind up to 14,000 tokens: 706 us,
+// Bound by the tensor cores at the clock that the power limit leaves: 2 sequences of up to 2148 rows behind up to 14,000 tokens: 704 us,
 // 1.22 PFLOP/s, 88 % of what a long run of a library product reaches.
 // Where there are few blocks, the key tiles are split over several, whose results chunk_merge_kernel joins.
 #include <cuda_fp8.h>
@@ -145,18 +145,17 @@ struct ChunkSmem {
   static constexpr int kTotal = kBarOff + (9 + 2 * kStages) * 8 + 16;
 };
 
-// two of 2^x, x >= -126: see above
+// two of 2^x: see above.  0 from -127 down: a weight of what a row does not see times a large value would be seen
 __device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
   const float2 big = make_float2(12582912.f, 12582912.f), small = make_float2(-12582912.f, -12582912.f);      // 1.5 * 2^23
   const float2 t = add_f32x2(x, big), n = add_f32x2(t, small), minus = make_float2(-1.f, -1.f);
   const float2 f = fma_f32x2(n, minus, x);
   float2 p = fma_f32x2(f, make_float2(0.0551716817f, 0.0551716817f), make_float2(0.24261115979f, 0.24261115979f));
   p = fma_f32x2(p, f, make_float2(0.69326098678f, 0.69326098678f));
   p = fma_f32x2(p, f, make_float2(0.99992807130f, 0.99992807130f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  return mul_f32x2(p, make_float2(__int_as_float(0x3f800000 + (__float_as_int(t.x) << 23)), __int_as_float(0x3f800000 + (__float_as_int(t.y) << 23))));
 }
 
 // One thread's MMAs, of operands whose descriptors have the high word of 128-byte swizzle and 1024 bytes between groups of eight

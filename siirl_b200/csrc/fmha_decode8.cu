@@ -7,7 +7,9 @@
 //     number has, down to 2^-22 of the row's largest;
 //   * a weight into three e5m2 terms, each remainder 16 times enlarged: off by at most 2^-11 of itself or 2^-36 of the largest
 //     weight.  e5m2 for its range: thousands of small weights may stand beside one large one whose value is near zero.
-// The block's scales go into the score and into the weight, in 32 bits.
+// The block's scales go into the score and into the weight, in 32 bits.  So a block with a large scale and small codes would take
+// the weights' range from the others: a piece whose blocks' value scales are more than 2^16 apart (those below 2^-60 aside) is
+// computed again in 32 bits by the output warps (d8_exact), some ten times slower.
 //
 // A tile is 128 rows of 128 bytes: two cache blocks at D = 128; at D = 64, where a row holds two tokens, four.
 //   S^T[row, (token of the row, term, head)] = K Q^T     A = the K tile, B = the terms of all query heads of a kv head
@@ -39,6 +41,7 @@ namespace sb {
 constexpr int kQ8Rows = 1024;        // sequences of one launch
 constexpr int kQ8Smem = 227 * 1024;
 constexpr int kQ8MinTiles = 2;       // tiles of a range, where there are so few that not every SM gets as many
+constexpr float kQ8Spread = 16.f, kQ8Low = -60.f;      // log2 of value scales: apart, and of those that do not count
 constexpr float kQ8None = -3.0e38f;  // reference before anything has been seen
 
 // mbar_wait() with all but the first look in one place: sixteen warps run seven programs here, and what each of them takes of the
@@ -107,6 +110,7 @@ __device__ __forceinline__ float2 from_e5m2x2(uint32_t codes) {
 struct Decode8Params {
   const __nv_bfloat16* q;   // [B, row_stride], q heads first
   long long row_stride;
+  const uint8_t* codes;     // [num_blocks, 2, Hkv, 64, D]
   const float* scales;      // [num_blocks, 2, Hkv]
   const int* seq_lens;      // [B]
   const int* block_table;   // [B, max_blocks]
@@ -139,7 +143,8 @@ struct D8 {
   static constexpr int kPieceOff = kBlockOff + kStages * BPT * 16;     // [NQ] {sequence, entry, first tile, tiles}
   static constexpr int kRedOff = kPieceOff + NQ * 16;                  // [2 groups][4][NR] {max z, max z + log2 vs}
   static constexpr int kStatOff = kRedOff + 2 * 4 * NR * 8;            // [2 buffers][2 groups]: l [4][NR], m [NR], M [NR]
-  static constexpr int kFactorOff = kStatOff + 4 * 6 * NR * 4;         // [NQ][NR] factor of the scores
+  static constexpr int kSpreadOff = kStatOff + 4 * 6 * NR * 4;         // [2 buffers][8 warps] {least, largest log2 vs} of the piece
+  static constexpr int kFactorOff = kSpreadOff + 16 * 8;               // [NQ][NR] factor of the scores
   static constexpr int kBarOff = kFactorOff + NQ * NR * 4;
   static constexpr int kBars = 3 * kStages + 2 * NQ + 14;
   static constexpr int kPreOff = kBarOff + kBars * 8 + 24;
@@ -259,6 +264,72 @@ __device__ __noinline__ void d8_join(const float* parts, const float* lses, int*
     if (h < heads) orow[h * D] = __float2bfloat16(sum[h] == 0.f ? 0.f : acc[h] / sum[h]);
 }
 
+// Tokens t0 .. t1 - 1 of a kv head for `heads` query rows in 32 bits, by one warp: o[h] of column d, lse of the lane's head.
+// A lane takes the scores of every 32nd token, and column d of the weighted sum.
+template <int D, int NR>
+__device__ __noinline__ void d8_exact(const __nv_bfloat16* q, int heads, const uint8_t* codes, const float* scales, const int* blocks,
+                                      int num_blocks, int Hkv, int kv_head, int t0, int t1, float scale_log2, int d, float (&o)[NR],
+                                      float& lse) {
+  const int lane = threadIdx.x & 31;
+  lse = -INFINITY;
+  float m[NR], l[NR], w[NR], acc[NR];
+#pragma unroll
+  for (int h = 0; h < NR; ++h) {
+    m[h] = kQ8None;
+    l[h] = acc[h] = 0.f;
+  }
+#pragma unroll 1
+  for (int base = t0; base < t1; base += 32) {
+    const int t = base + lane;
+    int id = t < t1 ? blocks[t / 64] : -1;
+    if (id >= num_blocks) id = -1;
+    const size_t at = id < 0 ? 0 : (size_t)id * 2 * Hkv + kv_head;
+    const uint32_t* k = reinterpret_cast<const uint32_t*>(codes + (at * 64 + t % 64) * D);
+    const float vs = id < 0 ? 0.f : scales[at + Hkv];
+#pragma unroll
+    for (int h = 0; h < NR; ++h) w[h] = 0.f;
+    if (id >= 0) {
+#pragma unroll 1
+      for (int c = 0; c < D / 4; ++c) {
+        const uint32_t x = k[c];
+        const float2 a = from_e4m3x2(x & 0xffffu), b = from_e4m3x2(x >> 16);
+#pragma unroll
+        for (int h = 0; h < NR; ++h)
+          if (h < heads) {
+            const __nv_bfloat162* r = reinterpret_cast<const __nv_bfloat162*>(q + h * D + 4 * c);
+            const float2 e = __bfloat1622float2(r[0]), f = __bfloat1622float2(r[1]);
+            w[h] = fmaf(e.x, a.x, fmaf(e.y, a.y, fmaf(f.x, b.x, fmaf(f.y, b.y, w[h]))));
+          }
+      }
+    }
+    const float ks = id < 0 ? 0.f : scales[at] * scale_log2;
+#pragma unroll
+    for (int h = 0; h < NR; ++h) {
+      const float z = id < 0 ? -INFINITY : w[h] * ks, now = fmaxf(m[h], redux_max(z)), f = fast_exp2(m[h] - now);
+      w[h] = fast_exp2(z - now);
+      l[h] = fmaf(l[h], f, w[h]);      // of the lane's tokens
+      acc[h] *= f;
+      m[h] = now;
+    }
+#pragma unroll 1
+    for (int j = 0; j < 32 && base + j < t1; ++j) {
+      const int block = __shfl_sync(0xffffffffu, id, j);
+      const float s = __shfl_sync(0xffffffffu, vs, j);
+      if (block < 0) continue;
+      const float v = s * from_e4m3x2(codes[(((size_t)block * 2 + 1) * Hkv + kv_head) * 64 * D + (size_t)((base + j) % 64) * D + d]).x;
+#pragma unroll
+      for (int h = 0; h < NR; ++h) acc[h] = fmaf(__shfl_sync(0xffffffffu, w[h], j), v, acc[h]);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < NR; ++h) {
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], i);
+    o[h] = l[h] == 0.f ? 0.f : acc[h] / l[h];
+    if (lane == h) lse = l[h] == 0.f ? -INFINITY : m[h] + log2f(l[h]);
+  }
+}
+
 constexpr int kQ8Threads = 16 * 32;
 
 template <int D, int NR>
@@ -277,6 +348,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   int4* s_piece = reinterpret_cast<int4*>(smem + L::kPieceOff);
   float2* s_red = reinterpret_cast<float2*>(smem + L::kRedOff);
   float* s_stat = reinterpret_cast<float*>(smem + L::kStatOff);
+  float2* s_spread = reinterpret_cast<float2*>(smem + L::kSpreadOff);
   float* s_factor = reinterpret_cast<float*>(smem + L::kFactorOff);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* v_full = k_full + NST;
@@ -612,6 +684,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
         l[i] = make_float2(0.f, 0.f);
       }
       bool first = true;
+      float least = INFINITY, largest = -INFINITY;      // of log2 vs; lane 0 has the warp's, as what is seen begins with its row
       for (int t = PACK == 1 ? tn + ((tn ^ g) & 1) : tn; t < stop; t += 3 - PACK) {
         const uint32_t b = t & 1, phase = t >> 1 & 1;
         ok = ok && wait(&s_full[b], phase);
@@ -646,6 +719,10 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < NR / 2; ++i)
             if (!seen) z[i] = make_float2(-INFINITY, -INFINITY);
+        }
+        if (seen && lv > kQ8Low) {
+          least = fminf(least, lv);
+          largest = fmaxf(largest, lv);
         }
         if constexpr (PACK == 2) {
           if (g == 0 && __any_sync(0xffffffffu, left == 1)) {
@@ -820,6 +897,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
             *reinterpret_cast<float2*>(stat + 5 * NR + 2 * i) = make_float2(-M[i].x, -M[i].y);
           }
       }
+      if (lane == 0) s_spread[ib * 8 + warp] = make_float2(least, largest);
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&q_empty[iq]);
@@ -843,6 +921,12 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       const uint32_t ib = piece_no & 1;
       if (!__all_sync(0xffffffffu, bar_wait(&o_full[ib], (piece_no >> 1) & 1, p.status, kStatusTimeoutEpilogue))) break;
       tc_fence_after();
+      float2 spread = s_spread[ib * 8];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) {
+        const float2 x = s_spread[ib * 8 + w];
+        spread = make_float2(fminf(spread.x, x.x), fmaxf(spread.y, x.y));
+      }
       // lane h: head h's factors of the two O^T, and its log-sum-exp
       float f[2] = {0.f, 0.f}, lse = -INFINITY;
       if (lane < NR) {
@@ -902,6 +986,15 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
         const int left = heads_of(q.entry);
         const int slot = 2 * blockIdx.x + (cur == begin ? 0 : 1);
         const bool whole = q.n == q.tiles;
+        if (spread.y - spread.x > kQ8Spread) {
+          float exact[NR], exact_lse;      // o and lse stay in registers
+          d8_exact<D, NR>(p.q + (size_t)q.row * p.row_stride + (size_t)first_head(q.entry) * D, left, p.codes, p.scales,
+                          p.block_table + (size_t)q.row * p.max_blocks, p.num_blocks, p.Hkv, kv_head(q.entry), q.t0 * L::TT,
+                          min(s_len[q.row], (q.t0 + q.n) * L::TT), p.scale_log2, d, exact, exact_lse);
+#pragma unroll
+          for (int h = 0; h < NR; ++h) o[h] = exact[h];
+          lse = exact_lse;
+        }
         __nv_bfloat16* orow = p.out + ((size_t)q.row * p.Hq + first_head(q.entry)) * D + d;
         float* wrow = p.ws_o + (size_t)slot * NR * D + d;
 #pragma unroll
@@ -985,7 +1078,7 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   const int r = make_tensor_map_bf16_2d(&mc, codes, 64, rows, 64, 64, D / 2);
   if (r) return r;
   Decode8Params p;
-  p.q = (const __nv_bfloat16*)q; p.row_stride = row_stride; p.scales = scales; p.seq_lens = seq_lens;
+  p.q = (const __nv_bfloat16*)q; p.row_stride = row_stride; p.codes = (const uint8_t*)codes; p.scales = scales; p.seq_lens = seq_lens;
   p.block_table = block_table; p.num_blocks = num_blocks; p.max_blocks = max_blocks; p.B = B; p.Hq = Hq; p.Hkv = Hkv;
   const int most = Hq / Hkv <= 8 || D == 64 ? 8 : 16;
   p.groups = (Hq / Hkv + most - 1) / most;

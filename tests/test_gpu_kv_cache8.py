@@ -541,3 +541,38 @@ def test_refusals_of_what_starts_at_odd_places():
     n, p, s = [2], [3], [0]
     assert torch.equal(kvc.prefill_attention_with_prefix(odd, n, p, s, cache, table, hq, hkv, d),
                        kvc.prefill_attention_with_prefix(q, n, p, s, cache, table, hq, hkv, d))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (2, 2, 128), (16, 1, 128)])
+@pytest.mark.parametrize("new,old", [((5,), (3000,)), ((300, 40), (70, 0)), ((700,), (1,))])
+def test_attention_does_not_feel_large_values_that_it_does_not_see(hq, hkv, d, new, old):
+    """The last three tokens of each sequence have the largest keys and values that a cache can hold: rows before them stay within
+    the bounds that they have without these.  (Not to the bit: what the tensor cores keep of a sum depends on the largest exponent that
+    takes part, also where the other factor is zero.)"""
+    total = [a + b for a, b in zip(new, old)]
+    need = [(n + 63) // 64 for n in total]
+    cache = _random_cache(sum(need), hkv, d)
+    table, first = torch.full((len(new), max(need)), -1, dtype=torch.int32), 0
+    for i, (n, k) in enumerate(zip(total, need)):
+        table[i, :k] = torch.arange(first, first + k)
+        first += k
+        assert n % 64 >= 3
+        cache.codes[first - 1] = 0
+        cache.codes[first - 1, :, :, n % 64 - 3:] = 448.0
+        cache.scales[first - 1] = 2.0 ** 118
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d).bfloat16()
+    ends, q = torch.tensor(total, dtype=torch.int32) - 3, torch.randn(len(new), hq * d).bfloat16()
+    g = _gpu(cache)
+    chunks = kvc.prefill_attention_with_prefix(rows.to(DEV), new, old, list(range(len(new))), g, table.to(DEV), hq, hkv, d).cpu().double()
+    single = kvc.decode_attention(q.to(DEV), g, ends.to(DEV), table.to(DEV), hq, hkv, d).cpu().double()
+    lib.check_status()
+    at = 0
+    for i, (a, o, k) in enumerate(zip(new, old, need)):
+        pick = sorted(set(range(0, a - 3, 97)) | set(range(max(0, a - 8), a - 3)))
+        want, size = oracle.attention(rows[[at + j for j in pick], :hq * d], *cache, table[i, :k].long(), [o + j + 1 for j in pick], hq, hkv, d,
+                                      d ** -0.5)
+        err = (chunks[[at + j for j in pick]] - want).abs()
+        assert bool((err <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size).all())
+        want, size = oracle.attention(q[i:i + 1], *cache, table[i, :k].long(), [int(ends[i])], hq, hkv, d, d ** -0.5)
+        assert bool(((single[i:i + 1] - want).abs() <= BF16 * want.abs() + 2.0 ** -10 * size).all())
+        at += a
