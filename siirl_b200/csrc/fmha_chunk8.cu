@@ -578,54 +578,50 @@ using namespace sb;
 
 extern "C" int sb_kv8_chunk_seqs() { return kChunkSeqs; }
 
-// Sizes of a call's workspaces: sizes[0] 16-bit numbers for unpacked keys and values (`kv`), sizes[1] floats (0: the result is written at
-// once); sizes[2]: rows of the chunks.  The lists are the host's, of at most kChunkSeqs sequences.  -5: chunks that `rows` rows, or
-// a table of `slots` rows of `max_blocks` blocks, cannot hold.
-extern "C" int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D, int rows, int slots,
-                                  int max_blocks, long long* sizes) {
-  if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32) return -3;
+// Chunks of n sequences, at most kChunkSeqs, one behind the other in `qkv` (q heads first, row_stride apart), whose keys and values
+// are in the cache.  The lists are the host's.  sizes[0]: bytes that the workspace has to have (16-byte aligned), sizes[1]: rows of
+// the chunks, sizes[2]: kernels launched.  -5: chunks that `rows` rows, or a table of `slots` rows of `max_blocks` blocks, cannot
+// hold; -6: the workspace is too small, and nothing has been launched.
+extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, int rows, const void* codes, const float* scales, int num_blocks,
+                             const int* block_table, int slots, int max_blocks, const int* chunk, const int* prefix, const int* slot,
+                             int n, void* ws, long long ws_bytes, long long* sizes, void* out, int Hq, int Hkv, int D, float scale,
+                             int* status, cudaStream_t stream) {
+  sizes[0] = sizes[1] = sizes[2] = 0;
+  if (D != 64 && D != 128) return -2;
+  if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32 || row_stride % 8 || reinterpret_cast<uintptr_t>(qkv) % 16 || !(scale > 0.f)) return -3;
   long long sum = 0;
   for (int i = 0; i < n; ++i) {
     if (chunk[i] < 0 || prefix[i] < 0 || slot[i] < 0 || slot[i] >= slots || (long long)prefix[i] + chunk[i] > max_blocks * 64ll) return -5;
     sum += chunk[i];
   }
   if (sum > rows) return -5;
+  sizes[1] = sum;
   ChunkPlan c;
-  const int rc = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
-  sizes[0] = unpacked(c, Hkv, D) + marks_of(c, Hkv);
-  sizes[1] = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * 128 * (D + 1) : 0;
-  sizes[2] = sum;
-  return rc;
-}
-
-// Rows of n chunks, one behind the other in `qkv` (q heads first, row_stride apart), whose keys and values are in the cache.
-extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, const void* codes, const float* scales, int num_blocks,
-                             const int* block_table, int max_blocks, const int* chunk, const int* prefix, const int* slot, int n,
-                             void* kv, float* ws, void* out, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream) {
-  if (D != 64 && D != 128) return -2;
-  if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32 || row_stride % 8 || reinterpret_cast<uintptr_t>(qkv) % 16 || !(scale > 0.f)) return -3;
+  int r = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
+  if (r || c.s.tiles == 0) return r;
+  // unpacked keys and values, marks, results of shares
+  const long long kv_bytes = 2 * unpacked(c, Hkv, D), marks_bytes = 2 * marks_of(c, Hkv);
+  const long long parts = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * 128 : 0;
+  sizes[0] = kv_bytes + marks_bytes + parts * (D + 1) * 4;
+  if (sizes[0] > ws_bytes) return -6;
   static thread_local bool tl_context_bound = false;
   if (!tl_context_bound) {
     cudaFree(0);
     tl_context_bound = true;
   }
-  ChunkPlan c;
-  int r = make_chunk_plan(c, chunk, prefix, slot, n, Hq, Hkv, D);
-  if (r || c.s.tiles == 0) return r;
-  long long rows = 0;
-  for (int i = 0; i < n; ++i) rows += chunk[i];
   CUtensorMap mq, mkv;
-  r = make_tensor_map_bf16_3d(&mq, qkv, D, Hq, rows, D, row_stride, 64, Hq / Hkv, c.span);
+  r = make_tensor_map_bf16_3d(&mq, qkv, D, Hq, sum, D, row_stride, 64, Hq / Hkv, c.span);
   if (r) return r;
-  r = make_tensor_map_bf16_2d(&mkv, kv, D, 2ll * Hkv * c.s.rows, D, 64, kChunkKeys);
+  r = make_tensor_map_bf16_2d(&mkv, ws, D, 2ll * Hkv * c.s.rows, D, 64, kChunkKeys);
   if (r) return r;
-  int* marks = reinterpret_cast<int*>((__nv_bfloat16*)kv + unpacked(c, Hkv, D));
+  int* marks = reinterpret_cast<int*>((char*)ws + kv_bytes);
   r = launch_chained(D == 128 ? unpack8_kernel<128> : unpack8_kernel<64>, dim3(c.s.rows / 64, 2 * Hkv), 256, 0, stream, c.s,
-                     (const uint8_t*)codes, scales, num_blocks, block_table, max_blocks, Hkv, (__nv_bfloat16*)kv, marks);
+                     (const uint8_t*)codes, scales, num_blocks, block_table, max_blocks, Hkv, (__nv_bfloat16*)ws, marks);
   if (r) return r;
   ChunkParams p;
-  p.out = (__nv_bfloat16*)out; p.ws_o = ws;
-  p.ws_lse = ws + (long long)c.s.tiles * Hkv * c.splits * 128 * D;
+  p.out = (__nv_bfloat16*)out; p.ws_o = reinterpret_cast<float*>((char*)ws + kv_bytes + marks_bytes);
+  p.ws_lse = p.ws_o + parts * D;
+  sizes[2] = c.splits > 1 ? 3 : 2;
   p.marks = marks; p.codes = (const uint8_t*)codes; p.block_table = block_table; p.max_blocks = max_blocks;
   p.Hq = Hq; p.Hkv = Hkv; p.rep = Hq / Hkv; p.span = c.span; p.splits = c.splits;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;

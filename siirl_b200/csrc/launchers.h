@@ -158,11 +158,10 @@ int sb_kv8_decode(const void* q, long long row_stride, const void* codes, const 
                   int* counts, int B, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream);
 // ---- fmha_chunk8.cu ----
 int sb_kv8_chunk_seqs();
-int sb_kv8_chunk_sizes(const int* chunk, const int* prefix, const int* slot, int n, int Hq, int Hkv, int D, int rows, int slots,
-                       int max_blocks, long long* sizes);
-int sb_kv8_chunks(const void* qkv, long long row_stride, const void* codes, const float* scales, int num_blocks,
-                  const int* block_table, int max_blocks, const int* chunk, const int* prefix, const int* slot, int n, void* kv,
-                  float* ws, void* out, int Hq, int Hkv, int D, float scale, int* status, cudaStream_t stream);
+int sb_kv8_chunks(const void* qkv, long long row_stride, int rows, const void* codes, const float* scales, int num_blocks,
+                  const int* block_table, int slots, int max_blocks, const int* chunk, const int* prefix, const int* slot, int n,
+                  void* ws, long long ws_bytes, long long* sizes, void* out, int Hq, int Hkv, int D, float scale, int* status,
+                  cudaStream_t stream);
 // ---- fmha_decode.cu ----
 int sb_fmha_decode(const void* q, int row_stride, const void* cache, long long num_blocks, const int* seq_lens,
                    const int* block_table, int max_blocks, void* out, int B, int Hq, int Hkv, int D, float scale,

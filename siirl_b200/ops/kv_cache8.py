@@ -13,7 +13,6 @@ that lie in the same block have to follow one another; where one place is named 
 from __future__ import annotations
 
 import array
-import contextlib
 import ctypes
 import math
 from typing import NamedTuple, Optional
@@ -26,6 +25,7 @@ BLOCK = 64
 LARGEST = 448.0             # of e4m3
 HEAD_DIMS = (64, 128)       # of the kernels; the CPU statements take any
 ROWS = 1024                 # sequences of one launch of the single-token kernel
+CHUNK_BYTES = 2 ** 20       # chunks that need no more take a workspace that is kept
 
 
 class Cache8(NamedTuple):
@@ -80,11 +80,6 @@ def _check_ints(rows: torch.Tensor, *ints: torch.Tensor) -> None:
     for t in ints:
         if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
             _refuse("lengths, ids, positions and block tables are contiguous int32 tensors on the rows' device")
-
-
-def _device(index: int):
-    """Makes a device current where it is not."""
-    return contextlib.nullcontext() if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 # ---- appending ----------------------------------------------------------------------------------
@@ -174,6 +169,9 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
         if rope is not None:
             qkv.copy_(x)
         return qkv
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return append(qkv, rope, seq_ids, positions, block_table, cache, n_heads, n_kv_heads, head_dim, bias)
     if slabs is not None:
         qkv = torch.empty(T, width, dtype=torch.bfloat16, device=slabs.device)
     stride, one = qkv.stride()
@@ -181,13 +179,12 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
         _refuse("rows are bf16 numbers next to one another, from an even one on, and do not overlap")
     codes, scales = cache
     sequences, max_blocks = block_table.shape
-    with _device(dev):
-        _lib.check(_lib.get_lib().sb_kv8_append(
-            qkv.data_ptr(), stride, 0 if slabs is None else slabs.data_ptr(), T * width,
-            0 if slabs is None else slabs.shape[0], 0 if bias is None else bias.data_ptr(), 0 if pos is None else pos.data_ptr(),
-            rows, s0, s1, 0 if cos is None else table[0], 0 if cos is None else cos.data_ptr(),
-            0 if sin is None else sin.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), block_table.data_ptr(),
-            sequences, max_blocks, codes.data_ptr(), scales.data_ptr(), codes.shape[0], T, n_heads, n_kv_heads, head_dim, _lib.stream()), "sb_kv8_append")
+    _lib.check(_lib.get_lib().sb_kv8_append(
+        qkv.data_ptr(), stride, 0 if slabs is None else slabs.data_ptr(), T * width, 0 if slabs is None else slabs.shape[0],
+        0 if bias is None else bias.data_ptr(), 0 if pos is None else pos.data_ptr(), rows, s0, s1, 0 if cos is None else table[0],
+        0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(),
+        block_table.data_ptr(), sequences, max_blocks, codes.data_ptr(), scales.data_ptr(), codes.shape[0], T, n_heads, n_kv_heads,
+        head_dim, torch._C._cuda_getCurrentRawStream(dev)), "sb_kv8_append")
     return qkv
 
 
@@ -202,10 +199,32 @@ def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
     _check_ints(codes, src, dst)
     if src.shape != dst.shape or src.dim() != 1:
         _refuse("as many sources as destinations")
-    with _device(codes.get_device()):
+    with torch.cuda.device(codes.get_device()):
         _lib.check(_lib.get_lib().sb_kv8_copy_blocks(
             _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(src), _lib.ptr(dst), src.numel(), codes.shape[0], 2 * codes.shape[2],
             ctypes.c_longlong(codes[0].numel()), _lib.stream()), "sb_kv8_copy_blocks")
+
+
+# ---- workspaces ---------------------------------------------------------------------------------
+# Workspaces, and counters of pieces, which every call leaves as zeros: of each stream, whose calls come one after the other,
+# and of each stream of a capture, since a graph may be replayed beside anything.  A capture's are kept until the stream's next one,
+# so that nothing else in the graph gets their memory, and its first call clears the counters in every replay.
+_buffers: dict = {}
+
+
+def _workspace(dev: int, stream: int, floats: int, counts: int):
+    capture = _lib.get_lib().sb_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
+    held = _buffers.get((dev, stream, capture != 0))
+    if held is None or held[2] != capture or held[0].numel() < floats or held[1].numel() < counts:
+        more = (0, 0) if held is None or held[2] != capture else (held[0].numel(), held[1].numel())
+        held = (torch.empty(max(floats, more[0]), dtype=torch.float32, device=f"cuda:{dev}"),
+                torch.zeros(max(counts, more[1]), dtype=torch.int32, device=f"cuda:{dev}"), capture)
+        _buffers[dev, stream, capture != 0] = held
+    return held[:2]
+
+
+# a kernel that gave up a wait may have left counters behind
+_lib.on_status_error(_buffers.clear)
 
 
 # ---- single tokens ------------------------------------------------------------------------------
@@ -255,7 +274,7 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
     part = 2 * L.sb_kv8_decode_grid() * rows        # rows of partial results: two for each block of the grid
     entries = n_kv_heads * -(-(n_heads // n_kv_heads) // rows)
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    floats, counts = _decode_workspace(dev, stream, part * (head_dim + 4), 4 * min(B, ROWS) * entries)
+    floats, counts = _workspace(dev, stream, part * (head_dim + 4), 4 * min(B, ROWS) * entries)
     for at in range(0, B, ROWS):
         n = min(ROWS, B - at)
         _lib.check(L.sb_kv8_decode(
@@ -264,27 +283,6 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
             out.data_ptr() + 2 * at * width, floats.data_ptr(), floats.data_ptr() + 4 * part * head_dim, counts.data_ptr(), n,
             n_heads, n_kv_heads, head_dim, scale, _lib.status_word(q_rows.device).data_ptr(), stream), "sb_kv8_decode")
     return out
-
-
-# Partial results, and counters of pieces, which every call leaves as zeros: of each stream, whose calls come one after the other,
-# and of each stream of a capture, since a graph may be replayed beside anything.  A capture's are kept until the stream's next one,
-# so that nothing else in the graph gets their memory, and its first call clears the counters in every replay.
-_decode_buffers: dict = {}
-
-
-def _decode_workspace(dev: int, stream: int, floats: int, counts: int):
-    capture = _lib.get_lib().sb_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
-    held = _decode_buffers.get((dev, stream, capture != 0))
-    if held is None or held[2] != capture or held[0].numel() < floats or held[1].numel() < counts:
-        more = (0, 0) if held is None or held[2] != capture else (held[0].numel(), held[1].numel())
-        held = (torch.empty(max(floats, more[0]), dtype=torch.float32, device=f"cuda:{dev}"),
-                torch.zeros(max(counts, more[1]), dtype=torch.int32, device=f"cuda:{dev}"), capture)
-        _decode_buffers[dev, stream, capture != 0] = held
-    return held[:2]
-
-
-# a kernel that gave up a wait may have left counters behind
-_lib.on_status_error(_decode_buffers.clear)
 
 
 # ---- chunks of prompts --------------------------------------------------------------------------
@@ -319,34 +317,39 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     lists = [array.array("i", v) for v in (chunk_lens, prefix_lens, slots)]
     total = len(lists[0])
     if width != (n_heads + 2 * n_kv_heads) * head_dim or qkv.dtype is not torch.bfloat16 or block_table.dim() != 2 or \
-            total != len(lists[1]) or total != len(lists[2]):
+            total != len(lists[1]) or total != len(lists[2]) or sum(lists[0]) != rows:
         check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
+    dev = qkv.get_device()
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return chunk_attention(qkv, chunk_lens, prefix_lens, slots, cache, block_table, n_heads, n_kv_heads, head_dim)
     held, max_blocks = block_table.shape
-    out = torch.empty(rows, n_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
-    if rows == 0 and not any(lists[0]):
-        return out
+    heads = n_heads * head_dim
+    out = torch.empty(rows, heads, dtype=qkv.dtype, device=qkv.device)
     stride, one = qkv.stride()
     if one != 1 or stride % 8 or stride < width or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)      # contiguous rows may be the odd ones
         stride = qkv.shape[1]
     L = _lib.get_lib()
-    with _device(qkv.get_device()):
-        most, at = L.sb_kv8_chunk_seqs(), 0
-        sizes = array.array("q", (0, 0, 0))
-        for i in range(0, total, most):
-            n = min(most, total - i)
-            places = [v.buffer_info()[0] + 4 * i for v in lists]
-            rc = L.sb_kv8_chunk_sizes(*places, n, n_heads, n_kv_heads, head_dim, rows - at, held, max_blocks, sizes.buffer_info()[0])
-            if rc == -5 or i + n == total and at + sizes[2] != rows:
-                check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
-            _lib.check(rc, "sb_kv8_chunk_sizes")
-            # buffers of the call's own
-            ws = torch.empty(2 * sizes[0] + 4 * sizes[1], dtype=torch.uint8, device=qkv.device)
-            _lib.check(L.sb_kv8_chunks(
-                qkv.data_ptr() + 2 * at * stride, stride, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.codes.shape[0],
-                block_table.data_ptr(), max_blocks, *places, n, ws.data_ptr(), ws.data_ptr() + 2 * sizes[0],
-                out.data_ptr() + 2 * at * out.shape[1], n_heads, n_kv_heads, head_dim, 1.0 / math.sqrt(head_dim),
-                _lib.status_word(qkv.device).data_ptr(), _lib.stream()), "sb_kv8_chunks")
-            _lib.add_launches(int(sizes[1] > 0))        # shares of the keys are joined
-            at += sizes[2]
+    most, at = L.sb_kv8_chunk_seqs(), 0
+    sizes, stream = array.array("q", (0, 0, 0)), torch._C._cuda_getCurrentRawStream(dev)
+    codes, scales = cache
+    starts = [v.buffer_info()[0] for v in lists]
+    ws = _workspace(dev, stream, CHUNK_BYTES // 4, 0)[0]
+    for i in range(0, total, most):
+        n = min(most, total - i)
+        while True:
+            rc = L.sb_kv8_chunks(
+                qkv.data_ptr() + 2 * at * stride, stride, rows - at, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+                block_table.data_ptr(), held, max_blocks, starts[0] + 4 * i, starts[1] + 4 * i, starts[2] + 4 * i, n, ws.data_ptr(),
+                4 * ws.numel(), sizes.buffer_info()[0], out.data_ptr() + 2 * at * heads, n_heads, n_kv_heads, head_dim,
+                1.0 / math.sqrt(head_dim), _lib.status_word(qkv.device).data_ptr(), stream)
+            if rc != -6:
+                break
+            ws = torch.empty(sizes[0] // 4, dtype=torch.float32, device=qkv.device)     # of the call's own
+        if rc == -5:
+            check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
+        _lib.check(rc, "sb_kv8_chunks")
+        _lib.add_launches(sizes[2])
+        at += sizes[1]
     return out

@@ -24,8 +24,8 @@ _status_words: dict[int, torch.Tensor] = {}
 _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_rows": 0, "sb_ppo_token_loss": 2,
                      "sb_fmha_bwd": 3, "sb_kk_partition": 0, "sb_rmsnorm_bwd_blocks": 0, "sb_colsum_blocks": 0,
                      "sb_colsum_bf16": 2, "sb_gemm_set_pair_kernel": 0, "sb_fmha_decode_chunk_tiles": 0,
-                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_capture_id": 0, "sb_kv8_chunk_seqs": 0, "sb_kv8_chunk_sizes": 0,
-                     "sb_kv8_chunks": 2, "sb_recurrence_prefill": 2, "sb_attn_window_decode": 2, "sb_latent_decode": 2,
+                     "sb_attn_window_decode_chunks": 0, "sb_kv8_decode_grid": 0, "sb_capture_id": 0, "sb_kv8_chunk_seqs": 0,
+                     "sb_kv8_chunks": 0, "sb_recurrence_prefill": 2, "sb_attn_window_decode": 2, "sb_latent_decode": 2,
                      "sb_delta_prefill": 3}
 
 
@@ -33,7 +33,7 @@ _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_
 # then passed as plain numbers, which saves an object for each.
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 _ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
-              "sb_capture_id": "p", "sb_kv8_chunk_sizes": "pppiiiiiiip", "sb_kv8_chunks": "plppipipppipppiiifpp"}
+              "sb_capture_id": "p", "sb_kv8_chunks": "plippipiipppiplppiiifpp"}
 
 
 class _CountingLib:
@@ -42,24 +42,21 @@ class _CountingLib:
     def __init__(self, cdll: ctypes.CDLL):
         self._cdll = cdll
         self.launches = 0
-        self._cache: dict = {}
 
-    def __getattr__(self, name: str):
-        fn = self._cache.get(name)
-        if fn is None:
-            raw = getattr(self._cdll, name)
-            if name == "sb_capture_id":
-                raw.restype = ctypes.c_ulonglong
-            if name in _ARGUMENTS:
-                raw.argtypes = [_LETTERS[x] for x in _ARGUMENTS[name]]
-            k = _KERNELS_PER_CALL.get(name, 1)
+    def __getattr__(self, name: str):        # once for each name
+        raw = getattr(self._cdll, name)
+        if name == "sb_capture_id":
+            raw.restype = ctypes.c_ulonglong
+        if name in _ARGUMENTS:
+            raw.argtypes = [_LETTERS[x] for x in _ARGUMENTS[name]]
+        k = _KERNELS_PER_CALL.get(name, 1)
 
-            def counted(*args, _raw=raw, _k=k):
-                self.launches += _k
-                return _raw(*args)
+        def counted(*args):
+            self.launches += k
+            return raw(*args)
 
-            fn = counted
-            self._cache[name] = fn
+        fn = counted if k else raw
+        setattr(self, name, fn)
         return fn
 
 
