@@ -78,24 +78,22 @@ __global__ void __launch_bounds__(256) unpack8_kernel(const __grid_constant__ Ch
   if (blk >= num_blocks) blk = -1;
   const size_t at = blk < 0 ? 0 : ((size_t)blk * 2 + kv) * Hkv + (hd - kv * Hkv);
   const float scale = blk < 0 ? 0.f : scales[at];
-  const uint4* src = reinterpret_cast<const uint4*>(codes + at * 64 * D);
+  const uint2* src = reinterpret_cast<const uint2*>(codes + at * 64 * D);
   uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)hd * q.rows + row) * D);
+  constexpr int N = D / 32;      // eight numbers at a time: a warp writes whole sectors
+  uint2 c[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int u = k * 256 + threadIdx.x;
+    c[k] = blk >= 0 && u * 8 / D < left ? src[u] : make_uint2(0, 0);
+  }
   uint32_t nan = 0;
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k) {
-    const int u = k * 256 + threadIdx.x;      // 16 numbers
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (blk >= 0 && u * 16 / D < left) {
-      uint4 c = src[u];
-      const uint4 m = make_uint4(nan_codes(c.x), nan_codes(c.y), nan_codes(c.z), nan_codes(c.w));
-      c = make_uint4(c.x & ~m.x, c.y & ~m.y, c.z & ~m.z, c.w & ~m.w);
-      nan |= m.x | m.y | m.z | m.w;
-      const uint2 p0 = bf16_of(c.x, scale), p1 = bf16_of(c.y, scale), p2 = bf16_of(c.z, scale), p3 = bf16_of(c.w, scale);
-      a = make_uint4(p0.x, p0.y, p1.x, p1.y);
-      b = make_uint4(p2.x, p2.y, p3.x, p3.y);
-    }
-    dst[2 * u] = a;
-    dst[2 * u + 1] = b;
+  for (int k = 0; k < N; ++k) {
+    const uint2 m = make_uint2(nan_codes(c[k].x), nan_codes(c[k].y));
+    nan |= m.x | m.y;
+    const uint2 p0 = bf16_of(c[k].x & ~m.x, scale), p1 = bf16_of(c[k].y & ~m.y, scale);
+    dst[k * 256 + threadIdx.x] = make_uint4(p0.x, p0.y, p1.x, p1.y);
   }
   const int any = __syncthreads_or(nan != 0);
   if (threadIdx.x == 0) marks[hd * (q.rows / 64) + blockIdx.x] = any;
