@@ -22,6 +22,8 @@
 // one CTA per SM takes an equal range of it.  A range is a few pieces, each a run of tiles of one entry.  A piece that is not
 // the whole entry leaves a normalised result and its log-sum-exp in a workspace, two slots per CTA, and counts itself; whoever
 // finds that all others have joins them.  A second kernel for that would cost the host as much again as this one.
+// Up to 32 sequences, if there are few tiles, are cut instead into pieces of at most so many tiles that each CTA gets one: a second
+// piece costs a CTA about 1.6 us, a join 3, a tile 0.7 (28 / 4 heads, 300 tokens: 7.2 us whole, 11.0 in equal ranges; 32 x 1000: 11.4 and 15.3).
 // The warps:
 //   0..7   soft-max in two groups, each with an O^T and weights' references of its own.  D = 128: thread = row of the tile, the
 //          first four warps take the even tiles of the range, the others the odd ones, so that two tiles are under way.
@@ -188,6 +190,36 @@ __device__ __forceinline__ void d8_next(const int* pre, int entries, D8Piece& q,
 // ranges of the list, and the first position of one
 __device__ __forceinline__ int d8_ranges(int total, int grid) { return min(grid, max(1, total / kQ8MinTiles)); }
 __device__ __forceinline__ int d8_begin(int total, int cta, int ranges) { return (int)((long long)total * min(cta, ranges) / ranges); }
+
+// At most 32 sequences, one for each lane of a warp, of `tiles` tiles, `sum` up to the lane's: if there are few, what this CTA takes
+// in mine[0 .. 3]: list positions from, to; number of its piece, pieces of that entry.  Else mine[0] = -1.
+__device__ __noinline__ void d8_alone(int tiles, int sum, int entries, int* mine) {
+  const int lane = threadIdx.x & 31, grid = gridDim.x, cta = blockIdx.x;
+  const int most = __reduce_max_sync(0xffffffffu, tiles), all = __shfl_sync(0xffffffffu, sum, 31);
+  // the fewest tiles of a piece with which there are enough CTAs; whole entries, where they are short
+  int r = most <= 4 ? most : 2;
+  while (r > 0 && r <= 16 && (long long)__reduce_add_sync(0xffffffffu, (tiles + r - 1) / r) * entries > grid) r += r < 4 ? 1 : r < 8 ? 2 : 4;
+  if (r == 0 || r > 16 || r > (long long)all * entries / grid + 4) {
+    if (lane == 0) mine[0] = -1;
+    return;
+  }
+  const int pieces = (tiles + r - 1) / r;
+  int upto = pieces;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  const int before = (upto - pieces) * entries;
+  if (pieces && before <= cta && cta < upto * entries) {
+    const int e = (cta - before) / pieces, k = (cta - before) % pieces, first = (sum - tiles) * entries + e * tiles;
+    mine[0] = first + k * tiles / pieces;
+    mine[1] = first + (k + 1) * tiles / pieces;
+    mine[2] = k;
+    mine[3] = pieces;
+  }
+  if (lane == 31 && cta >= upto * entries) mine[0] = mine[1] = 0;
+}
 
 template <int N>
 __device__ __forceinline__ void tmem_ld_heads(uint32_t taddr, uint32_t (&r)[N]) {
@@ -368,6 +400,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
   int* s_pre = reinterpret_cast<int*>(smem + L::kPreOff);
   int* s_tot = s_pre + kQ8Rows + 1;
   int* s_len = s_tot + 32;
+  int* s_mine = s_tot + 4;      // where a single total is there: what d8_alone() writes
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int entries = p.Hkv * p.groups, rep = p.Hq / p.Hkv, per_group = (rep + p.groups - 1) / p.groups;
@@ -422,6 +455,7 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
       s_pre[b + 1] = v;
     }
     if (lane == 31) s_tot[c] = v;
+    if (p.B <= 32) d8_alone((n + L::TT - 1) / L::TT, v, entries, s_mine);
   }
   if (tid == 0) s_pre[0] = 0;
   __syncthreads();
@@ -434,7 +468,9 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
     __syncthreads();
   }
   const int total = s_pre[p.B] * entries, ranges = d8_ranges(total, gridDim.x);
-  const int begin = d8_begin(total, blockIdx.x, ranges), end = d8_begin(total, blockIdx.x + 1, ranges);
+  const bool alone = p.B <= 32 && s_mine[0] >= 0;
+  const int begin = alone ? s_mine[0] : d8_begin(total, blockIdx.x, ranges);
+  const int end = alone ? s_mine[1] : d8_begin(total, blockIdx.x + 1, ranges);
 
   if (warp == 12) {
     // ------------------------------ producer ------------------------------
@@ -1007,9 +1043,10 @@ __global__ void __launch_bounds__(kQ8Threads, 1) fmha_decode8_kernel(const __gri
           if (lane < NR) p.ws_lse[((size_t)slot * 4 + quarter) * NR + lane] = lse;
           // the range that holds position x is the last one that begins at or before it
           const int first = s_pre[q.row] * entries + q.entry * q.tiles;
-          const int c0 = (int)(((long long)(first + 1) * ranges - 1) / total), c1 = (int)(((long long)(first + q.tiles) * ranges - 1) / total);
+          const int c0 = alone ? blockIdx.x - s_mine[2] : (int)(((long long)(first + 1) * ranges - 1) / total);
+          const int c1 = alone ? c0 + s_mine[3] - 1 : (int)(((long long)(first + q.tiles) * ranges - 1) / total);
           d8_join<D, NR>(p.ws_o + d, p.ws_lse + quarter * NR, p.counts + ((size_t)q.row * entries + q.entry) * 4 + quarter, c0, c1,
-                         d8_begin(total, c0, ranges) >= first ? 0 : 1, left, orow);
+                         alone || d8_begin(total, c0, ranges) >= first ? 0 : 1, left, orow);
         }
       }
       cur += q.n;

@@ -576,3 +576,9 @@ def test_attention_does_not_feel_large_values_that_it_does_not_see(hq, hkv, d, n
         want, size = oracle.attention(q[i:i + 1], *cache, table[i, :k].long(), [int(ends[i])], hq, hkv, d, d ** -0.5)
         assert bool(((single[i:i + 1] - want).abs() <= BF16 * want.abs() + 2.0 ** -10 * size).all())
         at += a
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (32, 1, 64), (32, 1, 128)])
+@pytest.mark.parametrize("scale", [0.0, -0.07])
+def test_decode_attention_with_scales_of_any_sign(hq, hkv, d, scale):
+    _check_decode(*_decode([700, 1, 0, 129], hq, hkv, d, 12), hq, hkv, d, scale)
