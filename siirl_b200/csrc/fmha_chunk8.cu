@@ -143,10 +143,16 @@ struct ChunkSmem {
   static constexpr int kTotal = kBarOff + (9 + 2 * kStages) * 8 + 16;
 };
 
-// two of 2^x: see above.  0 from -127 down: a weight of what a row does not see times a large value would be seen
+// the larger one, NaN where one is NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// two of 2^x: see above.  0 from -127 down: a weight of what a row does not see times a large value would be seen.  NaN stays NaN
 __device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
   const float2 big = make_float2(12582912.f, 12582912.f), small = make_float2(-12582912.f, -12582912.f);      // 1.5 * 2^23
   const float2 t = add_f32x2(x, big), n = add_f32x2(t, small), minus = make_float2(-1.f, -1.f);
   const float2 f = fma_f32x2(n, minus, x);
@@ -406,8 +412,9 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (ok) {
       tc_fence_after();
       const bool row_valid = at < p.span && qpos < total;
-      const float l = m_ref == -INFINITY ? 0.f : (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
-      const float inv_l = l != 0.f ? 1.f / l : 0.f;
+      // 0: all scores are -inf, of a share's keys that the row does not see, or of all its keys, where 0 / 0 is soft-max's answer.
+      // Scores that are NaN do not raise the reference, but make the sum NaN
+      const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y), inv_l = 1.f / l;
       const size_t part = (((size_t)tile * p.Hkv + g) * p.splits + split) * 128 + row;
       const size_t out_row = (size_t)seqs.q_row[seq] + (row_valid ? qpos - prefix : 0);
       __nv_bfloat16* orow = p.out + out_row * (size_t)(p.Hq * D) + (size_t)(g * p.rep + head) * D;
@@ -437,7 +444,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         }
       }
-      if (p.splits > 1 && row_valid) p.ws_lse[part] = l != 0.f ? m_ref + log2f(l) : -INFINITY;      // NaN stays NaN
+      if (p.splits > 1 && row_valid) p.ws_lse[part] = l == 0.f ? -INFINITY : l != l ? l : m_ref + log2f(l);
     }
   }
   tc_fence_before();
@@ -490,7 +497,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant_
       acc[k].x += e * o.x; acc[k].y += e * o.y; acc[k].z += e * o.z; acc[k].w += e * o.w;
     }
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const float inv = 1.f / sum;      // every row sees a token: a sum of 0 is one of scores that are all -inf, and the result NaN
   __nv_bfloat16* out = p.out + (size_t)(seqs.q_row[seq] + pos) * (p.Hq * D) + (size_t)(g * p.rep + row - at * p.rep) * D;
 #pragma unroll
   for (int k = 0; k < N; ++k)

@@ -582,3 +582,67 @@ def test_attention_does_not_feel_large_values_that_it_does_not_see(hq, hkv, d, n
 @pytest.mark.parametrize("scale", [0.0, -0.07])
 def test_decode_attention_with_scales_of_any_sign(hq, hkv, d, scale):
     _check_decode(*_decode([700, 1, 0, 129], hq, hkv, d, 12), hq, hkv, d, scale)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (9, 1, 64)])
+@pytest.mark.parametrize("new,old", [((5,), (100,)), ((5,), (3000,)), ((300, 40), (4000, 0))])
+def test_queries_that_are_not_finite_spoil_their_head_alone(hq, hkv, d, new, old):
+    """NaN and infinities in some heads of some rows, keys split over several blocks or not: these heads are NaN, as soft-max has
+    it, and all others hold the bounds of _check_prefix and _check_decode."""
+    total = [a + b for a, b in zip(new, old)]
+    need = [(n + 63) // 64 for n in total]
+    cache = _random_cache(sum(need), hkv, d)
+    table, first = torch.full((len(new), max(need)), -1, dtype=torch.int32), 0
+    for i, k in enumerate(need):
+        table[i, :k] = torch.arange(first, first + k)
+        first += k
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d).bfloat16()
+    bad = torch.zeros(len(rows), hq, dtype=torch.bool)
+    for r, h, at, x in ((0, 0, 5, math.nan), (1, hq - 1, 0, math.inf), (3, 1, d - 1, -math.inf), (len(rows) - 1, hq // 2, 9, math.nan)):
+        rows[r, h * d + at] = x
+        bad[r, h] = True
+    bad = bad.repeat_interleave(d, 1)
+    g = _gpu(cache)
+    out = kvc.prefill_attention_with_prefix(rows.to(DEV), new, old, list(range(len(new))), g, table.to(DEV), hq, hkv, d).cpu().double()
+    assert torch.equal(out.isnan(), bad)
+    at = 0
+    for i, (a, o, k) in enumerate(zip(new, old, need)):
+        pick = sorted({0, 1, 2, 3, 4, a // 2, a - 1})
+        good = ~bad[[at + j for j in pick]]
+        want, size = oracle.attention(rows[[at + j for j in pick], :hq * d], *cache, table[i, :k].long(), [o + j + 1 for j in pick],
+                                      hq, hkv, d, d ** -0.5)
+        err = (out[[at + j for j in pick]] - want).abs()
+        assert bool((err <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size)[good].all())
+        at += a
+    q, ends = rows[[0, 2][:len(new)]], torch.tensor(total, dtype=torch.int32)      # one with a NaN, one without
+    out = kvc.decode_attention(q.to(DEV), g, ends.to(DEV), table.to(DEV), hq, hkv, d).cpu().double()
+    lib.check_status()
+    assert torch.equal(out.isnan(), bad[[0, 2][:len(new)]])
+    for i, (n, k) in enumerate(zip(total, need)):
+        want, size = oracle.attention(q[i:i + 1, :hq * d], *cache, table[i, :k].long(), [n], hq, hkv, d, d ** -0.5)
+        x = cache.dequantize(table[i, :k].long(), torch.float64)[:, 1].transpose(0, 1).reshape(hkv, -1, d)[:, :n]
+        least = 2.0 ** -36 * x.abs().sum(1).repeat_interleave(hq // hkv, 0).reshape(-1)
+        ok = (out[i] - want[0]).abs() <= least + BF16 * want[0].abs() + 2.0 ** -10 * size[0]
+        assert bool(ok[~out[i].isnan()].all())
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 128), (2, 1, 64)])
+@pytest.mark.parametrize("old", [60, 3000])
+@pytest.mark.parametrize("largest", [(), (6, 7), (2, 6), (0,)])
+def test_an_infinite_query_is_nan_whichever_keys_it_meets(hq, hkv, d, old, largest):
+    """Scores that are infinite: all of them -inf (``largest`` empty), or +inf for the tokens whose number modulo 8 is named."""
+    need = (old + 1 + 63) // 64
+    cache = _random_cache(need, hkv, d)
+    key = torch.full((64,), -3.0)
+    for i in largest:
+        key[i::8] = 3.0
+    cache.codes[:, 0, 0, :, 0] = key.to(torch.float8_e4m3fn)
+    table = torch.arange(need, dtype=torch.int32)[None]
+    rows = torch.zeros(1, (hq + 2 * hkv) * d)
+    rows[0, 0] = math.inf
+    g = _gpu(cache)
+    out = kvc.prefill_attention_with_prefix(rows.bfloat16().to(DEV), [1], [old], [0], g, table.to(DEV), hq, hkv, d)
+    assert bool(out[:, :d].isnan().all()) and bool(torch.isfinite(out[:, d:]).all())
+    one = kvc.decode_attention(rows.bfloat16().to(DEV), g, torch.tensor([old + 1], dtype=torch.int32, device=DEV), table.to(DEV), hq, hkv, d)
+    assert bool(one[:, :d].isnan().all()) and bool(torch.isfinite(one[:, d:]).all())
+    lib.check_status()
