@@ -15,6 +15,7 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -206,20 +207,25 @@ def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
 
 
 # ---- workspaces ---------------------------------------------------------------------------------
-# Workspaces, and counters of pieces, which every call leaves as zeros: of each stream, whose calls come one after the other,
-# and of each stream of a capture, since a graph may be replayed beside anything.  A capture's are kept until the stream's next one,
-# so that nothing else in the graph gets their memory, and its first call clears the counters in every replay.
+# Workspaces, and counters of pieces, which every call leaves as zeros: of each stream, whose kernels run one after the other,
+# and of each stream of a capture, since a graph may be replayed beside anything.  A capture's are kept until the stream's next
+# one, so that nothing else in the graph gets their memory, and its first call clears the counters in every replay.
+# Threads may share a stream.  A launch for single tokens needs nothing of another one.  A call for chunks launches several kernels
+# that hand data on through the workspace, which nobody else may write in between: it is the chunks' own, and their calls go to the
+# library one at a time.
 _buffers: dict = {}
+_chunk_calls = threading.Lock()
 
 
-def _workspace(dev: int, stream: int, floats: int, counts: int):
+def _workspace(dev: int, stream: int, floats: int, counts: int, use: str = "pieces"):
     capture = _lib.get_lib().sb_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
-    held = _buffers.get((dev, stream, capture != 0))
+    key = dev, stream, capture != 0, use
+    held = _buffers.get(key)
     if held is None or held[2] != capture or held[0].numel() < floats or held[1].numel() < counts:
         more = (0, 0) if held is None or held[2] != capture else (held[0].numel(), held[1].numel())
         held = (torch.empty(max(floats, more[0]), dtype=torch.float32, device=f"cuda:{dev}"),
                 torch.zeros(max(counts, more[1]), dtype=torch.int32, device=f"cuda:{dev}"), capture)
-        _buffers[dev, stream, capture != 0] = held
+        _buffers[key] = held
     return held[:2]
 
 
@@ -335,21 +341,22 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     sizes, stream = array.array("q", (0, 0, 0)), torch._C._cuda_getCurrentRawStream(dev)
     codes, scales = cache
     starts = [v.buffer_info()[0] for v in lists]
-    ws = _workspace(dev, stream, CHUNK_BYTES // 4, 0)[0]
-    for i in range(0, total, most):
-        n = min(most, total - i)
-        while True:
-            rc = L.sb_kv8_chunks(
-                qkv.data_ptr() + 2 * at * stride, stride, rows - at, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
-                block_table.data_ptr(), held, max_blocks, starts[0] + 4 * i, starts[1] + 4 * i, starts[2] + 4 * i, n, ws.data_ptr(),
-                4 * ws.numel(), sizes.buffer_info()[0], out.data_ptr() + 2 * at * heads, n_heads, n_kv_heads, head_dim,
-                1.0 / math.sqrt(head_dim), _lib.status_word(qkv.device).data_ptr(), stream)
-            if rc != -6:
-                break
-            ws = torch.empty(sizes[0] // 4, dtype=torch.float32, device=qkv.device)     # of the call's own
-        if rc == -5:
-            check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
-        _lib.check(rc, "sb_kv8_chunks")
-        _lib.add_launches(sizes[2])
-        at += sizes[1]
+    with _chunk_calls:
+        ws = _workspace(dev, stream, CHUNK_BYTES // 4, 0, "chunks")[0]
+        for i in range(0, total, most):
+            n = min(most, total - i)
+            while True:
+                rc = L.sb_kv8_chunks(
+                    qkv.data_ptr() + 2 * at * stride, stride, rows - at, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+                    block_table.data_ptr(), held, max_blocks, starts[0] + 4 * i, starts[1] + 4 * i, starts[2] + 4 * i, n,
+                    ws.data_ptr(), 4 * ws.numel(), sizes.buffer_info()[0], out.data_ptr() + 2 * at * heads, n_heads, n_kv_heads,
+                    head_dim, 1.0 / math.sqrt(head_dim), _lib.status_word(qkv.device).data_ptr(), stream)
+                if rc != -6:
+                    break
+                ws = torch.empty(sizes[0] // 4, dtype=torch.float32, device=qkv.device)     # of the call's own
+            if rc == -5:
+                check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
+            _lib.check(rc, "sb_kv8_chunks")
+            _lib.add_launches(sizes[2])
+            at += sizes[1]
     return out

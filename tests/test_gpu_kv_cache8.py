@@ -646,3 +646,39 @@ def test_an_infinite_query_is_nan_whichever_keys_it_meets(hq, hkv, d, old, large
     one = kvc.decode_attention(rows.bfloat16().to(DEV), g, torch.tensor([old + 1], dtype=torch.int32, device=DEV), table.to(DEV), hq, hkv, d)
     assert bool(one[:, :d].isnan().all()) and bool(torch.isfinite(one[:, d:]).all())
     lib.check_status()
+
+
+def test_threads_on_one_stream():
+    """Chunks and single tokens of four threads, all on the default stream."""
+    import threading
+    hq, hkv, d = 14, 2, 64
+    lists, calls = [([9], [130]), ([5], [700]), ([64, 1], [1, 300])], []
+    for new, old in lists:
+        total = [a + b for a, b in zip(new, old)]
+        need = [(n + 63) // 64 for n in total]
+        g, table, first = _gpu(_random_cache(sum(need), hkv, d)), torch.full((len(new), max(need)), -1, dtype=torch.int32), 0
+        for i, k in enumerate(need):
+            table[i, :k] = torch.arange(first, first + k)
+            first += k
+        q, table = torch.randn(sum(new), (hq + 2 * hkv) * d).bfloat16().to(DEV), table.to(DEV)
+        ends = torch.tensor(total, dtype=torch.int32, device=DEV)
+        calls.append(lambda q=q, new=new, old=old, g=g, table=table: kvc.prefill_attention_with_prefix(
+            q, new, old, list(range(len(new))), g, table, hq, hkv, d))
+        calls.append(lambda q=q[:len(new)], ends=ends, g=g, table=table: kvc.decode_attention(q, g, ends, table, hq, hkv, d))
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(shift):
+        for i in range(300):
+            j = (i + shift) % len(calls)
+            got = calls[j]()
+            if i % 7 == shift and not torch.equal(got, want[j]):
+                wrong.append((shift, i, j))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    lib.check_status()
+    assert not wrong

@@ -135,6 +135,53 @@ def test_refusals():
             call()
 
 
+def test_chunk_calls_of_threads_do_not_meet_in_a_workspace(monkeypatch):
+    """A call for chunks launches kernels that hand data on through a workspace: while one is in the library, no other call may be
+    there with the same memory, nor may single tokens have it."""
+    import ctypes
+    import threading
+    import time
+    from siirl_b200.ops import kv_cache8
+    inside, met, rows = {}, [], 3
+
+    class Library:
+        def sb_kv8_chunk_seqs(self):
+            return 48
+
+        def sb_kv8_chunks(self, *args):
+            kept, sizes = args[13], ctypes.cast(args[15], ctypes.POINTER(ctypes.c_longlong))
+            met.append(inside.get(kept, 0))
+            inside[kept] = inside.get(kept, 0) + 1
+            time.sleep(0.02)
+            inside[kept] -= 1
+            sizes[1], sizes[2] = rows, 2
+            return 0
+    monkeypatch.setattr(kv_cache8._lib, "get_lib", Library)
+    monkeypatch.setattr(kv_cache8._lib, "add_launches", lambda n: None)
+    monkeypatch.setattr(kv_cache8._lib, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    for name, value in (("_cuda_getDevice", -1), ("_cuda_getCurrentRawStream", 0), ("_cuda_isCurrentStreamCapturing", False)):
+        monkeypatch.setattr(torch._C, name, lambda *args, value=value: value)
+    real = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *size, device=None, **kw: real(*size, **kw))
+    real_zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *size, device=None, **kw: real_zeros(*size, **kw))
+    monkeypatch.setattr(kv_cache8, "_buffers", {})
+    hq, hkv, d = 4, 2, 64
+    cache, table = Cache8.zeros(4, hkv, d), real_zeros(1, 2, dtype=torch.int32)
+    qkv = real_zeros(rows, (hq + 2 * hkv) * d, dtype=torch.bfloat16)
+    threads = [threading.Thread(target=lambda: [kv_cache8.chunk_attention(qkv, [rows], [5], [0], cache, table, hq, hkv, d)
+                                                for _ in range(4)]) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(met) == 12 and not any(met)
+    # the buffers that are kept for the stream: that of the chunks, and another one for single tokens
+    kv_cache8._workspace(-1, 0, 100, 8)
+    places = [held[0].data_ptr() for held in kv_cache8._buffers.values()]
+    assert len(set(places)) == 2 and set(places) > set(inside)
+
+
 # ---- the rollout engine -------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def tiny():
