@@ -602,12 +602,9 @@ class DecoderLM(nn.Module):
             qkv = kvc.rope_kv_append(qkv if qkv is not None else layer.qkv_pre_rope(x), rp32, rope[0], rope[1],
                                      cfg.mrope_section, seq_ids, pos32, block_table, cache[li], cfg.num_heads,
                                      cfg.num_kv_heads, cfg.head_dim, bias)
-            if prefill_info is not None and prefix_lens is not None and any(int(p) > 0 for p in prefix_lens):
-                # chunked prefill / prefix-cache hit: the chunk attends to the tokens already in the cache as well
-                a = kvc.prefill_attention_with_prefix(qkv, prefill_info.seqlens, prefix_lens, prefill_slots, cache[li],
-                                                      block_table, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim)
-            elif prefill_info is not None:
-                a = attention_packed(qkv, prefill_info, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, causal=True)
+            if prefill_info is not None:
+                a = kvc.prefill_attention(qkv, prefill_info, prefix_lens, prefill_slots, cache[li], block_table,
+                                          cfg.num_heads, cfg.num_kv_heads, cfg.head_dim)
             else:
                 a = kvc.decode_attention(qkv, cache[li], seq_lens, block_table, cfg.num_heads, cfg.num_kv_heads,
                                          cfg.head_dim)

@@ -32,6 +32,14 @@ class SeqInfo:
         self._tiles = {}
         self._cu_dev = None
         self._pos = None
+        self._parts = {}
+
+    def part(self, which: Sequence[int]) -> "SeqInfo":
+        """The same of some of the sequences, packed by themselves; kept for the layers to come."""
+        which = tuple(which)
+        if which not in self._parts:
+            self._parts[which] = SeqInfo([self.seqlens[i] for i in which], device=self.device)
+        return self._parts[which]
 
     @property
     def cu_seqlens(self) -> torch.Tensor:

@@ -176,6 +176,36 @@ def decode_attention(q_rows: torch.Tensor, cache_layer: torch.Tensor, seq_lens: 
     return out
 
 
+def prefill_attention(qkv: torch.Tensor, info, prefix_lens, slots, cache_layer: torch.Tensor, block_table: torch.Tensor,
+                      n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """Attention of a prefill batch: ``info`` (:class:`~siirl_b200.ops.attention.SeqInfo`) has the new rows, ``prefix_lens`` the
+    earlier tokens of each sequence (None: of none), ``slots`` their places in the table.  Sequences without earlier tokens
+    attend to the keys and values of their rows, the others to the cache.  What a 16-bit cache holds are the rows' own, so one call
+    takes both kinds; an 8-bit cache has rounded them, and each kind gets a call, so that no prompt's result depends on what it was
+    admitted with."""
+    from .attention import attention_packed
+    shape = (n_heads, n_kv_heads, head_dim)
+    kinds = ([], [])
+    for i in range(len(info.seqlens)):
+        kinds[prefix_lens is not None and int(prefix_lens[i]) > 0].append(i)
+    whole, behind = kinds
+    if not behind:
+        return attention_packed(qkv, info, *shape, causal=True)
+    if not whole or not isinstance(cache_layer, Cache8):
+        return prefill_attention_with_prefix(qkv, info.seqlens, prefix_lens, slots, cache_layer, block_table, *shape)
+    parts, out = qkv.split(info.seqlens), [None] * len(info.seqlens)
+    for kind in kinds:
+        own, rows = info.part(kind), torch.cat([parts[i] for i in kind])
+        if kind is whole:
+            a = attention_packed(rows, own, *shape, causal=True)
+        else:
+            a = prefill_attention_with_prefix(rows, own.seqlens, [prefix_lens[i] for i in kind], [slots[i] for i in kind],
+                                              cache_layer, block_table, *shape)
+        for i, x in zip(kind, a.split(own.seqlens)):
+            out[i] = x
+    return torch.cat(out)
+
+
 def prefill_attention_with_prefix(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache_layer: torch.Tensor,
                                   block_table: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int) -> torch.Tensor:
     """Causal attention of freshly projected chunk rows against (cached prefix + chunk) -- chunked prefill and prompts

@@ -682,3 +682,26 @@ def test_threads_on_one_stream():
         t.join()
     lib.check_status()
     assert not wrong
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64)])
+def test_prefill_attention_of_mixed_batches(hq, hkv, d):
+    """Sequences without earlier tokens attend to the rows' own keys and values, the others to the cache.  Bounds: _check_prefix."""
+    from siirl_b200.ops.attention import SeqInfo
+    new, old, slots = [5, 170, 1, 90], [100, 0, 700, 0], [2, 1, 0, 3]
+    cache = _random_cache(30, hkv, d)
+    table = torch.randperm(28).to(torch.int32).view(4, 7).repeat(1, 2).contiguous()
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d).bfloat16()
+    info = SeqInfo(new, device=torch.device(DEV))
+    out = kvc.prefill_attention(rows.to(DEV), info, old, slots, _gpu(cache), table.to(DEV), hq, hkv, d).cpu().double()
+    lib.check_status()
+    for n, o, slot, got, x in zip(new, old, slots, out.split(new), rows.split(new)):
+        k = -(-(n + o) // 64)
+        held, blocks = cache, table[slot, :k].long()
+        if o == 0:      # a cache of the rows themselves, without rounding
+            kv = torch.zeros(k * 64, 2, hkv, d, dtype=torch.float64)
+            kv[:n] = x[:, hq * d:].double().view(n, 2, hkv, d)
+            held, blocks = Cache8(kv.view(k, 64, 2, hkv, d).permute(0, 2, 3, 1, 4), torch.ones(k, 2, hkv)), torch.arange(k)
+        pick = sorted({0, n // 2, n - 1})
+        want, size = oracle.attention(x[pick, :hq * d], *held, blocks, [o + j + 1 for j in pick], hq, hkv, d, d ** -0.5)
+        assert bool(((got[pick] - want).abs() <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size).all())

@@ -242,6 +242,51 @@ def test_engine_chunks_and_reuses_prompts(tiny):
     assert all(bool(torch.isfinite(x.codes.float()).all()) for x in eng.cache)
 
 
+def test_whole_prompts_attend_to_unrounded_keys_whatever_they_are_admitted_with(tiny):
+    """A prompt that is prefilled whole: alone, and in one batch with prompts whose first blocks the prefix cache holds, before and
+    behind it.  These in turn get what they get without it."""
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    sp = SamplingParams(n=1, temperature=0.0, max_new_tokens=3, ignore_eos=True)
+    kw = dict(max_num_seqs=8, max_model_len=256, num_blocks=40, kv_cache_dtype="fp8")
+    known, whole = [list(range(7, 7 + n)) for n in (150, 70)], list(range(30, 130))
+    again = [p + [3, 4] for p in known]
+    alone = RolloutEngine(tiny, **kw).generate([whole], sp)[0]
+    eng = RolloutEngine(tiny, **kw)
+    eng.generate(known, sp)
+    reused = eng.generate(again, sp)
+    eng = RolloutEngine(tiny, **kw)
+    eng.generate(known, sp)
+    mixed = eng.generate([again[0], whole, again[1]], sp)
+    assert eng.stats["prefix_cache_hit_tokens"] == 128 + 64
+    for got, want in zip(mixed, (reused[0], alone, reused[1])):
+        assert got.token_ids == want.token_ids
+        assert all(abs(a - b) < 1e-5 for a, b in zip(got.logprobs, want.logprobs))
+
+
+def test_prefill_attention_of_mixed_batches():
+    hq, hkv, d = 4, 2, 32
+    cache = Cache8((torch.randn(9, 2, hkv, 64, d) * 50).clamp(-400, 400).to(torch.float8_e4m3fn), 2.0 ** torch.randint(-9, -4, (9, 2, hkv)).float())
+    table = torch.tensor([[0, 3, 5], [1, 6, -1], [2, 4, 8], [7, -1, -1]], dtype=torch.int32)
+    from siirl_b200.ops.attention import SeqInfo, attention_packed
+    new, old, slots = [5, 70, 1, 9], [100, 0, 64, 0], [2, 1, 0, 3]
+    rows = torch.randn(sum(new), (hq + 2 * hkv) * d)
+    got = kvc.prefill_attention(rows, SeqInfo(new), old, slots, cache, table, hq, hkv, d).split(new)
+    parts = rows.split(new)
+    for i in range(4):
+        if old[i]:
+            want = kvc.prefill_attention_with_prefix(parts[i], [new[i]], [old[i]], [slots[i]], cache, table, hq, hkv, d)
+        else:
+            want = attention_packed(parts[i], SeqInfo([new[i]]), hq, hkv, d)
+        assert torch.allclose(got[i], want, rtol=1e-5, atol=1e-6)
+    # a cache of the rows' type: as before, in one call
+    plain = cache.dequantize(torch.arange(9))
+    assert torch.equal(kvc.prefill_attention(rows, SeqInfo(new), old, slots, plain, table, hq, hkv, d),
+                       kvc.prefill_attention_with_prefix(rows, new, old, slots, plain, table, hq, hkv, d))
+    for none in (None, [0, 0, 0, 0]):
+        assert torch.equal(kvc.prefill_attention(rows, SeqInfo(new), none, None, cache, table, hq, hkv, d),
+                           attention_packed(rows, SeqInfo(new), hq, hkv, d))
+
+
 def test_engine_refusals(tiny):
     from siirl_b200.engine.rollout.native_engine import RolloutEngine
     with pytest.raises(ValueError, match="kv_cache_dtype"):
