@@ -77,3 +77,40 @@ def attention(q, codes, scales, blocks, seen, hq, hkv, d, scale):
                 w = torch.softmax(k[:n] @ q[i, h * d:(h + 1) * d].double() * scale, 0)
                 out[i, h], size[i, h] = w @ v[:n], w @ v[:n].abs()
     return out.view(len(q), hq * d), size.view(len(q), hq * d)
+
+
+def engine_by_hand(model, logits, ids, cuts, steps):
+    """Greedy tokens and log-probabilities of one prompt, as a rollout engine with an 8-bit cache has to get them: the prompt in
+    portions that end at ``cuts``, each behind the ones before, then token by token, on a cache of its own."""
+    from siirl_b200.ops.attention import SeqInfo
+    from siirl_b200.ops.kv_cache import Cache8
+    cfg, dev = model.cfg, next(model.parameters()).device
+    n = -(-(len(ids) + steps) // 64)
+    cache = [Cache8.zeros(n + 1, cfg.num_kv_heads, cfg.head_dim, dev) for _ in range(cfg.num_layers)]
+    table = torch.arange(n, 0, -1, dtype=torch.int32, device=dev)[None]
+    a = 0
+    for b in cuts:
+        info, seq = SeqInfo([b - a], device=dev), torch.zeros(b - a, dtype=torch.int32, device=dev)
+        at = {} if a == 0 else {"prefix_lens": [a], "prefill_slots": [0]}
+        hidden = model.forward_cached(torch.tensor(ids[a:b], device=dev), info.positions + a, cache, table, seq, prefill_info=info, **at)
+        a = b
+    tokens, probs, one = [], [], torch.zeros(1, dtype=torch.int32, device=dev)
+    for n in range(len(ids), len(ids) + steps):
+        z = logits(hidden[-1:])[0].detach().double()
+        tokens.append(int(z.argmax()))
+        probs.append(float(torch.log_softmax(z, 0)[tokens[-1]]))
+        hidden = model.forward_cached(torch.tensor(tokens[-1:], device=dev), one + n, cache, table, one, seq_lens=one + n + 1)
+    return tokens, probs
+
+
+def record_cuts(engine):
+    """{number of the prompt: (from, to) of its portions} of the prefills to come."""
+    cuts, prefill = {}, engine._prefill
+
+    def recorded(seqs, chunks, starts=None, *args, **kw):
+        for i, c in enumerate(chunks):
+            a = starts[i] if starts is not None else 0
+            cuts.setdefault(seqs[i].prompt_index, []).append((a, a + len(c)))
+        return prefill(seqs, chunks, starts, *args, **kw)
+    engine._prefill = recorded
+    return cuts

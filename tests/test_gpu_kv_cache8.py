@@ -705,3 +705,33 @@ def test_prefill_attention_of_mixed_batches(hq, hkv, d):
         pick = sorted({0, n // 2, n - 1})
         want, size = oracle.attention(x[pick, :hq * d], *held, blocks, [o + j + 1 for j in pick], hq, hkv, d, d ** -0.5)
         assert bool(((got[pick] - want).abs() <= BF16 * want.abs() + (BF16 + 2.0 ** -10) * size).all())
+
+
+def test_engine_chunks_and_reused_blocks_follow_from_the_cache():
+    """One prompt at a time, so that the same kernels run on as many rows: in portions, and behind blocks of the prefix cache, with the
+    tokens that the same portions give by hand.  Log-probabilities: of 32-bit logits, whose sums over the vocabulary may be in
+    another order."""
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    from siirl_b200.models.config import get_config
+    from siirl_b200.models.decoder import build_model
+    model, steps = build_model(get_config("tiny-gpu"), dtype=torch.bfloat16, device=DEV, seed=1), 20
+    sp = SamplingParams(n=1, temperature=0.0, max_new_tokens=steps, ignore_eos=True)
+    kw = dict(max_num_seqs=1, max_model_len=512, num_blocks=32, use_cuda_graph=False, kv_cache_dtype="fp8")
+    eng = RolloutEngine(model, **kw)
+    for n in (130, 70):
+        prompt = list(range(5, 5 + n))
+        eng.generate([prompt], sp)
+        prompt, old = prompt + [9, 8], n // 64 * 64
+        kept, cuts = eng._prefill, oracle.record_cuts(eng)
+        got = eng.generate([prompt], sp)[0]
+        eng._prefill = kept
+        assert cuts == {0: [(old, n + 2)]}
+        want, probs = oracle.engine_by_hand(model, eng._logits, prompt, [old, n + 2], steps)
+        assert got.token_ids == want and all(abs(a - b) < 1e-4 for a, b in zip(got.logprobs, probs))
+    eng = RolloutEngine(model, max_num_batched_tokens=64, enable_chunked_prefill=True, **kw)
+    cuts = oracle.record_cuts(eng)
+    got = eng.generate([prompt], sp)[0]
+    assert cuts == {0: [(0, 64), (64, 72)]}
+    want, probs = oracle.engine_by_hand(model, eng._logits, prompt, [64, 72], steps)
+    assert got.token_ids == want and all(abs(a - b) < 1e-4 for a, b in zip(got.logprobs, probs))
+    lib.check_status()

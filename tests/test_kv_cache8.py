@@ -242,6 +242,32 @@ def test_engine_chunks_and_reuses_prompts(tiny):
     assert all(bool(torch.isfinite(x.codes.float()).all()) for x in eng.cache)
 
 
+def test_engine_chunks_and_reused_blocks_follow_from_the_cache(tiny):
+    """Prompts in portions, and prompts whose first blocks come from the prefix cache: tokens and log-probabilities are those of the
+    same portions recomputed by hand, on a cache that has held nothing else."""
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    prompts, steps = [list(range(7, 7 + n)) for n in (150, 70)], 5
+    sp = SamplingParams(n=1, temperature=0.0, max_new_tokens=steps, ignore_eos=True)
+    kw = dict(max_num_seqs=8, max_model_len=256, num_blocks=40, kv_cache_dtype="fp8")
+    eng = RolloutEngine(tiny, **kw)
+    eng.generate(prompts, sp)
+    again = [p + [3, 4] for p in prompts]
+    cuts = oracle.record_cuts(eng)
+    reused = eng.generate(again, sp)
+    assert cuts == {0: [(128, 152)], 1: [(64, 72)]}
+    for i, got in enumerate(reused):
+        want, probs = oracle.engine_by_hand(tiny, eng._logits, again[i], [cuts[i][0][0], len(again[i])], steps)
+        assert got.token_ids == want and all(abs(a - b) < 1e-5 for a, b in zip(got.logprobs, probs))
+    eng = RolloutEngine(tiny, max_num_batched_tokens=64, enable_chunked_prefill=True, **kw)
+    cuts = oracle.record_cuts(eng)
+    chunked = eng.generate(prompts, sp)
+    assert len(cuts[0]) == 3 and len(cuts[1]) == 2
+    for i, got in enumerate(chunked):
+        assert [a for a, _ in cuts[i]] == [0] + [b for _, b in cuts[i][:-1]]
+        want, probs = oracle.engine_by_hand(tiny, eng._logits, prompts[i], [b for _, b in cuts[i]], steps)
+        assert got.token_ids == want and all(abs(a - b) < 1e-5 for a, b in zip(got.logprobs, probs))
+
+
 def test_whole_prompts_attend_to_unrounded_keys_whatever_they_are_admitted_with(tiny):
     """A prompt that is prefilled whole: alone, and in one batch with prompts whose first blocks the prefix cache holds, before and
     behind it.  These in turn get what they get without it."""
