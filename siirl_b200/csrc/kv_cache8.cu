@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t codes, float ratio) {
 
 struct Append8Params {
   __nv_bfloat16* qkv;      // [T, row_stride]: heads q | k | v
-  int row_stride;
+  long long row_stride;
   const float* slabs;      // the projection's partial sums [splits, T, heads * D], slab_stride floats apart, or null
   long long slab_stride;
   int splits;
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(256) copy8_blocks_kernel(uint8_t* codes, float
 using namespace sb;
 
 // Rows of one cache block have to follow one another.  rope_pos null: nothing is rotated.
-extern "C" int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long long slab_stride, int splits,
+extern "C" int sb_kv8_append(void* qkv, long long row_stride, const float* slabs, long long slab_stride, int splits,
                              const void* bias, const int* rope_pos, int pos_rows, int sec0, int sec1, int table_rows,
                              const float* cos_tab, const float* sin_tab, const int* seq_ids, const int* cache_pos,
                              const int* block_table, int sequences, int max_blocks, void* codes, float* scales,

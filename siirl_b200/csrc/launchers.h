@@ -143,7 +143,7 @@ int sb_rope_kv_append(void* qkv, int row_stride, const float* slabs, long long s
 int sb_kv_copy_blocks(void* cache, const int* src, const int* dst, int n_pairs, long long block_elems,
                       cudaStream_t stream);
 // ---- kv_cache8.cu: paged cache of e4m3 codes [num_blocks, 2, Hkv, 64, D] with scales [num_blocks, 2, Hkv] ----
-int sb_kv8_append(void* qkv, int row_stride, const float* slabs, long long slab_stride, int splits, const void* bias,
+int sb_kv8_append(void* qkv, long long row_stride, const float* slabs, long long slab_stride, int splits, const void* bias,
                   const int* rope_pos, int pos_rows, int sec0, int sec1, int table_rows, const float* cos_tab,
                   const float* sin_tab, const int* seq_ids, const int* cache_pos, const int* block_table, int sequences,
                   int max_blocks, void* codes, float* scales, int num_blocks, int T, int Hq, int Hkv, int D,

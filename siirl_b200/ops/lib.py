@@ -32,7 +32,7 @@ _KERNELS_PER_CALL = {"sb_rmsnorm_bwd": 2, "sb_grpo_group_adv": 2, "sb_grpo_scan_
 # Arguments of entry points that single steps call most, one letter each (p: address, i: int, l: 64 bits, f: float): they are
 # then passed as plain numbers, which saves an object for each.
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
-_ARGUMENTS = {"sb_kv8_append": "piplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
+_ARGUMENTS = {"sb_kv8_append": "plplippiiiipppppiippiiiiip", "sb_kv8_decode": "plppippippppiiiifpp",
               "sb_capture_id": "p", "sb_kv8_chunks": "plippipiipppiplppiiifpp"}
 
 

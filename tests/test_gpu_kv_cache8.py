@@ -735,3 +735,22 @@ def test_engine_chunks_and_reused_blocks_follow_from_the_cache():
     want, probs = oracle.engine_by_hand(model, eng._logits, prompt, [64, 72], steps)
     assert got.token_ids == want and all(abs(a - b) < 1e-4 for a, b in zip(got.logprobs, probs))
     lib.check_status()
+
+
+def test_append_to_rows_that_are_far_apart():
+    """Two rows 2^31 + 8 numbers apart: the distance does not fit 32 bits."""
+    hq, hkv, d = 4, 2, 64
+    width, far = (hq + 2 * hkv) * d, 2 ** 31 + 8
+    if torch.cuda.mem_get_info()[0] < 3 * far:
+        pytest.skip("4 GB of rows")
+    cache, table = _gpu(_random_cache(3, hkv, d)), torch.tensor([[1], [2]], dtype=torch.int32, device=DEV)
+    other = Cache8(cache.codes.clone(), cache.scales.clone())
+    cos, sin = (x.to(DEV) for x in ref.rope_tables(d, 64, 1e4))
+    at, seq = torch.tensor([7, 30], dtype=torch.int32, device=DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    near = torch.randn(2, width, device=DEV).bfloat16()
+    rows = torch.empty(far + width, dtype=torch.bfloat16, device=DEV).as_strided((2, width), (far, 1))
+    rows.copy_(near)
+    want = kvc.rope_kv_append(near, at, cos, sin, None, seq, at, table, other, hq, hkv, d)
+    got = kvc.rope_kv_append(rows, at, cos, sin, None, seq, at, table, cache, hq, hkv, d)
+    assert torch.equal(got, want) and torch.equal(cache.codes.view(torch.uint8), other.codes.view(torch.uint8))
+    assert torch.equal(cache.scales, other.scales)

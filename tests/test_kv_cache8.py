@@ -182,6 +182,22 @@ def test_chunk_calls_of_threads_do_not_meet_in_a_workspace(monkeypatch):
     assert len(set(places)) == 2 and set(places) > set(inside)
 
 
+def test_arguments_are_passed_as_the_library_declares_them():
+    """Numbers go to these entry points without a ctypes object of their own: a letter that is too narrow would cut them off in
+    silence.  Distances between rows are 64 bits wide."""
+    import pathlib
+    import re
+    from siirl_b200.ops import lib
+    header = (pathlib.Path(lib.__file__).parent.parent / "csrc" / "launchers.h").read_text()
+    for name, letters in lib._ARGUMENTS.items():
+        arguments = [x.strip() for x in re.search(rf"\b{name}\(([^)]*)\)", header).group(1).split(",")]
+        kinds = ["p" if "*" in x or "cudaStream_t" in x else "l" if "long long" in x else "f" if x.startswith("float") else "i"
+                 for x in arguments]
+        assert "".join(kinds) == letters, name
+        for x, kind in zip(arguments, kinds):
+            assert "stride" not in x or kind == "l", (name, x)
+
+
 # ---- the rollout engine -------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def tiny():
