@@ -593,6 +593,7 @@ extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, int rows, co
                              int* status, cudaStream_t stream) {
   sizes[0] = sizes[1] = sizes[2] = 0;
   if (D != 64 && D != 128) return -2;
+  if (max_blocks > 1 << 24) return -4;      // lengths, rounded up to tiles: 32 bits
   if (n > kChunkSeqs || Hq % Hkv || Hq / Hkv > 32 || row_stride % 8 || reinterpret_cast<uintptr_t>(qkv) % 16 || !(scale > 0.f)) return -3;
   long long sum = 0;
   for (int i = 0; i < n; ++i) {

@@ -1103,8 +1103,8 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || reinterpret_cast<uintptr_t>(q) % 4 || reinterpret_cast<uintptr_t>(out) % 16 || max_blocks < 1 || num_blocks < 1) return -3;
-  const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (long long)(max_blocks + 1) / 2 * B * Hkv * 4;
-  if (rows > 0x7fffffffll || tiles > 0x7fffffffll) return -4;
+  const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (max_blocks + 1ll) / 2 * B * Hkv * 4;
+  if (rows > 0x7fffffffll || tiles > 0x7fffffffll || max_blocks > 1 << 24) return -4;      // lengths, rounded up to tiles: 32 bits
   static thread_local bool tl_context_bound = false;
   if (!tl_context_bound) {
     cudaFree(0);

@@ -26,6 +26,7 @@ BLOCK = 64
 LARGEST = 448.0             # of e4m3
 HEAD_DIMS = (64, 128)       # of the kernels; the CPU statements take any
 ROWS = 1024                 # sequences of one launch of the single-token kernel
+TABLE = 2 ** 24             # blocks of a sequence: lengths and what they are rounded up to stay within 32 bits
 CHUNK_BYTES = 2 ** 20       # chunks that need no more take a workspace that is kept
 
 
@@ -123,8 +124,8 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
     T, width = qkv.shape[-2:]
     if width != (n_heads + 2 * n_kv_heads) * head_dim:
         _refuse(f"rows are {(n_heads + 2 * n_kv_heads) * head_dim} wide, got {width}")
-    if seq_ids.shape != (T,) or positions.shape != (T,) or block_table.dim() != 2:
-        _refuse(f"one sequence and position for each of {T} rows, and a table of blocks for each sequence")
+    if seq_ids.shape != (T,) or positions.shape != (T,) or block_table.dim() != 2 or block_table.shape[1] > TABLE:
+        _refuse(f"one sequence and position for each of {T} rows, and a table of at most {TABLE} blocks for each sequence")
     _check(cache, n_heads, n_kv_heads, head_dim, qkv)
     _check_ints(qkv, seq_ids, positions, block_table)
     dev = qkv.get_device()
@@ -245,8 +246,8 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
     if len(shape) != 2 or shape[1] < width or q_rows.stride(1) != 1:
         _refuse(f"query rows are at least {width} wide")
     B, table = shape[0], block_table.shape
-    if seq_lens.shape != (B,) or len(table) != 2 or table[0] < B:
-        _refuse(f"a length and a row of the table for each of {B} rows")
+    if seq_lens.shape != (B,) or len(table) != 2 or table[0] < B or table[1] > TABLE:
+        _refuse(f"a length and a row of the table, of at most {TABLE} blocks, for each of {B} rows")
     if out is None:
         out = torch.empty(B, width, dtype=q_rows.dtype, device=q_rows.device)
     elif out.shape != (B, width) or not out.is_contiguous() or out.dtype != q_rows.dtype or out.get_device() != q_rows.get_device():
@@ -302,8 +303,8 @@ def check_chunks(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Cache
     rows, width = sum(chunk_lens), (n_heads + 2 * n_kv_heads) * head_dim
     if qkv.shape != (rows, width):
         _refuse(f"{rows} rows of {width} numbers, got {tuple(qkv.shape)}")
-    if block_table.dim() != 2:
-        _refuse("a table of blocks for each sequence")
+    if block_table.dim() != 2 or block_table.shape[1] > TABLE:
+        _refuse(f"a table of at most {TABLE} blocks for each sequence")
     slots_held, tokens_held = block_table.shape[0], block_table.shape[1] * BLOCK
     for c, p, s in zip(chunk_lens, prefix_lens, slots):
         if c < 0 or p < 0 or not 0 <= s < slots_held or c + p > tokens_held:
@@ -323,7 +324,7 @@ def chunk_attention(qkv: torch.Tensor, chunk_lens, prefix_lens, slots, cache: Ca
     lists = [array.array("i", v) for v in (chunk_lens, prefix_lens, slots)]
     total = len(lists[0])
     if width != (n_heads + 2 * n_kv_heads) * head_dim or qkv.dtype is not torch.bfloat16 or block_table.dim() != 2 or \
-            total != len(lists[1]) or total != len(lists[2]) or sum(lists[0]) != rows:
+            block_table.shape[1] > TABLE or total != len(lists[1]) or total != len(lists[2]) or sum(lists[0]) != rows:
         check_chunks(qkv, *lists, cache, block_table, n_heads, n_kv_heads, head_dim)
     dev = qkv.get_device()
     if dev != torch._C._cuda_getDevice():

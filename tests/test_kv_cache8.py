@@ -198,6 +198,27 @@ def test_arguments_are_passed_as_the_library_declares_them():
             assert "stride" not in x or kind == "l", (name, x)
 
 
+def test_tables_whose_lengths_pass_32_bits_are_refused():
+    """More than 2^24 blocks: 64 times their number, rounded up, is not sure to fit."""
+    import ctypes
+    from siirl_b200.ops import lib
+    hq, hkv, d = 2, 1, 64
+    cache, table = Cache8.zeros(2, hkv, d), torch.zeros(1, 2 ** 24 + 1, dtype=torch.int32)
+    q, one = torch.randn(1, (hq + 2 * hkv) * d), torch.ones(1, dtype=torch.int32)
+    for call in (lambda: kvc.decode_attention(q, cache, one, table, hq, hkv, d),
+                 lambda: kvc.kv_append(q, one * 0, one, table, cache, hq, hkv, d),
+                 lambda: kvc.prefill_attention_with_prefix(q, [1], [3], [0], cache, table, hq, hkv, d)):
+        with pytest.raises(ValueError, match="8-bit cache"):
+            call()
+    # the library by itself, before it looks at anything else
+    L, sizes, lists = lib.get_lib(), (ctypes.c_longlong * 3)(), (ctypes.c_int * 2)(1, 0)
+    for blocks in (2 ** 24 + 1, 2 ** 25, 2 ** 31 - 1):
+        assert L.sb_kv8_decode(16, 256, 16, 16, 2, 16, 16, blocks, 16, 16, 16, 16, 1, hq, hkv, d, 0.1, 16, 0) == -4
+        at = ctypes.addressof(lists)
+        assert L.sb_kv8_chunks(16, 256, 1, 16, 16, 2, 16, 1, blocks, at, at, at + 4, 1, 16, 0,
+                               ctypes.addressof(sizes), 16, hq, hkv, d, 0.1, 16, 0) == -4
+
+
 # ---- the rollout engine -------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def tiny():
