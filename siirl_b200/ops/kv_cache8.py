@@ -204,7 +204,7 @@ def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
     with torch.cuda.device(codes.get_device()):
         _lib.check(_lib.get_lib().sb_kv8_copy_blocks(
             _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(src), _lib.ptr(dst), src.numel(), codes.shape[0], 2 * codes.shape[2],
-            ctypes.c_longlong(codes[0].numel()), _lib.stream()), "sb_kv8_copy_blocks")
+            ctypes.c_longlong(codes.shape[2:].numel() * 2), _lib.stream()), "sb_kv8_copy_blocks")
 
 
 # ---- workspaces ---------------------------------------------------------------------------------
@@ -266,6 +266,8 @@ def decode_attention(q_rows: torch.Tensor, cache: Cache8, seq_lens: torch.Tensor
         return out
     if q_rows.dtype is not torch.bfloat16 or out.data_ptr() % 16:
         _refuse("query rows are bf16, and the output starts on a 16-byte boundary")
+    if not table[1] or not cache.codes.shape[0]:
+        return out.zero_()      # nothing to be seen
     dev = q_rows.get_device()
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):

@@ -754,3 +754,21 @@ def test_append_to_rows_that_are_far_apart():
     got = kvc.rope_kv_append(rows, at, cos, sin, None, seq, at, table, cache, hq, hkv, d)
     assert torch.equal(got, want) and torch.equal(cache.codes.view(torch.uint8), other.codes.view(torch.uint8))
     assert torch.equal(cache.scales, other.scales)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (28, 4, 128)])
+def test_calls_without_a_table_or_without_blocks(hq, hkv, d):
+    """A table of no blocks, a cache of none: nothing is seen, by single tokens as on the CPU."""
+    q, i = torch.randn(3, hq * d, device=DEV).bfloat16(), lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    cache, none = _gpu(_random_cache(2, hkv, d)), Cache8.zeros(0, hkv, d, DEV)
+    table, lens = torch.zeros(3, 2, dtype=torch.int32, device=DEV), i(0, 5, 128)
+    for c, t, n in ((cache, table[:, :0].contiguous(), lens), (cache, table[:, :0].contiguous(), i(0, 0, 0)), (none, table, lens)):
+        out = torch.full((3, hq * d), 7.0, device=DEV, dtype=torch.bfloat16)
+        assert kvc.decode_attention(q, c, n, t, hq, hkv, d, out=out) is out and not out.any()
+    rows = torch.randn(2, (hq + 2 * hkv) * d, device=DEV).bfloat16()
+    kept = rows.clone()
+    kvc.kv_append(rows, i(0, 1), i(3, 4), table, none, hq, hkv, d)
+    kvc.kv_append(rows, i(0, 1), i(3, 4), table[:, :0].contiguous(), cache, hq, hkv, d)
+    kvc.kv_copy_blocks(none, i(0), i(1))
+    assert torch.equal(rows, kept)
+    lib.check_status()
