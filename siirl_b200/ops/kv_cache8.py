@@ -191,16 +191,20 @@ def append(qkv: torch.Tensor, rope, seq_ids: torch.Tensor, positions: torch.Tens
 
 
 def copy_blocks(cache: Cache8, src: torch.Tensor, dst: torch.Tensor) -> None:
-    """Blocks ``src[i]`` with their scales to ``dst[i]``."""
+    """Blocks ``src[i]`` with their scales to ``dst[i]``; pairs that name no block are left out.  The destinations differ from one
+    another and from all sources: pairs are copied at the same time."""
     codes, scales = cache
-    if not codes.is_cuda:
-        codes.view(torch.uint8)[dst.long()] = codes.view(torch.uint8)[src.long()]
-        scales[dst.long()] = scales[src.long()]
-        return
-    _check(cache, codes.shape[2], codes.shape[2], codes.shape[4], codes)
+    heads = codes.shape[2] if codes.dim() == 5 else 0
+    _check(cache, heads, heads, codes.shape[-1], codes)
     _check_ints(codes, src, dst)
     if src.shape != dst.shape or src.dim() != 1:
         _refuse("as many sources as destinations")
+    if not codes.is_cuda:
+        ok = (src >= 0) & (src < len(codes)) & (dst >= 0) & (dst < len(codes))
+        src, dst = src[ok].long(), dst[ok].long()
+        codes.view(torch.uint8)[dst] = codes.view(torch.uint8)[src]
+        scales[dst] = scales[src]
+        return
     with torch.cuda.device(codes.get_device()):
         _lib.check(_lib.get_lib().sb_kv8_copy_blocks(
             _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(src), _lib.ptr(dst), src.numel(), codes.shape[0], 2 * codes.shape[2],

@@ -107,6 +107,19 @@ def test_copied_blocks_bring_their_scales():
     assert torch.equal(cache.dequantize(torch.tensor([0, 4])), want)
 
 
+def test_copies_that_name_no_block_are_left_out():
+    cache = Cache8.zeros(5, 2, 32)
+    cache.codes.view(torch.uint8).copy_(torch.randint(0, 120, cache.codes.shape))
+    cache.scales.copy_(2.0 ** torch.randint(-9, 9, cache.scales.shape))
+    want = cache.dequantize(torch.tensor([0, 1, 2, 3, 1]))
+    i = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    kvc.kv_copy_blocks(cache, i(1, -1, 2, 3, 5), i(4, 0, -1, 99, 1))
+    assert torch.equal(cache.dequantize(torch.arange(5)), want)
+    for src, dst in ((i(1), i(2, 3)), (i(1).long(), i(2).long()), (i(1)[None], i(2)[None])):
+        with pytest.raises(ValueError, match="8-bit cache"):
+            kvc.kv_copy_blocks(cache, src, dst)
+
+
 def test_refusals():
     hq, hkv, d = 4, 2, 64
     cache = Cache8.zeros(4, hkv, d)
