@@ -327,6 +327,9 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int row = tid, at = row / p.rep, head = row - at * p.rep;
     const uint32_t lane_off = (uint32_t)(warp * 32) << 16, tmem_o = tmem_base + lane_off + 2 * KV;
     const int qpos = first + at;      // position within the sequence
+    // Of a row of the tile that is none of the chunk's, shared memory has other numbers, which rows of its warp must not feel: their
+    // references are raised together
+    const bool row_valid = at < p.span && qpos < total;
     const float sc = p.scale_log2;
     float m_ref = -INFINITY;          // reference of the weights, scaled
     float2 l_run[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -351,7 +354,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < KV; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i / 32][i % 32]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+      const float top = row_valid ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc : -INFINITY;
       if (__any_sync(0xffffffffu, top > m_ref + 8.f)) {
         // The barrier of the scores also said that the products of the tile before the last one are done: o_step is at most one
         // phase behind
@@ -411,7 +414,6 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // ---- O / l -> bf16, or the share's normalised result (TMEM loads are warp-collective; only the stores are predicated) ----
     if (ok) {
       tc_fence_after();
-      const bool row_valid = at < p.span && qpos < total;
       // 0: all scores are -inf, of a share's keys that the row does not see, or of all its keys, where 0 / 0 is soft-max's answer.
       // Scores that are NaN do not raise the reference, but make the sum NaN
       const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y), inv_l = 1.f / l;

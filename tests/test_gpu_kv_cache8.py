@@ -772,3 +772,31 @@ def test_calls_without_a_table_or_without_blocks(hq, hkv, d):
     kvc.kv_copy_blocks(none, i(0), i(1))
     assert torch.equal(rows, kept)
     lib.check_status()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (5, 1, 128)])
+@pytest.mark.parametrize("new,old", [((130, 41), (2500, 700)), ((2048, 3), (6000, 40)), ((9, 9), (130, 60))])
+def test_chunks_repeat_themselves_whatever_ran_before(hq, hkv, d, new, old):
+    """To the bit, after kernels that leave other numbers in shared memory; and whatever the other sequences' queries are: tiles of
+    128 rows are not full where the heads of a kv head do not divide 128, or a sequence ends."""
+    total = [a + b for a, b in zip(new, old)]
+    need = [(n + 63) // 64 for n in total]
+    cache, table, first = _random_cache(sum(need), hkv, d), torch.full((2, max(need)), -1, dtype=torch.int32), 0
+    for i, k in enumerate(need):
+        table[i, :k] = torch.arange(first, first + k)
+        first += k
+    g, table = _gpu(cache), table.to(DEV)
+    rows = (3 * torch.randn(sum(new), (hq + 2 * hkv) * d)).bfloat16().to(DEV)
+
+    def call(x):
+        return kvc.prefill_attention_with_prefix(x, new, old, [0, 1], g, table, hq, hkv, d)
+    want = call(rows)
+    for i, size in enumerate((1.0, 30.0, 1000.0, 0.01)):
+        call((size * torch.randn(rows.shape)).bfloat16().to(DEV))
+        assert torch.equal(call(rows), want), i
+    for i in range(2):
+        other = rows.clone()
+        other[new[0] * i:new[0] + new[1] * i] *= 100
+        keep = slice(new[0], None) if i == 0 else slice(0, new[0])
+        assert torch.equal(call(other)[keep], want[keep]), i
+    lib.check_status()
