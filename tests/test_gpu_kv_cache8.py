@@ -800,3 +800,51 @@ def test_chunks_repeat_themselves_whatever_ran_before(hq, hkv, d, new, old):
         keep = slice(new[0], None) if i == 0 else slice(0, new[0])
         assert torch.equal(call(other)[keep], want[keep]), i
     lib.check_status()
+
+
+def test_appended_chunks_in_graphs_that_take_turns():
+    """Appending and chunks, with a workspace that is kept and with one of the call's own, captured twice and replayed on new
+    numbers between calls outside of the graphs, and from another stream."""
+    hq, hkv, d = 14, 2, 64
+    cos, sin = (x.to(DEV) for x in ref.rope_tables(d, 4200, 1e4))
+    width, i32 = (hq + 2 * hkv) * d, dict(dtype=torch.int32, device=DEV)
+    lists = [([9], [130]), ([300, 2], [4000, 65])]
+    calls = []
+    for new, old in lists:
+        need = [(a + b + 63) // 64 for a, b in zip(new, old)]
+        table, first = torch.full((len(new), max(need)), -1, dtype=torch.int32), 0
+        for i, k in enumerate(need):
+            table[i, :k] = torch.arange(first, first + k)
+            first += k
+        at = torch.cat([torch.arange(b, b + a) for a, b in zip(new, old)]).to(**i32)
+        seq = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new)).to(**i32)
+        held, table, rows = _gpu(_random_cache(first, hkv, d)), table.to(DEV), torch.zeros(sum(new), width, device=DEV).bfloat16()
+
+        def call(rows, cache, new=new, old=old, at=at, seq=seq, table=table):
+            kvc.rope_kv_append(rows, at, cos, sin, None, seq, at, table, cache, hq, hkv, d)
+            return kvc.prefill_attention_with_prefix(rows, new, old, list(range(len(new))), cache, table, hq, hkv, d)
+        call(rows.clone(), Cache8(*(x.clone() for x in held)))
+        calls.append((call, rows, held))
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, [call(rows, held) for call, rows, held in calls]))
+    side = torch.cuda.Stream()
+    for step, n in enumerate((0, 1, 1, 0)):
+        fresh = [torch.randn(rows.shape, device=DEV).bfloat16() for _, rows, _ in calls]
+        other = [Cache8(held.codes.clone(), held.scales.clone()) for _, _, held in calls]
+        for (_, rows, _), x in zip(calls, fresh):
+            rows.copy_(x)
+        want = [call(x, c) for (call, _, _), x, c in zip(calls, fresh, other)]
+        if step % 2:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graphs[n][0].replay()
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            graphs[n][0].replay()
+        for (_, rows, held), got, x, y, c in zip(calls, graphs[n][1], want, fresh, other):
+            assert torch.equal(got, x) and torch.equal(rows, y) and torch.equal(held.scales, c.scales)
+            assert torch.equal(held.codes.view(torch.uint8), c.codes.view(torch.uint8))
+    lib.check_status()
