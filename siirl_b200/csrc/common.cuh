@@ -477,6 +477,15 @@ inline int launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, siz
   return (int)e;
 }
 
+// The driver's tensor-map encoder needs a current context on the calling thread; threads that only ever launched through torch
+// (autograd workers) may not have one yet.  cudaSetDevice binds it also while a stream is captured, where a call of cudaFree
+// would end the capture.
+inline void bind_context() {
+  static thread_local bool bound = false;
+  int dev = 0;
+  if (!bound && cudaGetDevice(&dev) == cudaSuccess) bound = cudaSetDevice(dev) == cudaSuccess;
+}
+
 // ---------------------------------------------------------------------------------------
 // misc numerics
 // ---------------------------------------------------------------------------------------

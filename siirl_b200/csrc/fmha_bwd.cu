@@ -640,11 +640,7 @@ extern "C" int sb_fmha_bwd(const void* qkv, const void* out, const void* d_out, 
   if (num_tiles == 0 || T == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (head_splits < 1 || head_splits > Hq / Hkv || (head_splits > 1 && !dkv_accum)) return -3;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const long long width = (long long)(Hq + 2 * Hkv) * D;
   const long long qwidth = (long long)Hq * D;
   CUtensorMap mqkv, mdo;

@@ -612,11 +612,7 @@ extern "C" int sb_kv8_chunks(const void* qkv, long long row_stride, int rows, co
   const long long parts = c.splits > 1 ? (long long)c.s.tiles * Hkv * c.splits * 128 : 0;
   sizes[0] = kv_bytes + marks_bytes + parts * (D + 1) * 4;
   if (sizes[0] > ws_bytes) return -6;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   CUtensorMap mq, mkv;
   r = make_tensor_map_bf16_3d(&mq, qkv, D, Hq, sum, D, row_stride, 64, Hq / Hkv, c.span);
   if (r) return r;

@@ -459,11 +459,7 @@ extern "C" int sb_fmha_decode(const void* q, int row_stride, const void* cache, 
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (Hq % Hkv || Hq / Hkv > 32) return -3;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   CUtensorMap mc;
   int r = make_tensor_map_bf16_2d(&mc, cache, D, num_blocks * 2 * Hkv * kBlk, D, 64, kBlk);
   if (r) return r;

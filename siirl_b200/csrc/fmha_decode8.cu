@@ -1105,11 +1105,7 @@ extern "C" int sb_kv8_decode(const void* q, long long row_stride, const void* co
   if (B > kQ8Rows || Hq % Hkv || Hq / Hkv > 32 || row_stride % 2 || reinterpret_cast<uintptr_t>(q) % 4 || reinterpret_cast<uintptr_t>(out) % 16 || max_blocks < 1 || num_blocks < 1) return -3;
   const long long rows = (long long)num_blocks * 2 * Hkv * (D / 2), tiles = (max_blocks + 1ll) / 2 * B * Hkv * 4;
   if (rows > 0x7fffffffll || tiles > 0x7fffffffll || max_blocks > 1 << 24) return -4;      // lengths, rounded up to tiles: 32 bits
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   // rows of 128 bytes, as 64 16-bit numbers; a box is a cache block of one head
   CUtensorMap mc;
   const int r = make_tensor_map_bf16_2d(&mc, codes, 64, rows, 64, 64, D / 2);

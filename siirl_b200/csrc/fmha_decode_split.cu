@@ -751,11 +751,7 @@ extern "C" int sb_fmha_decode_split(const void* q, int row_stride, const void* c
   if (B == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (Hq % Hkv || Hq / Hkv > 32 || row_stride % D) return -3;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const int rep = Hq / Hkv;
   CUtensorMap mc, mq;
   int r = make_tensor_map_bf16_2d(&mc, cache, D, num_blocks * 2 * Hkv * kSBlk, D, 64, kSBlk);
@@ -805,11 +801,7 @@ extern "C" int sb_attn_window_decode(const void* params, const int* seq_lens, fl
   if (w.T == 0) return 0;
   const int chunks = sb_attn_window_decode_chunks(params);
   if (chunks < 0) return -2;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const int rep = w.Hq / w.Hkv;
   const __nv_bfloat16* cache = reinterpret_cast<const __nv_bfloat16*>(w.cache);
   CUtensorMap mk, mv, mq;

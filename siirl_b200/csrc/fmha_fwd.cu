@@ -331,11 +331,7 @@ extern "C" int sb_fmha_fwd(const void* qkv, void* out, float* lse, const int* ti
   if (num_tiles == 0 || T == 0) return 0;
   if (D != 64 && D != 128) return -2;
   if (tile_rows != 128 && tile_rows != 256) return -3;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const long long width = (long long)(Hq + 2 * Hkv) * D;
   CUtensorMap mq, mkv;
   int r = make_tensor_map_bf16_2d(&mq, qkv, width, T, width, 64, 128);

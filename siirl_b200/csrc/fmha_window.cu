@@ -560,11 +560,7 @@ extern "C" int sb_attn_window_prefill(const void* params, const int* tile_row, c
       p.q_off % 8 || p.out_stride % 8 || p.out_off % 8 || p.block_elems % 8 || ((uintptr_t)p.out & 15) ||
       p.kv_mode == kLatent || p.gate_stride % 8 || ((uintptr_t)p.gate & 15) || (p.rel && (p.rel_n < 1 || p.bias_exp > 0.f)) || !pool_valid(p))
     return -2;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(p.x);
   const __nv_bfloat16* cache = reinterpret_cast<const __nv_bfloat16*>(p.cache);
   CUtensorMap mq, mk, mv;

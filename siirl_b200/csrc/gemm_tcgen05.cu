@@ -1104,13 +1104,7 @@ static int gemm_impl(const void* A, const void* B, void* C, const void* bias, in
     if (((uintptr_t)C & 15) || (ldc % 4) || (N % 4)) return -3;
   }
   if ((epi == EPI_LMSTAT || epi == EPI_DLOGITS) && !lm) return -3;
-  // The driver-API tensor-map encoder needs a current context on the calling thread; threads
-  // that only ever launched through torch (autograd workers) may not have one bound yet.
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   int BN = tile_n;
   if (BN != 128 && BN != 256) {
     // 256-wide tiles halve the A traffic per FLOP and measured 1.5x faster than 128-wide ones on

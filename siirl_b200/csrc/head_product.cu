@@ -229,11 +229,7 @@ extern "C" int sb_head_product(const void* params, int* status, cudaStream_t str
   if (p.H > 65535 || p.T > 128 * 65535 || N % 8 || p.b_cols % 8 || p.a_head % 8 || p.a_row % 8 || p.c_row % 8 ||
       p.gate_row % 8 || ((uintptr_t)p.a & 15) || ((uintptr_t)p.b & 15) || ((uintptr_t)p.c & 15) || ((uintptr_t)p.gate & 15))
     return -3;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   CUtensorMap ma, mb;
   int r = make_tensor_map_bf16_3d(&ma, p.a, K, p.H, p.T, p.a_head, p.a_row, 64, 1, 128);
   if (r) return r;

@@ -667,11 +667,7 @@ extern "C" int sb_latent_decode(const void* params, float* ws_o, float* ws_stat,
   if (w.T <= 0) return 0;
   const int groups = sb_latent_decode_groups(w.H, w.R);
   if (!groups || w.T > kLMaxRows || ((uintptr_t)w.qa & 15) || ((uintptr_t)w.cache & 15)) return -2;
-  static thread_local bool tl_context_bound = false;
-  if (!tl_context_bound) {
-    cudaFree(0);
-    tl_context_bound = true;
-  }
+  bind_context();
   const LdLayout L(w.H, w.R, w.T);
   CUtensorMap mc;
   int r = make_tensor_map_bf16_3d(&mc, w.cache, w.R, kLBlk, w.num_blocks, w.R, (long long)kLBlk * w.R, 64, kLBlk, 1);

@@ -848,3 +848,29 @@ def test_appended_chunks_in_graphs_that_take_turns():
             assert torch.equal(got, x) and torch.equal(rows, y) and torch.equal(held.scales, c.scales)
             assert torch.equal(held.codes.view(torch.uint8), c.codes.view(torch.uint8))
     lib.check_status()
+
+
+def test_a_thread_whose_first_calls_are_captured():
+    """Nothing that a thread's first call sets up may end a capture."""
+    import threading
+    hq, hkv, d = 14, 2, 64
+    cache, table, q, n = _decode([300, 5], hq, hkv, d, 8)
+    g, q, n, table = _gpu(cache), q.to(DEV), n.to(DEV), table.to(DEV)
+
+    def calls():
+        return [kvc.decode_attention(q, g, n, table, hq, hkv, d), kvc.prefill_attention_with_prefix(q, [2], [3], [0], g, table, hq, hkv, d)]
+    want, got = calls(), []
+
+    def work():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = calls()
+        graph.replay()
+        torch.cuda.synchronize()
+        got.extend(x.clone() for x in held)
+    torch.cuda.synchronize()
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    lib.check_status()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, want))
