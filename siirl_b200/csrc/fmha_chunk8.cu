@@ -20,11 +20,11 @@
 // The reference of a row's weights is raised only when its maximum grows by 2^8, so the output is rarely rescaled.
 // The exponentials (16 a cycle and SM) take as long as the products, at D = 64 twice as long: every fourth pair, at D = 64 every
 // second one, is computed on the fused-multiply-add units (2048 rows of one prompt, 28 / 4 heads: 155 us, 162 without; 4 sequences
-// of up to 2000 rows, 14 / 2 heads, D = 64: 253, 266 without): 2^x = 2^n 2^f with n the nearest integer and a cubic in f,
+// of up to 2000 rows, 14 / 2 heads, D = 64: 254, 266 without): 2^x = 2^n 2^f with n the nearest integer and a cubic in f,
 // |f| <= 1/2, fitted for the smallest largest relative error (7.5e-5, a fiftieth of a bf16 step) by iteratively reweighted
 // least squares.
-// Bound by the tensor cores at the clock that the power limit leaves: 2 sequences of up to 2148 rows behind up to 14,000 tokens: 704 us,
-// 1.22 PFLOP/s, 88 % of what a long run of a library product reaches.
+// Bound by the tensor cores and the power limit: 2 sequences of up to 2148 rows behind up to 14,000 tokens: 704 us in short loops, 1.23
+// PFLOP/s, 75 % of a library product's 1.64; 800 us in long ones, whose clock the limit lowers, 1.08 PFLOP/s, 78 % of its 1.39.
 // Where there are few blocks, the key tiles are split over several, whose results chunk_merge_kernel joins.
 #include <cuda_fp8.h>
 
@@ -472,7 +472,7 @@ fmha_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 }
 
 // Mean of the shares' results, weighted by 2^(log-sum-exp).  A block takes 16 rows, half a warp each: first the largest weight,
-// then all shares at once, so that their reads are under way together (32 shares of 30 rows: 9 us less than one after the other).
+// then all shares at once, so that their reads are under way together.
 template <int D>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkSeqs seqs, ChunkParams p) {
   chain_sync();

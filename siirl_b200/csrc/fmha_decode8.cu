@@ -9,7 +9,9 @@
 //     weight.  e5m2 for its range: thousands of small weights may stand beside one large one whose value is near zero.
 // The block's scales go into the score and into the weight, in 32 bits.  So a block with a large scale and small codes would take
 // the weights' range from the others: a piece whose blocks' value scales are more than 2^16 apart (those below 2^-60 aside) is
-// computed again in 32 bits by the output warps (d8_exact), some ten times slower.
+// computed again in 32 bits by the output warps (d8_exact), at 20 to 30 us for 32 tokens: a call takes a hundred times as long, also
+// where only one sequence needs it, whose heads are one CTA's (256 x 1300-5120, 28 / 4 heads: 14.4 ms with one block of one sequence,
+// 18.4 with one of each, 135 us without; 8 x 20001-32768, 32 / 8: 8.4, 8.8 and 0.074 ms).
 //
 // A tile is 128 rows of 128 bytes: two cache blocks at D = 128; at D = 64, where a row holds two tokens, four.
 //   S^T[row, (token of the row, term, head)] = K Q^T     A = the K tile, B = the terms of all query heads of a kv head
@@ -23,7 +25,9 @@
 // the whole entry leaves a normalised result and its log-sum-exp in a workspace, two slots per CTA, and counts itself; whoever
 // finds that all others have joins them.  A second kernel for that would cost the host as much again as this one.
 // Up to 32 sequences, if there are few tiles, are cut instead into pieces of at most so many tiles that each CTA gets one: a second
-// piece costs a CTA about 1.6 us, a join 3, a tile 0.7 (28 / 4 heads, 300 tokens: 7.2 us whole, 11.0 in equal ranges; 32 x 1000: 11.4 and 15.3).
+// piece costs a CTA about 1.6 us, a join 3, a tile 0.7 (28 / 4 heads, 300 tokens: 7.2 us whole, 11.0 in equal ranges; 32 x 1000: 11.4
+// and 15.3).  32, as a warp's lanes take a sequence each, not because more would not gain: 33 x 300 take 14.4 us where 32 take 8.8,
+// 33 x 1000 16.4 and 12.4.
 // The warps:
 //   0..7   soft-max in two groups, each with an O^T and weights' references of its own.  D = 128: thread = row of the tile, the
 //          first four warps take the even tiles of the range, the others the odd ones, so that two tiles are under way.

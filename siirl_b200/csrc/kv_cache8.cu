@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(256) append8_rows_kernel(Append8Params p, int 
 // keeps the eight angles of its pairs for `per` heads.
 //
 // Bound by memory: 32 / 8 heads, D = 128, 32653 rows (819 MB): 145 us, 5.6 TB/s (with rows held in registers instead of asked for
-// four heads ahead, 177); 28 / 4 heads, 8992 rows of 24 prompts (170 MB): 38 us.
+// four heads ahead, 177); 28 / 4 heads, 8992 rows of 24 prompts (170 MB): 38 us; 421 rows of three partial sums (28 MB): 12.4 us.
 // ---------------------------------------------------------------------------------------
 
 // Eight pairs from element i0 on of one head of a row, not rotated.  bf16 rows are asked for several heads ahead: a thread's
@@ -564,9 +564,10 @@ extern "C" int sb_kv8_append(void* qkv, long long row_stride, const float* slabs
   p.block_table = block_table; p.sequences = sequences; p.max_blocks = max_blocks; p.codes = (uint8_t*)codes;
   p.scales = scales; p.num_blocks = num_blocks; p.T = T; p.Hq = Hq; p.Hkv = Hkv;
   auto on = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  // At most as many rows as sequences: a decoding step, if it is anything, and then the second kernel would go from row to row
-  // (256 rows, 28 / 4 heads, D = 128: 7.4 us against 22.7; 1000: 24 against 28).  More rows come in runs (825 rows of three prompts:
-  // 21.5 against 10.7; 60 rows of one: 7.9 either way).
+  // At most as many rows as the table has sequences may be a decoding step, where the second kernel would go from row to row (256
+  // rows, 28 / 4 heads, D = 128: 7.4 us against 22.7; 1000: 24 against 28).  More rows come in runs (60 rows of one prompt: 7.9 either
+  // way).  What the rows are is not known here: prompts of more than 128 rows but no more than the table has sequences take the
+  // first kernel as well, which is slower for them (three prompts, table of 1024: 460 rows 13.5 us against 9.2, 886: 21.0 against 10.7).
   if (T <= 128 || T <= sequences || row_stride % 8 || !on(qkv) || !on(slabs) || slab_stride % 4 || !on(cos_tab) || !on(sin_tab)) {
     const int rows = 1024 / D;
     const long long kv = (long long)((T + rows - 1) / rows) * 2 * Hkv;

@@ -181,8 +181,8 @@ def prefill_attention(qkv: torch.Tensor, info, prefix_lens, slots, cache_layer: 
     """Attention of a prefill batch: ``info`` (:class:`~siirl_b200.ops.attention.SeqInfo`) has the new rows, ``prefix_lens`` the
     earlier tokens of each sequence (None: of none), ``slots`` their places in the table.  Sequences without earlier tokens
     attend to the keys and values of their rows, the others to the cache.  What a 16-bit cache holds are the rows' own, so one call
-    takes both kinds; an 8-bit cache has rounded them, and each kind gets a call, so that no prompt's result depends on what it was
-    admitted with."""
+    takes both kinds; an 8-bit cache has rounded them, and each kind gets a call, so that whether a prompt meets rounded keys
+    does not depend on what it was admitted with."""
     from .attention import attention_packed
     shape = (n_heads, n_kv_heads, head_dim)
     kinds = ([], [])

@@ -3,7 +3,8 @@
 :class:`Cache8` stands where the functions of :mod:`siirl_b200.ops.kv_cache` take the cache of a layer (``rope_kv_append``,
 ``kv_append``, ``decode_attention``, ``prefill_attention_with_prefix``, ``kv_copy_blocks``); those call what is here.  It holds
 ``codes [num_blocks, 2, Hkv, 64, D]`` (e4m3; keys, then values) and ``scales [num_blocks, 2, Hkv]`` (fp32): a cached value is
-code times scale, half the bytes of the bf16 cache.
+code times scale, half the bytes of the bf16 cache.  Scales are powers of two; of others, which only a caller's own cache can
+have, chunks round the values to bf16.
 
 Appending keeps each scale at the smallest power of two (at least 2^-126) with which every finite value that its block and
 head have met fits e4m3's range, ``|x| <= 448 * scale``.  New values are rounded once, from the rotated 32-bit ones, to the
@@ -42,7 +43,7 @@ class Cache8(NamedTuple):
                    torch.zeros(num_blocks, 2, n_kv_heads, dtype=torch.float32, device=device))
 
     def dequantize(self, blocks: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """Values ``[len(blocks), 2, Hkv, 64, D]`` of some blocks; exact in bf16, too."""
+        """Values ``[len(blocks), 2, Hkv, 64, D]`` of some blocks; exact in bf16, too, where the scales are powers of two."""
         codes = self.codes.view(torch.uint8)[blocks].view(torch.float8_e4m3fn)
         return (codes.float() * self.scales[blocks][..., None, None]).to(dtype)
 
