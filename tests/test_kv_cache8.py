@@ -372,3 +372,47 @@ def test_engine_refusals(tiny):
     hybrid = build_model(get_config("tiny-domavik"), dtype=torch.float32, device="cpu", seed=0)
     with pytest.raises(ValueError, match="hybrid"):
         RolloutEngine(hybrid, max_num_seqs=8, max_model_len=64, num_blocks=8, kv_cache_dtype="fp8")
+
+
+def _tensor_parallel_rank(rank, where, results):
+    """Rank of test_tensor_parallel_engines_keep_their_heads_in_8_bits."""
+    import torch.distributed as dist
+    from siirl_b200.engine.rollout.native_engine import RolloutEngine, SamplingParams
+    from siirl_b200.models.config import get_config
+    from siirl_b200.models.decoder import build_model
+    from siirl_b200.models.tp_decoder import TPDecoder
+    from siirl_b200.parallel.tensor_parallel import TPContext
+    torch.set_num_threads(2)
+    dist.init_process_group("gloo", init_method=f"file://{where}", rank=rank, world_size=2)
+    cfg = get_config("tiny")
+    model = build_model(cfg, dtype=torch.float32, device="cpu", seed=3)
+    view = TPDecoder(model, TPContext(dist.group.WORLD, None, max_rows=1024, max_cols=cfg.hidden_size, max_tiles=64))
+    sp = SamplingParams(n=1, temperature=0.0, max_new_tokens=5, ignore_eos=True)
+    known, whole, outs = [list(range(7, 7 + n)) for n in (150, 70)], list(range(30, 130)), []
+    for m in (model, view):
+        eng = RolloutEngine(m, max_num_seqs=8, max_model_len=256, num_blocks=40, kv_cache_dtype="fp8")
+        outs.append(eng.generate(known, sp) + eng.generate([known[0] + [3, 4], whole, known[1] + [3, 4]], sp))
+        assert eng.stats["prefix_cache_hit_tokens"] == 128 + 64
+    results.put((rank, eng.cache[0].codes.shape[2] == cfg.num_kv_heads // 2,
+                 [(o.token_ids, w.token_ids, max(abs(a - b) for a, b in zip(o.logprobs, w.logprobs))) for o, w in zip(*outs)]))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_tensor_parallel_engines_keep_their_heads_in_8_bits(tmp_path):
+    """Two ranks with half of the heads each, prompts with and without reused blocks: what one rank with all heads gets, as scales are
+    a head's own."""
+    import torch.multiprocessing as mp
+    ctx = mp.get_context("spawn")
+    results = ctx.Queue()
+    ranks = [ctx.Process(target=_tensor_parallel_rank, args=(i, str(tmp_path / "meet"), results)) for i in range(2)]
+    for r in ranks:
+        r.start()
+    got = [results.get(timeout=240) for _ in ranks]
+    for r in ranks:
+        r.join(60)
+        assert r.exitcode == 0
+    for _, halved, pairs in got:
+        assert halved and len(pairs) == 5
+        for mine, one, off in pairs:
+            assert mine == one and off < 1e-4
